@@ -19,9 +19,10 @@ ABI_VERSION = 1
 BF16, F16, F32 = 0, 1, 2
 W_UINT4, W_INT8 = 0, 1   # enum psq_weight_kind
 Q8_I8, Q8_E4M3, Q8_E5M2 = 0, 1, 2   # enum psq_q8_weights
+CODES_NONE, CODES_I8, CODES_E4M3 = 0, 1, 2   # enum psq_codes
 
 # Every exported entry point: name -> (restype, argtypes).  Mirrors include/psquant.h.
-_P, _I64, _I = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
+_P, _I64, _I, _F = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
 SIGNATURES = {
     "psq_abi_version": (_I, []),
     "psq_last_error": (ctypes.c_char_p, []),
@@ -50,6 +51,12 @@ SIGNATURES = {
     "psq_dequant_i8_rows": (_I, [_P, _P, _I64, _I64, _I, _P, _I, _P]),
     "psq_dequant_fp8": (_I, [_P, _P, _I, _I64, _I64, _P, _I, _P]),
     "psq_dequant_e5m2": (_I, [_P, _P, _I, _I64, _I64, _P, _I, _P]),
+    "psq_add_rms_norm": (_I, [_I, _P, _I, _I64, _P, _I64, _P, _I, _F, _P, _I64, _I, _P, _P, _I64, _P, _I64, _I64, _P]),
+    "psq_kv_write": (_I, [_I, _P, _P, _I, _I64, _I64, _I64, _I64, _P, _I64, _I, _I, _P, _P, _P, _P, _I64, _I, _P]),
+    "psq_kv_read": (_I, [_I, _P, _I64, _P, _P, _I, _P, _P, _I64, _I, _I, _I, _P, _P, _I, _P]),
+    "psq_paged_attention_workspace_bytes": (_I64, [_I, _I64, _I, _I, _I, _I64]),
+    "psq_paged_attention": (_I, [_I, _P, _I, _I64, _I64, _P, _P, _P, _P, _I64, _I, _P, _I64, _I64, _P, _I64, _I, _I, _I, _F,
+                                 _I64, _I64, _P, _P, _P, _I64, _P]),
     "psq_flag_nonfinite": (_I, [_P, _I, _I64, _P, ctypes.c_uint64, _P]),
 }
 

@@ -485,6 +485,190 @@ def dequant_fp8(q, w_scale, out_dtype=torch.bfloat16, e5m2=None):
     return out
 
 
+# ------------------------------------------------------------------ text decoder
+# What a decoder layer does between its quantized linears.  The checks are written out flat and the
+# addresses passed as integers: at one token the host call is most of the time.
+CODES = {None: _native.CODES_NONE, "none": _native.CODES_NONE, "int8": _native.CODES_I8, "fp8": _native.CODES_E4M3}
+_CODE_DTYPES = {torch.int8: _native.CODES_I8, torch.float8_e4m3fn: _native.CODES_E4M3,
+                torch.bfloat16: _native.CODES_NONE, torch.float16: _native.CODES_NONE}
+_HALF = (torch.bfloat16, torch.float16)
+
+
+def _one_device(name, first, *others):
+    """RuntimeError unless all tensors (None apart) are on the GPU of the first."""
+    device = first.device
+    for t in (first,) + others:
+        if t is not None and (t.device != device or device.type != "cuda"):
+            raise RuntimeError(f"{name}: psquant kernels need tensors of one GPU (got {device}, {t.device})")
+
+
+def add_rms_norm(x, weight, eps=1e-6, residual=None, codes=None, rot_group=0, static_scale=None):
+    """RMS norm of h = x + residual (rounded to x's dtype), rows as the operand of gemm_i8 / gemm_fp8.
+
+    x, residual: [M, K] bf16/f16 on the GPU, K a multiple of 16 up to 32768; weight: [K] bf16/f16/f32.
+    codes: None (rows in x's dtype), "int8" or "fp8" (e4m3fn); rot_group: ConvRot, as quantize_rows;
+    static_scale: fp32 tensor with one element in the place of the rows' own scales.
+    Returns (rows [M, K], scale [M] fp32 or None, h or None when there is no residual).
+    """
+    _one_device("add_rms_norm", x, weight, residual)
+    code = CODES.get(codes)
+    if code is None:
+        raise ValueError(f"add_rms_norm: unknown codes {codes!r}")
+    if x.dtype not in _HALF:
+        raise TypeError(f"add_rms_norm: rows must be bf16/f16, got {x.dtype}")
+    if static_scale is not None and not code:
+        raise ValueError("add_rms_norm: a static scale needs codes")
+    x = _rows2d(x)
+    M, K = x.shape
+    if weight.numel() != K:
+        raise ValueError(f"add_rms_norm: weight has {weight.numel()} elements, expected {K}")
+    if not weight.is_contiguous() or weight.data_ptr() % 16:
+        weight = torch.empty(K, dtype=weight.dtype, device=weight.device).copy_(weight.reshape(-1))
+    h, ldr = None, 0
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise ValueError(f"add_rms_norm: residual {tuple(residual.shape)} {residual.dtype} does not match the rows")
+        residual = _rows2d(residual)
+        ldr = residual.stride(0)
+        h = torch.empty(M, K, dtype=x.dtype, device=x.device)
+    scale, st = None, None
+    if code:
+        out = torch.empty(M, K, dtype=torch.int8 if code == _native.CODES_I8 else torch.float8_e4m3fn, device=x.device)
+        scale = torch.empty(M, dtype=torch.float32, device=x.device)
+        if static_scale is not None:
+            st = static_scale.to(device=x.device, dtype=torch.float32).reshape(-1)[:1].contiguous()
+    else:
+        out = torch.empty(M, K, dtype=x.dtype, device=x.device)
+    _launch("add_rms_norm", _native.lib().psq_add_rms_norm, code, x.data_ptr(), _DT[x.dtype], x.stride(0),
+            None if residual is None else residual.data_ptr(), ldr, weight.data_ptr(), _dt(weight, "weight"), eps,
+            None if h is None else h.data_ptr(), K, int(rot_group or 0), None if st is None else st.data_ptr(),
+            out.data_ptr(), K, None if scale is None else scale.data_ptr(), M, K, _stream(x))
+    return out, scale, h
+
+
+def _kv_pools(name, k_cache, v_cache, k_scale, v_scale):
+    """(codes, pages, kv heads, page size, head dim) of a paged cache's pools, checked."""
+    code = _CODE_DTYPES.get(k_cache.dtype)
+    if code is None or v_cache.dtype is not k_cache.dtype:
+        raise TypeError(f"{name}: unsupported cache dtypes {k_cache.dtype}, {v_cache.dtype}")
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape:
+        raise ValueError(f"{name}: the pools must both be [pages, kv heads, page size, head dim], got "
+                         f"{tuple(shape)}, {tuple(v_cache.shape)}")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError(f"{name}: the pools must be contiguous")
+    if code:
+        if k_scale is None or v_scale is None:
+            raise ValueError(f"{name}: a cache of codes needs its scales")
+        for t in (k_scale, v_scale):
+            if t.shape != shape[:3] or t.dtype is not torch.float32 or not t.is_contiguous():
+                raise ValueError(f"{name}: scales must be contiguous fp32 [pages, kv heads, page size]")
+    elif k_scale is not None or v_scale is not None:
+        raise ValueError(f"{name}: a 16-bit cache has no scales")
+    return (code,) + tuple(shape)
+
+
+def _slots(name, slots, T=None):
+    if slots.dim() != 1 or slots.dtype is not torch.int64 or (T is not None and slots.shape[0] != T):
+        raise ValueError(f"{name}: slots must be int64 [tokens], got {slots.dtype} {tuple(slots.shape)}")
+    return slots.contiguous()
+
+
+def _heads(name, t, dim):
+    """[tokens, heads, dim] with unit element stride, 16-byte aligned heads: t itself or a packed copy."""
+    if t.stride(2) != 1 or (t.stride(0) | t.stride(1)) % 8 or t.data_ptr() % 16:
+        t = torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+    return t
+
+
+def kv_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
+    """Writes new tokens' keys and values into a paged cache, quantized when the pools hold codes.
+
+    k, v: [tokens, kv heads, head dim] bf16/f16, any token and head strides.  slots: [tokens] int64,
+    distinct; slot s is place s % page_size of page s // page_size, a negative slot is skipped.
+    k_cache, v_cache: [pages, kv heads, page size, head dim], of k's dtype, int8 or float8_e4m3fn;
+    k_scale, v_scale: [pages, kv heads, page size] fp32 for codes (scale = max|row| / 127 or / 448).
+    """
+    _one_device("kv_write", k, v, slots, k_cache, v_cache, k_scale, v_scale)
+    code, pages, H, page, D = _kv_pools("kv_write", k_cache, v_cache, k_scale, v_scale)
+    if k.dtype not in _HALF or v.dtype is not k.dtype or (not code and k_cache.dtype is not k.dtype):
+        raise TypeError(f"kv_write: keys {k.dtype} and values {v.dtype} do not fit a {k_cache.dtype} cache")
+    if k.dim() != 3 or k.shape != v.shape or k.shape[1] != H or k.shape[2] != D:
+        raise ValueError(f"kv_write: keys {tuple(k.shape)} and values {tuple(v.shape)} must be [tokens, {H}, {D}]")
+    slots = _slots("kv_write", slots, k.shape[0])
+    k, v = _heads("kv_write", k, D), _heads("kv_write", v, D)
+    _launch("kv_write", _native.lib().psq_kv_write, code, k.data_ptr(), v.data_ptr(), _DT[k.dtype], k.stride(0), k.stride(1),
+            v.stride(0), v.stride(1), slots.data_ptr(), k.shape[0], H, D, k_cache.data_ptr(), v_cache.data_ptr(),
+            None if k_scale is None else k_scale.data_ptr(), None if v_scale is None else v_scale.data_ptr(), pages, page,
+            _stream(k))
+
+
+def kv_read(slots, k_cache, v_cache, k_scale=None, v_scale=None, out_dtype=None):
+    """Cached tokens back as dense rows: (k, v), each [tokens, kv heads, head dim] of out_dtype (default: the
+    cache's dtype, bf16 for codes).  slots as in kv_write; a negative slot reads as zeros."""
+    _one_device("kv_read", slots, k_cache, v_cache, k_scale, v_scale)
+    code, pages, H, page, D = _kv_pools("kv_read", k_cache, v_cache, k_scale, v_scale)
+    if out_dtype is None:
+        out_dtype = torch.bfloat16 if code else k_cache.dtype
+    if out_dtype not in _DT:
+        raise TypeError(f"kv_read: unsupported dtype {out_dtype}")
+    slots = _slots("kv_read", slots)
+    T = slots.shape[0]
+    k = torch.empty(T, H, D, dtype=out_dtype, device=slots.device)
+    v = torch.empty(T, H, D, dtype=out_dtype, device=slots.device)
+    _launch("kv_read", _native.lib().psq_kv_read, code, slots.data_ptr(), T, k_cache.data_ptr(), v_cache.data_ptr(),
+            0 if code else _DT[k_cache.dtype], None if k_scale is None else k_scale.data_ptr(),
+            None if v_scale is None else v_scale.data_ptr(), pages, page, H, D, k.data_ptr(), v.data_ptr(), _DT[out_dtype],
+            _stream(slots))
+    return k, v
+
+
+def paged_attention(q, k_cache, v_cache, block_table, lengths, k_scale=None, v_scale=None, scale=None, window=0,
+                    max_len=None, return_lse=False):
+    """Attention of one new token per sequence over a paged cache: [batch, heads, head dim] of q's dtype.
+
+    q: [batch, heads, head dim] bf16/f16, heads a multiple of the cache's kv heads; a 16-bit cache has q's
+    dtype.  block_table: [batch, columns] int32, the page of token t in column t // page_size; lengths:
+    [batch] int32, each sequence's tokens, the new one included (0: zeros).  scale: of the scores (default
+    head_dim ** -0.5); window: the last tokens that are attended to (0: all).  max_len: about the longest
+    length, which the host plans the split over the length by (default: what the table can hold).
+    return_lse: also the natural log of the softmax's denominator, [batch, heads] fp32.
+    A sequence that needs a page outside the pool, or more tokens than its table has, gets NaN.
+    """
+    _one_device("paged_attention", q, k_cache, v_cache, block_table, lengths, k_scale, v_scale)
+    code, pages, Hk, page, D = _kv_pools("paged_attention", k_cache, v_cache, k_scale, v_scale)
+    if q.dtype not in _HALF or (not code and k_cache.dtype is not q.dtype):
+        raise TypeError(f"paged_attention: {q.dtype} queries do not fit a {k_cache.dtype} cache")
+    if q.dim() != 3 or q.shape[2] != D or q.shape[1] % Hk:
+        raise ValueError(f"paged_attention: queries {tuple(q.shape)} must be [batch, a multiple of {Hk}, {D}]")
+    B, H, _ = q.shape
+    if block_table.dim() != 2 or block_table.shape[0] != B or block_table.dtype is not torch.int32:
+        raise ValueError(f"paged_attention: block_table must be int32 [{B}, columns]")
+    if lengths.shape != (B,) or lengths.dtype is not torch.int32:
+        raise ValueError(f"paged_attention: lengths must be int32 [{B}]")
+    window = int(window or 0)
+    if window < 0:
+        raise ValueError("paged_attention: window must be 0 or more")
+    cols = block_table.shape[1]
+    if block_table.stride(1) != 1 and cols > 1:
+        block_table = block_table.contiguous()
+    lengths = lengths.contiguous()
+    q = _heads("paged_attention", q, D)
+    max_len = cols * page if max_len is None else max(0, int(max_len))
+    if window:
+        max_len = min(max_len, window)
+    lib, stream = _native.lib(), _stream(q)
+    out = torch.empty(B, H, D, dtype=q.dtype, device=q.device)
+    lse = torch.empty(B, H, dtype=torch.float32, device=q.device) if return_lse else None
+    ws, nb = _workspace(q.device, stream.value, lib.psq_paged_attention_workspace_bytes(code, B, H, Hk, D, max_len))
+    _launch("paged_attention", lib.psq_paged_attention, code, q.data_ptr(), _DT[q.dtype], q.stride(0), q.stride(1),
+            k_cache.data_ptr(), v_cache.data_ptr(), None if k_scale is None else k_scale.data_ptr(),
+            None if v_scale is None else v_scale.data_ptr(), pages, page, block_table.data_ptr(), block_table.stride(0), cols,
+            lengths.data_ptr(), B, H, Hk, D, D ** -0.5 if scale is None else float(scale), window, max_len, out.data_ptr(),
+            None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), nb, stream)
+    return (out, lse) if return_lse else out
+
+
 # ------------------------------------------------------------------ checks
 # Non-finite flags, one per (device, stream), with the last ticket handed out: a call raises the
 # flag to its ticket when it finds a NaN or Inf, and the flag is never cleared.

@@ -293,6 +293,76 @@ PSQ_API int psq_dequant_fp8(const uint8_t *q, const float *w_scale, int w_scale_
 PSQ_API int psq_dequant_e5m2(const uint8_t *q, const float *w_scale, int w_scale_per_row, int64_t N,
                     int64_t K, void *out, int out_dtype, void *stream);
 
+/* ---------------------------------------------------------------- text decoder
+ * What a decoder layer does between its quantized linears (the reference's text encoders run these
+ * as torch modules around the int4 / int8 linears of powershard/quant_linear.py:191-227; it has no
+ * fused or cached form of them). */
+
+/* How rows are held: as they are (16 bits), as int8 codes, or as e4m3fn codes, with fp32 scales. */
+enum psq_codes { PSQ_CODES_NONE = 0, PSQ_CODES_I8 = 1, PSQ_CODES_E4M3 = 2 };
+
+/* RMS norm of x + residual, the rows leaving as the operand of psq_gemm_i8 / psq_gemm_fp8:
+ *   h = round_x(x + residual)               (residual NULL: h = x; else written to sum)
+ *   u = T(h w) 2^-k                         (T as in psq_quantize_rows_i8; rot_group 0: u = h w)
+ *   y = u / sqrt(mean(h^2) + eps)           fp32, the mean over the row's K elements
+ *   PSQ_CODES_I8 / _E4M3: out = codes of y, scale[m] = max|y| / 127 or / 448 (rows with max|h w| below
+ *     2^-120, zero rows among them: codes 0, scale 1); static_scale: *static_scale in its place
+ *   PSQ_CODES_NONE: out = round_x(y); scale unused
+ * The normalized row is never rounded to 16 bits on its way to the codes.  The factor
+ * 1 / sqrt(...) > 0 scales y and max|y| alike, so the codes do not depend on it, only the scale does.
+ * A row holding a NaN or Inf gets a NaN scale (codes) or NaN elements.
+ *   x, residual, sum [M, K] bf16/f16 (ldx, ldr, lds elements, multiples of 8, 16-byte aligned; sum may
+ *   be x or residual), weight [K] (weight_dtype, 16-byte aligned), out [M, K] (ldo elements, a multiple
+ *   of 16; of 8 for PSQ_CODES_NONE), K a multiple of 16, at most 32768. */
+PSQ_API int psq_add_rms_norm(int codes, const void *x, int x_dtype, int64_t ldx, const void *residual, int64_t ldr,
+                     const void *weight, int weight_dtype, float eps, void *sum, int64_t lds, int rot_group,
+                     const float *static_scale, void *out, int64_t ldo, float *scale, int64_t M, int64_t K,
+                     void *stream);
+
+/* A paged key-value cache: k_cache, v_cache [num_pages, Hkv, page_size, D], 16-bit elements
+ * (PSQ_CODES_NONE) or codes with k_scale, v_scale [num_pages, Hkv, page_size] fp32, one scale for the
+ * D elements of a token's head.  Slot s is place s % page_size of page s / page_size.  D a multiple of
+ * 16 in 16..256, page_size a multiple of 16, the pools contiguous and 16-byte aligned. */
+
+/* Writes T tokens' keys and values, quantized on the way: scale = max|row| / 127 or / 448 (rows below
+ * 2^-120: codes 0, scale 1), codes = round(v LIM / max|row|).  A row holding a NaN or Inf gets a
+ * non-finite scale.
+ *   k, v [T, Hkv, D] bf16/f16, element strides of tokens and heads (multiples of 8, 16-byte aligned)
+ *   slots [T] int64, distinct; a token whose slot is negative or past the pool is not written */
+PSQ_API int psq_kv_write(int codes, const void *k, const void *v, int dtype, int64_t k_token, int64_t k_head, int64_t v_token,
+                 int64_t v_head, const int64_t *slots, int64_t T, int Hkv, int D, void *k_cache, void *v_cache,
+                 float *k_scale, float *v_scale, int64_t num_pages, int page_size, void *stream);
+
+/* Reads T tokens back as dense rows: k, v [T, Hkv, D] of out_dtype (bf16, f16 or f32), round_out(code *
+ * scale).  cache_dtype: the elements of a PSQ_CODES_NONE cache.  A slot that is negative or past the
+ * pool reads as zeros. */
+PSQ_API int psq_kv_read(int codes, const int64_t *slots, int64_t T, const void *k_cache, const void *v_cache,
+                int cache_dtype, const float *k_scale, const float *v_scale, int64_t num_pages, int page_size,
+                int Hkv, int D, void *k, void *v, int out_dtype, void *stream);
+
+/* Attention of one token per sequence over the cache:
+ *   out[b][h] = sum_t p_t v_t, p = softmax_t(scale q[b][h] . k_t), t over the sequence's last
+ *   min(length, window) tokens (window 0: all), k_t and v_t of kv head h / (Hq / Hkv)
+ * Codes are exact in the matrix instructions' 16-bit operands and their scales are applied in fp32, to
+ * the scores and to the probabilities; scores, softmax statistics and sums are fp32.
+ *   q [B, Hq, D] bf16/f16 (element strides of sequences and heads, multiples of 8, 16-byte aligned;
+ *   PSQ_CODES_NONE: the cache's type), out [B, Hq, D] dense, of q's type; lse NULL or [B, Hq] fp32:
+ *   the natural log of the softmax's denominator
+ *   block_table [B, table_cols] int32 (table_stride elements a row): page of token t in column
+ *   t / page_size; columns past a sequence's length (and before its window) are not followed
+ *   lengths [B] int32, the tokens of each sequence, the new one included.  0 or less: zeros, lse -inf.
+ * A sequence longer than its table, or with a page outside the pool among those it needs, gets NaN.
+ * max_len: about the longest length, for the plan (any value gives right results).
+ * workspace: NULL (no split over the length), or at least psq_paged_attention_workspace_bytes() bytes
+ * with the arrival counters of the _ws GEMMs' workspace (zeroed once; every call leaves them zero). */
+PSQ_API int64_t psq_paged_attention_workspace_bytes(int codes, int64_t B, int Hq, int Hkv, int D, int64_t max_len);
+PSQ_API int psq_paged_attention(int codes, const void *q, int dtype, int64_t q_batch, int64_t q_head, const void *k_cache,
+                        const void *v_cache, const float *k_scale, const float *v_scale, int64_t num_pages,
+                        int page_size, const int32_t *block_table, int64_t table_stride, int64_t table_cols,
+                        const int32_t *lengths, int64_t B, int Hq, int Hkv, int D, float scale, int64_t window,
+                        int64_t max_len, void *out, float *lse, void *workspace, int64_t workspace_bytes,
+                        void *stream);
+
 /* ---------------------------------------------------------------- checks */
 
 /* Raises *flag (a device word) to max(*flag, ticket) when any of the n elements of x (bf16 / f16
