@@ -20,7 +20,7 @@ inline int check_kv_cache(const char *name, int codes, const void *k_cache, cons
     if (page_size % 16 || page_size > 65536)
         return set_error(PSQ_E_SHAPE, "%s: page size %d must be a multiple of 16 up to 65536", name, page_size);
     if (Hkv > 65535 || num_pages > 0x7fffffffLL || (int64_t)Hkv * page_size * D > 0x3fffffffLL ||
-        num_pages * page_size > 0xffffffffffLL)
+        num_pages * Hkv * (page_size / 16) > 0x7fffffffLL)
         return set_error(PSQ_E_SHAPE, "%s: a page of %d heads x %d x %d, or %lld pages, is too large", name, Hkv, page_size, D,
                          (long long)num_pages);
     if (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15 || ((uintptr_t)k_scale | (uintptr_t)v_scale) & 15)

@@ -1,96 +1,528 @@
 // paged_attention.hip -- attention of one new token per sequence over the paged key-value cache.
 //
-// The plain kernel: a workgroup per sequence and head, 256 tokens at a time, with the running maximum
-// and sum of the softmax.
+//   s_t = scale (q . k_t) ks_t,  p = softmax(s),  out = sum_t p_t vs_t v_t
+//
+// Bound by the cache's bytes: each key and value is read once for the G = Hq / Hkv heads that share it.
+// A workgroup of 4 waves takes a run of tokens of one sequence and kv head, for up to 16 of its heads;
+// its waves take steps of 32 tokens in turn, and each keeps a running maximum, sum and output of its own
+// (no barrier inside the run).  Everything goes from memory to registers in the layout that the matrix
+// instructions read (16x16x32, fp32 accumulation), with no LDS and no cross-lane move of keys, values or
+// probabilities.  Lane l, m = l & 15, g = l >> 4:
+//   S^T = K Q^T: K rows are tokens (lane row m), the contraction index 8 g + j stands for the dims that
+//     the lane has loaded, 16 bytes at 16 g of each 64-byte run of the row (Q is laid out to match);
+//     the result holds head m in the lane, tokens 4 g + i of each of the two tiles of 16;
+//   O^T = V^T P^T: those 8 probabilities are, as they are, the lane's part of P^T if contraction index
+//     8 g + j stands for token 4 g + j of tile 0 (j < 4) and 4 g + j - 4 of tile 1 (j >= 4).  For V^T the
+//     lane loads, of each of these 8 tokens, the dims m DV .. m DV + DV - 1 (whole rows per 16 lanes) and
+//     transposes 8 tokens x DV dims in its registers by byte permutes; row m of product dt is dim
+//     m DV + dt.
+// int8 and e4m3 codes are exact in bf16 (and f16), so they enter the products as they are; key scales
+// multiply the fp32 scores, value scales the fp32 probabilities.  A probability enters its product as a
+// pair of 16-bit numbers, p = hi + lo, two instructions each: 16 bits of it or more take part, and the
+// matrix units stay far below what the loads leave them.
+//
+// Split over the length: see plan().  A workgroup that holds part of a sequence writes its sums to the
+// workspace and counts itself; the last one adds the parts up in their order, so results do not depend
+// on timing.
 #include "kv_cache.hpp"
 
+#include <algorithm>
 #include <math.h>
 
 namespace psq {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kWaves = 4, kThreads = 64 * kWaves;
+constexpr int kStep = 32;                       // tokens of a wave's step
+constexpr int kTile = 16;                       // heads of a workgroup; tokens of a group (one page holds it)
+constexpr int kGrain = kStep * kWaves;          // tokens of a workgroup's round
+constexpr int kMaxSplits = 256;
+constexpr int64_t kCounterBytes = 64 * 1024;    // the arrival counters at the workspace's head
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttnArgs {
     const uint16_t *q;
     int64_t q_batch, q_head;
     const uint8_t *kc, *vc;
     const float *ks, *vs;
-    int64_t num_pages;
     const int32_t *table;
-    int64_t table_stride, table_cols;
+    int64_t table_stride;
     const int32_t *lengths;
     uint16_t *out;
     float *lse;
-    int64_t window;
-    int page, Hq, Hkv, D;
-    float scale;
+    uint32_t *count;
+    float *part;
+    int64_t part_floats;   // of one workgroup's part
+    int num_pages, cap;    // cap: tokens that a table row has room for
+    int page, Hq, Hkv, D, G, tiles, splits, chunk, window;
+    float scale;           // times log2(e)
 };
 
-template <int DT, int CODES>
-__device__ __forceinline__ float cache_elem(const uint8_t *pool, int64_t i)
+// Two fp32 values whose low 16 bits are zero as a packed bf16 pair.
+__device__ __forceinline__ uint32_t pack_exact_bf16(float lo, float hi)
 {
-    if constexpr (CODES == PSQ_CODES_I8) return (float)(int8_t)pool[i];
-    else if constexpr (CODES == PSQ_CODES_E4M3) return e4m3_to_f32(pool[i]);
-    else return half_to_f32<DT>(((const uint16_t *)pool)[i]);
+    return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+
+template <int B>
+__device__ __forceinline__ float i8_byte_f32(uint32_t w)
+{
+    float f;
+    if constexpr (B == 0)
+        asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(f) : "v"(w));
+    else if constexpr (B == 1)
+        asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(f) : "v"(w));
+    else if constexpr (B == 2)
+        asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(f) : "v"(w));
+    else
+        asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(f) : "v"(w));
+    return f;
+}
+
+// Bytes 2 H and 2 H + 1 of w, codes, as a packed pair of DT.
+template <int DT, int CODES, int H>
+__device__ __forceinline__ uint32_t code_pair(uint32_t w)
+{
+    if constexpr (CODES == PSQ_CODES_E4M3) {
+        if constexpr (DT == PSQ_BF16)
+            return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.0f, H != 0));
+        else
+            return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, H != 0));
+    } else if constexpr (DT == PSQ_BF16) {
+        return pack_exact_bf16(i8_byte_f32<2 * H>(w), i8_byte_f32<2 * H + 1>(w));
+    } else {
+        // the biased byte under the f16 exponent of 1024 is 1152 + q (integers to 2048 are exact)
+        const uint32_t h = __builtin_amdgcn_perm(0x64646464u, w ^ 0x80808080u, H ? 0x04030402u : 0x04010400u);
+        const f16x2_t q = __builtin_bit_cast(f16x2_t, h) - f16x2_t{(_Float16)1152.0f, (_Float16)1152.0f};
+        return __builtin_bit_cast(uint32_t, q);
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ v4f mfma(const v4i &a, const v4i &b, const v4f &c)
+{
+    if constexpr (DT == PSQ_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+
+// over the four lane groups g
+__device__ __forceinline__ float group_max(float x)
+{
+    const uint32_t u = __float_as_uint(x);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const float y = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+__device__ __forceinline__ float group_sum(float x)
+{
+    const uint32_t u = __float_as_uint(x);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const float y = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// DD: head dims the registers are laid out for; PART: D < DD, the rest of a row is not there.
+template <int DT, int CODES, int DD, bool PART>
+struct Step {
+    static constexpr int ES = CODES == PSQ_CODES_NONE ? 2 : 1;
+    static constexpr int KL = DD * ES / 64;       // 16-byte loads of a key row per lane group
+    static constexpr int DV = DD / 16, VW = DV * ES / 4;
+    v4i k[2][KL];
+    uint32_t v[8][VW];
+    v4f ks[2], vs[2];
+
+    // groups ga, gb: rows 16 ga .. and 16 gb .. of the pools
+    __device__ __forceinline__ void load(const AttnArgs &a, uint32_t ga, uint32_t gb, int m, int g)
+    {
+        const int row = (PART ? a.D : DD) * ES;
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const int64_t grp = t ? gb : ga;
+            const uint8_t *kp = a.kc + grp * (kTile * row), *vp = a.vc + grp * (kTile * row);
+#pragma unroll
+            for (int c = 0; c < KL; c++) {
+                const int at = 64 * c + 16 * g;
+                k[t][c] = v4i{0, 0, 0, 0};
+                if (!PART || at < row) k[t][c] = *(const v4i *)(kp + (uint32_t)(m * row + at));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                uint32_t *w = v[4 * t + i];
+                const uint8_t *src = vp + (uint32_t)((4 * g + i) * row + m * (DV * ES));
+#pragma unroll
+                for (int c = 0; c < VW; c++) w[c] = 0;
+                if (!PART || m * DV < a.D) {
+                    if constexpr (VW == 1) w[0] = *(const uint32_t *)src;
+                    else if constexpr (VW == 2) { const v2i x = *(const v2i *)src; w[0] = x[0], w[1] = x[1]; }
+                    else {
+#pragma unroll
+                        for (int c = 0; c < VW; c += 4) {
+                            const v4i x = *(const v4i *)(src + 4 * c);
+                            w[c] = x[0], w[c + 1] = x[1], w[c + 2] = x[2], w[c + 3] = x[3];
+                        }
+                    }
+                }
+            }
+            if constexpr (CODES != PSQ_CODES_NONE) {
+                ks[t] = *(const v4f *)(a.ks + grp * kTile + 4 * g);
+                vs[t] = *(const v4f *)(a.vs + grp * kTile + 4 * g);
+            }
+        }
+    }
+};
+
+template <int DT, int CODES, int DD, bool PART>
+__global__ void __launch_bounds__(kThreads, DD == 256 ? 1 : 2)
+paged_attention_kernel(AttnArgs a)
+{
+    using S = Step<DT, CODES, DD, PART>;
+    constexpr int ES = S::ES, DV = S::DV, VW = S::VW, NC = DD / 32;
+    constexpr int PVT = CODES == PSQ_CODES_NONE ? DT : PSQ_BF16;   // of the second product
+    extern __shared__ __attribute__((aligned(16))) float smem[];
+    __shared__ float wave_m[kWaves][kTile], wave_l[kWaves][kTile];
+    __shared__ uint32_t arrived;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int m = lane & 15, g = lane >> 4;
+    int id = blockIdx.x;
+    const int split = id % a.splits;
+    id /= a.splits;
+    const int ht = id % a.tiles;
+    const int hk = id / a.tiles % a.Hkv;
+    const int b = id / a.tiles / a.Hkv;
+    const int heads = min(a.G - ht * kTile, kTile);        // of this workgroup
+    const int D = PART ? a.D : DD;
+
+    // ---- the workgroup's run of tokens
+    int len = max(a.lengths[b], 0);
+    const bool past = len > a.cap;
+    len = min(len, a.cap);
+    const int lo = a.window ? max(len - a.window, 0) : 0;
+    const int base = lo & ~(kTile - 1);
+    int chunk = a.chunk;                                    // longer than planned for: longer runs
+    if ((len - base + chunk - 1) / chunk > a.splits)
+        chunk = ((len - base + a.splits - 1) / a.splits + kGrain - 1) / kGrain * kGrain;
+    const int parts = past ? 1 : max((len - base + chunk - 1) / chunk, 1);
+    if (split >= parts) return;
+    const int c0 = base + split * chunk, hi = past ? c0 : min(c0 + chunk, len);
+
+    // ---- queries
+    const int64_t head0 = (int64_t)hk * a.G + ht * kTile;
+    v4i qf[NC];
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+        const int d = ES == 2 ? 32 * c + 8 * g : 64 * (c >> 1) + 16 * g + 8 * (c & 1);
+        qf[c] = v4i{0, 0, 0, 0};
+        if (m < heads && (!PART || d < D)) qf[c] = *(const v4i *)(a.q + b * a.q_batch + (head0 + m) * a.q_head + d);
+    }
+
+    v4f o[DV];
+    float run_m, run_l;
+    bool pair = true;   // probabilities as hi + lo
+
+    const int steps = c0 + kStep * wave < hi ? (hi - c0 - kStep * wave + kGrain - 1) / kGrain : 0;
+    // the pool groups of 32 steps at a time, one per lane: lane 2 s + t has tile t of step s
+    const int per_page = a.page / kTile;
+    uint32_t grp = 0;
+    bool wild = false;
+    auto groups = [&](int s0) {
+        const int t = c0 + kStep * wave + (s0 + (lane >> 1)) * kGrain + kTile * (lane & 1);
+        grp = 0;
+        if (t < hi) {
+            const uint32_t n = (uint32_t)t / kTile, col = n / (uint32_t)per_page;
+            const int pg = a.table[b * a.table_stride + col];
+            if (pg < 0 || pg >= a.num_pages) wild = true;
+            else grp = ((uint32_t)pg * a.Hkv + hk) * per_page + (n - col * per_page);
+        }
+        wild = __any(wild);
+    };
+    auto load = [&](S &st, int s) {
+        const int i = 2 * (s & 31);
+        st.load(a, __builtin_amdgcn_readlane(grp, i), __builtin_amdgcn_readlane(grp, i + 1), m, g);
+    };
+    auto compute = [&](S &st, int s) {
+        const int t0 = c0 + kStep * wave + s * kGrain;
+        v4f sc[2];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            v4f x = {0, 0, 0, 0};
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                v4i kf;
+                if constexpr (ES == 2) {
+                    kf = st.k[t][c];
+                } else {
+                    const uint32_t w0 = (uint32_t)st.k[t][c >> 1][2 * (c & 1)], w1 = (uint32_t)st.k[t][c >> 1][2 * (c & 1) + 1];
+                    kf = v4i{(int)code_pair<DT, CODES, 0>(w0), (int)code_pair<DT, CODES, 1>(w0),
+                             (int)code_pair<DT, CODES, 0>(w1), (int)code_pair<DT, CODES, 1>(w1)};
+                }
+                x = mfma<DT>(kf, qf[c], x);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) sc[t][i] = x[i] * a.scale * (ES == 1 ? st.ks[t][i] : 1.0f);
+        }
+        if (t0 < lo || t0 + kStep > hi) {
+            // tokens outside: score -inf, and nothing of what their places hold (NaN, Inf) reaches the sums
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int tok = t0 + kTile * t + 4 * g + i;
+                    if (tok < lo || tok >= hi) {
+                        sc[t][i] = -INFINITY;
+                        if constexpr (ES == 1) st.vs[t][i] = 0.0f;
+                        if constexpr (CODES != PSQ_CODES_I8) {
+#pragma unroll
+                            for (int c = 0; c < VW; c++) st.v[4 * t + i][c] = 0;
+                        }
+                    }
+                }
+        }
+        float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
+                          fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+        top = group_max(top);
+        if (__any(top > run_m)) {
+            const float next = fmaxf(run_m, top);
+            const float keep = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(run_m - next);
+            run_m = next;
+            run_l *= keep;
+#pragma unroll
+            for (int dt = 0; dt < DV; dt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[dt][i] *= keep;
+        }
+        const float ref = run_m == -INFINITY ? 0.0f : run_m;
+        float p[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            p[j] = __builtin_amdgcn_exp2f(sc[j >> 2][j & 3] - ref);
+            run_l += p[j];
+            if constexpr (ES == 1) p[j] *= st.vs[j >> 2][j & 3];
+        }
+        v4i ph, pl;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint32_t h = pack_half2<PVT>(p[2 * j], p[2 * j + 1]);
+            ph[j] = (int)h;
+            pl[j] = (int)pack_half2<PVT>(p[2 * j] - half_to_f32<PVT>(h), p[2 * j + 1] - half_to_f32<PVT>(h >> 16));
+        }
+        if (!pair)
+#pragma unroll
+            for (int j = 0; j < 4; j++) ph[j] = pl[j] = (int)pack_half2<PVT>(0.5f * p[2 * j], 0.5f * p[2 * j + 1]);
+#pragma unroll
+        for (int dt = 0; dt < DV; dt++) {
+            v4i vf;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if constexpr (ES == 2) {
+                    vf[j] = (int)__builtin_amdgcn_perm(st.v[2 * j + 1][dt >> 1], st.v[2 * j][dt >> 1],
+                                                       dt & 1 ? 0x07060302u : 0x05040100u);
+                } else {
+                    const uint32_t w = __builtin_amdgcn_perm(st.v[2 * j + 1][dt >> 2], st.v[2 * j][dt >> 2],
+                                                             dt & 2 ? 0x07030602u : 0x05010400u);
+                    vf[j] = (int)(dt & 1 ? code_pair<PSQ_BF16, CODES, 1>(w) : code_pair<PSQ_BF16, CODES, 0>(w));
+                }
+            }
+            o[dt] = mfma<PVT>(vf, ph, o[dt]);
+            o[dt] = mfma<PVT>(vf, pl, o[dt]);
+        }
+    };
+
+    auto run = [&]() {
+#pragma unroll
+        for (int dt = 0; dt < DV; dt++) o[dt] = v4f{0, 0, 0, 0};
+        run_m = -INFINITY, run_l = 0.0f;
+        if (!steps) return;
+        groups(0);
+        if (wild) return;
+        S cur, nxt;
+        load(cur, 0);
+        for (int s = 0;; s += 2) {
+            if (s + 1 < steps) load(nxt, s + 1);
+            compute(cur, s);
+            if (s + 1 >= steps) break;
+            if (s + 2 < steps) {
+                if (((s + 2) & 31) == 0) {
+                    groups(s + 2);
+                    if (wild) break;
+                }
+                load(cur, s + 2);
+            }
+            compute(nxt, s + 1);
+            if (s + 2 >= steps) break;
+        }
+    };
+    for (;;) {
+        run();
+        // An infinite value meets lo = 0 or lo < 0 in the second product: NaN where the sum is infinite.
+        // Once more, then, with p as the sum of two equal halves (the precision of one 16-bit number).
+        float any = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < DV; dt++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) any = __builtin_fmaf(o[dt][i], 0.0f, any);
+        if (!pair || !__any(any != any)) break;
+        pair = false;
+    }
+    if (wild || past) run_m = 0.0f, run_l = NAN;
+
+    // ---- the waves' sums into one: each wave's output at its own maximum, in LDS
+    run_l = group_sum(run_l);
+    if (g == 0) {
+        wave_m[wave][m] = run_m;
+        wave_l[wave][m] = run_l;
+    }
+    constexpr int LD = DD + 4;
+    if (m < heads) {
+        float *w = smem + (wave * heads + m) * LD;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int dt = 0; dt < DV; dt += 4)
+                *(v4f *)(w + (4 * g + i) * DV + dt) = v4f{o[dt][i], o[dt + 1][i], o[dt + 2][i], o[dt + 3][i]};
+    }
+    __syncthreads();
+    const int quads = D / 4;
+    auto wave_sum = [&](int h, int d4, float &M, float &L) {
+        M = fmaxf(fmaxf(wave_m[0][h], wave_m[1][h]), fmaxf(wave_m[2][h], wave_m[3][h]));
+        const float ref = M == -INFINITY ? 0.0f : M;
+        v4f acc = {0, 0, 0, 0};
+        L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {
+            const float e = __builtin_amdgcn_exp2f(wave_m[w][h] - ref);
+            L += wave_l[w][h] * e;
+            const v4f x = *(const v4f *)(smem + (w * heads + h) * LD + 4 * d4);
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[i] += x[i] * e;
+        }
+        return acc;
+    };
+    auto finish = [&](int h, int d4, const v4f &acc, float M, float L) {
+        // no token: zeros; tokens whose scores are all -inf: 0 / 0, as softmax
+        const bool none = len == 0 && !past;
+        const float r = none ? 0.0f : 1.0f / L;
+        const int64_t head = b * (int64_t)a.Hq + head0 + h;
+        *(v2i *)(a.out + head * D + 4 * d4) = v2i{(int)pack_half2<DT>(acc[0] * r, acc[1] * r), (int)pack_half2<DT>(acc[2] * r, acc[3] * r)};
+        if (a.lse && d4 == 0) a.lse[head] = none ? -INFINITY : M * kLn2 + logf(L);
+    };
+    if (parts == 1) {
+        for (int i = tid; i < heads * quads; i += kThreads) {
+            const int h = i / quads, d4 = i - h * quads;
+            float M, L;
+            const v4f acc = wave_sum(h, d4, M, L);
+            finish(h, d4, acc, M, L);
+        }
+        return;
+    }
+
+    // ---- a part: outputs, then maxima and sums, written and read around the XCDs' own L2s (sc1), so that
+    // the count needs only the wait for the stores
+    constexpr int SC1 = 16;
+    const int64_t unit = id;                                // (sequence, kv head, head tile)
+    float *mine = a.part + (unit * a.splits + split) * a.part_floats;
+    {
+        const __amdgpu_buffer_rsrc_t rs = raw_rsrc(mine);
+        for (int i = tid; i < heads * quads; i += kThreads) {
+            const int h = i / quads, d4 = i - h * quads;
+            float M, L;
+            const v4f acc = wave_sum(h, d4, M, L);
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4i, acc), rs, i * 16, 0, SC1);
+            if (d4 == 0)
+                __builtin_amdgcn_raw_buffer_store_b64(v2i{__float_as_int(M), __float_as_int(L)}, rs,
+                                                      (heads * D + 2 * h) * 4, 0, SC1);
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0) arrived = atomicAdd(a.count + unit, 1u);
+    __syncthreads();
+    if (__builtin_amdgcn_readfirstlane(arrived) != (uint32_t)parts - 1) return;
+    // every other workgroup of the unit has counted itself: zero the count for the next launch
+    if (tid == 0) __hip_atomic_store(a.count + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const float *first = a.part + unit * a.splits * a.part_floats;
+    const __amdgpu_buffer_rsrc_t rs = raw_rsrc(first);
+    const int pitch = (int)a.part_floats * 4;
+    for (int i = tid; i < heads * quads; i += kThreads) {
+        const int h = i / quads, d4 = i - h * quads;
+        float M = -INFINITY;
+        for (int s = 0; s < parts; s++)
+            M = fmaxf(M, __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, (heads * D + 2 * h) * 4, s * pitch, SC1)));
+        const float ref = M == -INFINITY ? 0.0f : M;
+        v4f acc = {0, 0, 0, 0};
+        float L = 0.0f;
+        for (int s = 0; s < parts; s++) {
+            const v2i ml = __builtin_amdgcn_raw_buffer_load_b64(rs, (heads * D + 2 * h) * 4, s * pitch, SC1);
+            const v4f x = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rs, i * 16, s * pitch, SC1));
+            const float e = __builtin_amdgcn_exp2f(__int_as_float(ml[0]) - ref);
+            L += __int_as_float(ml[1]) * e;
+#pragma unroll
+            for (int c = 0; c < 4; c++) acc[c] += x[c] * e;
+        }
+        finish(h, d4, acc, M, L);
+    }
+}
+
+// ------------------------------------------------------------------ the split
+struct Plan {
+    int tiles, heads, splits, chunk;
+    int64_t part_floats, bytes;
+};
+
+Plan plan(int64_t B, int Hq, int Hkv, int D, int64_t max_len)
+{
+    Plan p{};
+    const int G = Hq / Hkv;
+    p.tiles = (G + kTile - 1) / kTile;
+    p.heads = std::min(G, kTile);
+    const int64_t units = B * Hkv * p.tiles;
+    const int64_t rounds = std::max<int64_t>((max_len + kGrain - 1) / kGrain, 1);   // of the longest sequence
+    int64_t splits = 1;
+    if (units * 4 <= kCounterBytes) {
+        const int64_t want = (1024 + units - 1) / units;
+        splits = std::min<int64_t>(std::min<int64_t>(std::max<int64_t>(want, (rounds + 7) / 8), rounds), kMaxSplits);
+    }
+    const int64_t per = (rounds + splits - 1) / splits;
+    p.chunk = (int)(per * kGrain);
+    p.splits = (int)((rounds + per - 1) / per);
+    p.part_floats = (int64_t)p.heads * D + (2 * p.heads + 3) / 4 * 4;
+    p.bytes = p.splits > 1 ? kCounterBytes + units * p.splits * p.part_floats * 4 : 0;
+    return p;
+}
+
+template <int DT, int CODES, int DD, bool PART>
+int launch(const AttnArgs &a, int64_t groups, hipStream_t st)
+{
+    const int heads = std::min(a.G, kTile), lds = kWaves * heads * (DD + 4) * 4;
+    auto *kernel = paged_attention_kernel<DT, CODES, DD, PART>;
+    if (lds > 48 * 1024) {
+        static bool raised[64] = {};
+        int dev = 0;
+        if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return set_error(PSQ_E_DEVICE, "no current HIP device");
+        if (!raised[dev]) {
+            if (hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kWaves * kTile * (DD + 4) * 4) != hipSuccess)
+                return set_error(PSQ_E_DEVICE, "paged_attention: cannot raise the LDS size");
+            raised[dev] = true;
+        }
+    }
+    kernel<<<(unsigned)groups, kThreads, lds, st>>>(a);
+    return check_launch("paged_attention");
 }
 
 template <int DT, int CODES>
-__global__ void __launch_bounds__(kThreads)
-paged_attention_kernel(AttnArgs a)
+int launch_dim(const AttnArgs &a, int64_t groups, hipStream_t st)
 {
-    __shared__ float q[256], p[kThreads], red[2];
-    __shared__ int64_t rows[kThreads];
-    const int tid = threadIdx.x, h = blockIdx.x, b = blockIdx.y, hk = h / (a.Hq / a.Hkv);
-    if (tid < a.D) q[tid] = half_to_f32<DT>(a.q[b * a.q_batch + h * a.q_head + tid]);
-    const int64_t cap = a.table_cols * a.page;
-    int64_t len = max(a.lengths[b], 0);
-    bool bad = len > cap;
-    len = min(len, cap);
-    int64_t t0 = a.window > 0 ? max((int64_t)0, len - a.window) : 0;
-    float m = -INFINITY, l = 0.0f, o = 0.0f;
-    for (; t0 < len; t0 += kThreads) {
-        const int n = (int)min((int64_t)kThreads, len - t0);
-        float s = -INFINITY;
-        __syncthreads();
-        if (tid < n) {
-            const int64_t t = t0 + tid;
-            int64_t pg = a.table[b * a.table_stride + t / a.page];
-            if (pg < 0 || pg >= a.num_pages) pg = -1;
-            rows[tid] = pg < 0 ? -1 : (pg * a.Hkv + hk) * a.page + t % a.page;
-            if (pg >= 0) {
-                float dot = 0.0f;
-                for (int d = 0; d < a.D; d++) dot += q[d] * cache_elem<DT, CODES>(a.kc, rows[tid] * a.D + d);
-                s = dot * a.scale * (CODES == PSQ_CODES_NONE ? 1.0f : a.ks[rows[tid]]);
-            } else {
-                s = NAN;
-            }
-        }
-        p[tid] = s;
-        __syncthreads();
-        if (tid == 0) {
-            float top = m;
-            for (int i = 0; i < n; i++) top = __builtin_elementwise_maximum(top, p[i]);
-            red[0] = top;
-        }
-        __syncthreads();
-        const float top = red[0], base = top == -INFINITY ? 0.0f : top;
-        p[tid] = tid < n ? expf(s - base) : 0.0f;
-        __syncthreads();
-        const float keep = expf(m - base);
-        l *= keep;
-        o *= keep;
-        m = top;
-        for (int i = 0; i < n; i++) {
-            l += p[i];
-            if (tid < a.D && rows[i] >= 0)
-                o += p[i] * (CODES == PSQ_CODES_NONE ? 1.0f : a.vs[rows[i]]) * cache_elem<DT, CODES>(a.vc, rows[i] * a.D + tid);
-        }
-    }
-    float y = len == 0 ? 0.0f : o / l;
-    if (bad) y = NAN;
-    if (tid < a.D) a.out[((int64_t)b * a.Hq + h) * a.D + tid] = (uint16_t)f32_to_half<DT>(y);
-    if (a.lse && tid == 0) a.lse[(int64_t)b * a.Hq + h] = bad ? NAN : m + logf(l);
+    if (a.D == 64) return launch<DT, CODES, 64, false>(a, groups, st);
+    if (a.D == 128) return launch<DT, CODES, 128, false>(a, groups, st);
+    if (a.D == 256) return launch<DT, CODES, 256, false>(a, groups, st);
+    if (a.D < 64) return launch<DT, CODES, 64, true>(a, groups, st);
+    if (a.D < 128) return launch<DT, CODES, 128, true>(a, groups, st);
+    return launch<DT, CODES, 256, true>(a, groups, st);
 }
 
 }  // namespace
@@ -100,8 +532,9 @@ extern "C" {
 
 int64_t psq_paged_attention_workspace_bytes(int codes, int64_t B, int Hq, int Hkv, int D, int64_t max_len)
 {
-    (void)codes, (void)B, (void)Hq, (void)Hkv, (void)D, (void)max_len;
-    return 0;
+    (void)codes;
+    if (B <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || max_len <= 0 || Hq % Hkv || B > 65535) return 0;
+    return psq::plan(B, Hq, Hkv, D, std::min<int64_t>(max_len, 0x7fffffffLL)).bytes;
 }
 
 int psq_paged_attention(int codes, const void *q, int dtype, int64_t q_batch, int64_t q_head, const void *k_cache,
@@ -123,22 +556,25 @@ int psq_paged_attention(int codes, const void *q, int dtype, int64_t q_batch, in
         return set_error(PSQ_E_SHAPE, "%s: queries and output must be 16-byte aligned, query strides multiples of 8", name);
     if (((uintptr_t)block_table | (uintptr_t)lengths | (uintptr_t)lse) & 3)
         return set_error(PSQ_E_SHAPE, "%s: misaligned table, lengths or lse", name);
-    if (B > 65535 || table_cols > 0x7fffffffLL / page_size)
-        return set_error(PSQ_E_SHAPE, "%s: %lld sequences of %lld pages are too many", name, (long long)B,
-                         (long long)table_cols);
-    (void)workspace, (void)max_len;
+    if (B > 65535 || table_cols > 0x3fffffffLL / page_size)
+        return set_error(PSQ_E_SHAPE, "%s: %lld sequences of %lld pages are too many", name, (long long)B, (long long)table_cols);
+    if ((uintptr_t)workspace & 255) return set_error(PSQ_E_SHAPE, "%s: the workspace must be 256-byte aligned", name);
+    const int64_t cap = table_cols * page_size;
+    Plan p = plan(B, Hq, Hkv, D, std::min(max_len, cap));
+    if (p.splits > 1 && (!workspace || workspace_bytes < p.bytes)) p.splits = 1;
+    const int64_t groups = B * Hkv * p.tiles * p.splits;
+    if (groups > 0x7fffffffLL) return set_error(PSQ_E_SHAPE, "%s: %lld workgroups are too many", name, (long long)groups);
     if (int e = require_device()) return e;
     const AttnArgs a{(const uint16_t *)q, q_batch, q_head, (const uint8_t *)k_cache, (const uint8_t *)v_cache, k_scale, v_scale,
-                     num_pages, block_table, table_stride, table_cols, lengths, (uint16_t *)out, lse, window, page_size, Hq, Hkv,
-                     D, scale};
+                     block_table, table_stride, lengths, (uint16_t *)out, lse, (uint32_t *)workspace,
+                     (float *)((uint8_t *)workspace + kCounterBytes), p.part_floats, (int)num_pages, (int)cap, page_size, Hq, Hkv,
+                     D, Hq / Hkv, p.tiles, p.splits, p.chunk, (int)std::min<int64_t>(window, cap), scale * kLog2e};
     hipStream_t st = (hipStream_t)stream;
-    const dim3 grid((unsigned)Hq, (unsigned)B);
     auto go = [&](auto dtc) {
         constexpr int DT = decltype(dtc)::value;
-        if (codes == PSQ_CODES_I8) paged_attention_kernel<DT, PSQ_CODES_I8><<<grid, kThreads, 0, st>>>(a);
-        else if (codes == PSQ_CODES_E4M3) paged_attention_kernel<DT, PSQ_CODES_E4M3><<<grid, kThreads, 0, st>>>(a);
-        else paged_attention_kernel<DT, PSQ_CODES_NONE><<<grid, kThreads, 0, st>>>(a);
-        return check_launch(name);
+        if (codes == PSQ_CODES_I8) return launch_dim<DT, PSQ_CODES_I8>(a, groups, st);
+        if (codes == PSQ_CODES_E4M3) return launch_dim<DT, PSQ_CODES_E4M3>(a, groups, st);
+        return launch_dim<DT, PSQ_CODES_NONE>(a, groups, st);
     };
     return dtype == PSQ_BF16 ? go(std::integral_constant<int, PSQ_BF16>{}) : go(std::integral_constant<int, PSQ_F16>{});
 }
