@@ -126,6 +126,20 @@ __device__ __forceinline__ float group_sum(float x)
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+__device__ __forceinline__ float wave_max(float x)
+{
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
+    return x;
+}
+
+__device__ __forceinline__ float wave_add(float x)
+{
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
+    return x;
+}
+
 // DD: head dims the registers are laid out for; PART: D < DD, the rest of a row is not there.
 template <int DT, int CODES, int DD, bool PART>
 struct Step {
@@ -445,26 +459,70 @@ paged_attention_kernel(AttnArgs a)
     if (__builtin_amdgcn_readfirstlane(arrived) != (uint32_t)parts - 1) return;
     // every other workgroup of the unit has counted itself: zero the count for the next launch
     if (tid == 0) __hip_atomic_store(a.count + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const float *first = a.part + unit * a.splits * a.part_floats;
-    const __amdgpu_buffer_rsrc_t rs = raw_rsrc(first);
+    // The parts' maxima and sums go to LDS (a wave per head turns them into weights), then every load of
+    // the outputs is independent: as many as the registers hold in flight, the parts shared out among
+    // the threads that a narrow unit leaves over.
+    const __amdgpu_buffer_rsrc_t rs = raw_rsrc(a.part + unit * a.splits * a.part_floats);
     const int pitch = (int)a.part_floats * 4;
-    for (int i = tid; i < heads * quads; i += kThreads) {
-        const int h = i / quads, d4 = i - h * quads;
-        float M = -INFINITY;
-        for (int s = 0; s < parts; s++)
-            M = fmaxf(M, __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, (heads * D + 2 * h) * 4, s * pitch, SC1)));
+    float *weight = smem, *sums = smem + heads * parts;
+    v4f *red = (v4f *)(smem + (2 * heads * parts + 3) / 4 * 4);
+    for (int i = tid; i < heads * parts; i += kThreads) {
+        const int s = i / heads, h = i - s * heads;
+        const v2i ml = __builtin_amdgcn_raw_buffer_load_b64(rs, (heads * D + 2 * h) * 4 + s * pitch, 0, SC1);
+        weight[h * parts + s] = __int_as_float(ml[0]);
+        sums[h * parts + s] = __int_as_float(ml[1]);
+    }
+    __syncthreads();
+    for (int h = wave; h < heads; h += kWaves) {
+        float M = -INFINITY, L = 0.0f;
+        for (int s = lane; s < parts; s += 64) M = fmaxf(M, weight[h * parts + s]);
+        M = wave_max(M);
         const float ref = M == -INFINITY ? 0.0f : M;
-        v4f acc = {0, 0, 0, 0};
-        float L = 0.0f;
-        for (int s = 0; s < parts; s++) {
-            const v2i ml = __builtin_amdgcn_raw_buffer_load_b64(rs, (heads * D + 2 * h) * 4, s * pitch, SC1);
-            const v4f x = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rs, i * 16, s * pitch, SC1));
-            const float e = __builtin_amdgcn_exp2f(__int_as_float(ml[0]) - ref);
-            L += __int_as_float(ml[1]) * e;
-#pragma unroll
-            for (int c = 0; c < 4; c++) acc[c] += x[c] * e;
+        for (int s = lane; s < parts; s += 64) {
+            const float e = __builtin_amdgcn_exp2f(weight[h * parts + s] - ref);
+            weight[h * parts + s] = e;
+            L += sums[h * parts + s] * e;
         }
-        finish(h, d4, acc, M, L);
+        L = wave_add(L);
+        if (lane == 0) wave_m[0][h] = M, wave_l[0][h] = L;
+    }
+    __syncthreads();
+    const int items = heads * quads, sharers = max(1, kThreads / items);
+    const int share = sharers > 1 ? tid / items : 0;
+    for (int i = tid - share * items; i < items && share < sharers; i += kThreads) {
+        const int h = i / quads;
+        v4f acc = {0, 0, 0, 0};
+        constexpr int U = 8;
+        for (int s0 = share; s0 < parts; s0 += U * sharers) {
+            v4i x[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int s = s0 + u * sharers;
+                x[u] = v4i{0, 0, 0, 0};
+                if (s < parts) x[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, i * 16 + s * pitch, 0, SC1);
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int s = s0 + u * sharers;
+                const float e = s < parts ? weight[h * parts + s] : 0.0f;
+#pragma unroll
+                for (int c = 0; c < 4; c++) acc[c] += __int_as_float(x[u][c]) * e;
+            }
+        }
+        if (sharers == 1) finish(h, i - h * quads, acc, wave_m[0][h], wave_l[0][h]);
+        else red[tid] = acc;
+    }
+    if (sharers == 1) return;
+    __syncthreads();
+    if (tid < items) {
+        const int h = tid / quads;
+        v4f acc = red[tid];
+        for (int k = 1; k < sharers; k++) {
+            const v4f x = red[k * items + tid];
+#pragma unroll
+            for (int c = 0; c < 4; c++) acc[c] += x[c];
+        }
+        finish(h, tid - h * quads, acc, wave_m[0][h], wave_l[0][h]);
     }
 }
 
@@ -498,19 +556,21 @@ Plan plan(int64_t B, int Hq, int Hkv, int D, int64_t max_len)
 template <int DT, int CODES, int DD, bool PART>
 int launch(const AttnArgs &a, int64_t groups, hipStream_t st)
 {
-    const int heads = std::min(a.G, kTile), lds = kWaves * heads * (DD + 4) * 4;
+    // the waves' outputs, then (the joining workgroup) the parts' weights, sums and 256 quads
+    const int heads = std::min(a.G, kTile);
+    const int lds = std::max(kWaves * heads * (DD + 4), (2 * heads * a.splits + 3) / 4 * 4 + 4 * kThreads) * 4;
     auto *kernel = paged_attention_kernel<DT, CODES, DD, PART>;
     if (lds > 48 * 1024) {
         static bool raised[64] = {};
         int dev = 0;
         if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return set_error(PSQ_E_DEVICE, "no current HIP device");
         if (!raised[dev]) {
-            if (hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kWaves * kTile * (DD + 4) * 4) != hipSuccess)
+            if (hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024) != hipSuccess)
                 return set_error(PSQ_E_DEVICE, "paged_attention: cannot raise the LDS size");
             raised[dev] = true;
         }
     }
-    kernel<<<(unsigned)groups, kThreads, lds, st>>>(a);
+    kernel<<<(unsigned)groups, kThreads, lds, st>>>(a);   // at most 65 KB (256 dims), 37 KB (256 splits)
     return check_launch("paged_attention");
 }
 
