@@ -21,9 +21,11 @@
 // pair of 16-bit numbers, p = hi + lo, two instructions each: 16 bits of it or more take part, and the
 // matrix units stay far below what the loads leave them.
 //
-// Split over the length: see plan().  A workgroup that holds part of a sequence writes its sums to the
-// workspace and counts itself; the last one adds the parts up in their order, so results do not depend
-// on timing.
+// Work is dealt in rounds of 128 tokens (a step of each wave).  The rounds of all units (sequence, kv
+// head, head tile), in their order, are cut into equal runs, one per workgroup, as many workgroups as the
+// chip holds at once: ragged lengths cost no balance, the host needs no lengths, and a unit is cut only
+// where a run ends.  The parts of a cut unit go through the workspace to a second kernel, which adds them
+// up in their order: results do not depend on timing.
 #include "kv_cache.hpp"
 
 #include <algorithm>
@@ -32,13 +34,20 @@
 namespace psq {
 namespace {
 
+typedef float v2f __attribute__((ext_vector_type(2)));
+
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kStep = 32;                       // tokens of a wave's step
 constexpr int kTile = 16;                       // heads of a workgroup; tokens of a group (one page holds it)
 constexpr int kGrain = kStep * kWaves;          // tokens of a workgroup's round
-constexpr int kMaxSplits = 256;
-constexpr int64_t kCounterBytes = 64 * 1024;    // the arrival counters at the workspace's head
+constexpr int64_t kCounterBytes = 64 * 1024;    // arrival counters of the GEMMs at the workspace's head
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// The unit that a run begins and does not end: its sequence, index in it, and parts (0: no such unit).
+struct Cut { int b, unit, parts; };
+
+// workgroups that a CU holds at once
+constexpr int groups_per_cu(int D) { return D > 128 ? 1 : D > 64 ? 2 : 3; }
 
 struct AttnArgs {
     const uint16_t *q;
@@ -50,11 +59,13 @@ struct AttnArgs {
     const int32_t *lengths;
     uint16_t *out;
     float *lse;
-    uint32_t *count;
-    float *part;
-    int64_t part_floats;   // of one workgroup's part
+    Cut *cut;              // one per run
+    float *part;           // two per run
+    int part_floats;       // of one part
     int num_pages, cap;    // cap: tokens that a table row has room for
-    int page, Hq, Hkv, D, G, tiles, splits, chunk, window;
+    int B, page, Hq, Hkv, D, G, tiles, window;
+    int least;             // rounds that a workgroup's run has at least
+    int alone;             // no workspace: units stay whole
     float scale;           // times log2(e)
 };
 
@@ -126,22 +137,55 @@ __device__ __forceinline__ float group_sum(float x)
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-__device__ __forceinline__ float wave_max(float x)
+// a value that all lanes hold, in scalar registers
+__device__ __forceinline__ uint64_t uniform(uint64_t x)
 {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
-    return x;
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)) << 32 |
+           (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)x);
 }
 
-__device__ __forceinline__ float wave_add(float x)
+// x / y, by the short division where x allows it
+__device__ __forceinline__ uint64_t divide(uint64_t x, uint32_t y)
 {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
-    return x;
+    return uniform(x >> 32 ? x / y : (uint64_t)((uint32_t)x / y));
 }
 
-// DD: head dims the registers are laid out for; PART: D < DD, the rest of a row is not there.
-template <int DT, int CODES, int DD, bool PART>
+// Sums of parts, kept at the maximum M: first brought to a new one, then a part (at maximum m) added.
+__device__ __forceinline__ float scale_to(float from, float to)
+{
+    return __builtin_amdgcn_exp2f(from - (to == -INFINITY ? 0.0f : to));
+}
+
+__device__ __forceinline__ void join_move(float &M, float &L, v4f &acc, float to)
+{
+    const float e = scale_to(M, to);
+    L *= e;
+#pragma unroll
+    for (int c = 0; c < 4; c++) acc[c] *= e;
+    M = to;
+}
+
+__device__ __forceinline__ void join_add(float M, float &L, v4f &acc, float m, float l, const v4f &y)
+{
+    const float e = scale_to(m, M);
+    L += l * e;
+#pragma unroll
+    for (int c = 0; c < 4; c++) acc[c] += y[c] * e;
+}
+
+// Four dims of a head's output from the sums at maximum M (in units of log2), and its lse.  none: no
+// token, zeros (tokens whose scores are all -inf: 0 / 0, as softmax).
+template <int DT>
+__device__ __forceinline__ void finish(uint16_t *out, float *lse, int64_t head, int D, int d4, const v4f &acc, float M, float L,
+                                       bool none)
+{
+    const float r = none ? 0.0f : 1.0f / L;
+    *(v2i *)(out + head * D + 4 * d4) = v2i{(int)pack_half2<DT>(acc[0] * r, acc[1] * r), (int)pack_half2<DT>(acc[2] * r, acc[3] * r)};
+    if (lse && d4 == 0) lse[head] = none ? -INFINITY : M * kLn2 + logf(L);
+}
+
+// A step's registers.  DD: head dims they are laid out for; PART: D < DD, the rest of a row is not there.
+template <int CODES, int DD, bool PART>
 struct Step {
     static constexpr int ES = CODES == PSQ_CODES_NONE ? 2 : 1;
     static constexpr int KL = DD * ES / 64;       // 16-byte loads of a key row per lane group
@@ -151,25 +195,37 @@ struct Step {
     v4f ks[2], vs[2];
 
     // groups ga, gb: rows 16 ga .. and 16 gb .. of the pools
-    __device__ __forceinline__ void load(const AttnArgs &a, uint32_t ga, uint32_t gb, int m, int g)
+    __device__ __forceinline__ void load_keys(const AttnArgs &a, uint32_t ga, uint32_t gb, int m, int g)
     {
         const int row = (PART ? a.D : DD) * ES;
 #pragma unroll
         for (int t = 0; t < 2; t++) {
             const int64_t grp = t ? gb : ga;
-            const uint8_t *kp = a.kc + grp * (kTile * row), *vp = a.vc + grp * (kTile * row);
+            const uint8_t *kp = a.kc + grp * (kTile * row);
 #pragma unroll
             for (int c = 0; c < KL; c++) {
                 const int at = 64 * c + 16 * g;
-                k[t][c] = v4i{0, 0, 0, 0};
+                if (PART) k[t][c] = v4i{0, 0, 0, 0};
                 if (!PART || at < row) k[t][c] = *(const v4i *)(kp + (uint32_t)(m * row + at));
             }
+            if constexpr (ES == 1) ks[t] = *(const v4f *)(a.ks + grp * kTile + 4 * g);
+        }
+    }
+
+    __device__ __forceinline__ void load_values(const AttnArgs &a, uint32_t ga, uint32_t gb, int m, int g)
+    {
+        const int row = (PART ? a.D : DD) * ES;
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const int64_t grp = t ? gb : ga;
+            const uint8_t *vp = a.vc + grp * (kTile * row);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 uint32_t *w = v[4 * t + i];
                 const uint8_t *src = vp + (uint32_t)((4 * g + i) * row + m * (DV * ES));
+                if (PART)
 #pragma unroll
-                for (int c = 0; c < VW; c++) w[c] = 0;
+                    for (int c = 0; c < VW; c++) w[c] = 0;
                 if (!PART || m * DV < a.D) {
                     if constexpr (VW == 1) w[0] = *(const uint32_t *)src;
                     else if constexpr (VW == 2) { const v2i x = *(const v2i *)src; w[0] = x[0], w[1] = x[1]; }
@@ -182,48 +238,95 @@ struct Step {
                     }
                 }
             }
-            if constexpr (CODES != PSQ_CODES_NONE) {
-                ks[t] = *(const v4f *)(a.ks + grp * kTile + 4 * g);
-                vs[t] = *(const v4f *)(a.vs + grp * kTile + 4 * g);
-            }
+            if constexpr (ES == 1) vs[t] = *(const v4f *)(a.vs + grp * kTile + 4 * g);
         }
     }
 };
 
 template <int DT, int CODES, int DD, bool PART>
-__global__ void __launch_bounds__(kThreads, DD == 256 ? 1 : 2)
+__global__ void __launch_bounds__(kThreads, groups_per_cu(DD))
 paged_attention_kernel(AttnArgs a)
 {
-    using S = Step<DT, CODES, DD, PART>;
-    constexpr int ES = S::ES, DV = S::DV, VW = S::VW, NC = DD / 32;
+    using S = Step<CODES, DD, PART>;
+    constexpr int ES = S::ES, DV = S::DV, VW = S::VW, NC = DD / 32, NB = 1;
     constexpr int PVT = CODES == PSQ_CODES_NONE ? DT : PSQ_BF16;   // of the second product
     extern __shared__ __attribute__((aligned(16))) float smem[];
     __shared__ float wave_m[kWaves][kTile], wave_l[kWaves][kTile];
-    __shared__ uint32_t arrived;
+    __shared__ uint32_t wave_rounds[kWaves], start_r;
+    __shared__ int start_b;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int m = lane & 15, g = lane >> 4;
-    int id = blockIdx.x;
-    const int split = id % a.splits;
-    id /= a.splits;
-    const int ht = id % a.tiles;
-    const int hk = id / a.tiles % a.Hkv;
-    const int b = id / a.tiles / a.Hkv;
-    const int heads = min(a.G - ht * kTile, kTile);        // of this workgroup
-    const int D = PART ? a.D : DD;
+    const int D = PART ? a.D : DD, per_page = a.page / kTile, units = a.Hkv * a.tiles;   // (units of a sequence)
 
-    // ---- the workgroup's run of tokens
-    int len = max(a.lengths[b], 0);
-    const bool past = len > a.cap;
-    len = min(len, a.cap);
-    const int lo = a.window ? max(len - a.window, 0) : 0;
-    const int base = lo & ~(kTile - 1);
-    int chunk = a.chunk;                                    // longer than planned for: longer runs
-    if ((len - base + chunk - 1) / chunk > a.splits)
-        chunk = ((len - base + a.splits - 1) / a.splits + kGrain - 1) / kGrain * kGrain;
-    const int parts = past ? 1 : max((len - base + chunk - 1) / chunk, 1);
-    if (split >= parts) return;
-    const int c0 = base + split * chunk, hi = past ? c0 : min(c0 + chunk, len);
+    // ---- the workgroup's run of rounds
+    auto span = [&](int b, int &len, int &lo, bool &past) {   // tokens of sequence b; its rounds
+        len = max(a.lengths[b], 0);
+        past = len > a.cap;
+        len = min(len, a.cap);
+        lo = a.window ? max(len - a.window, 0) : 0;
+        return past ? 1 : max((len - (lo & ~(kTile - 1)) + kGrain - 1) / kGrain, 1);
+    };
+    int len, lo, rounds;
+    bool past;
+    const int each = (a.B + kThreads - 1) / kThreads;       // sequences of a thread
+    uint32_t own = 0;
+    for (int i = 0; i < each; i++)
+        if (tid * each + i < a.B) own += span(tid * each + i, len, lo, past);
+    uint32_t before = own;                                  // rounds up to and with this thread's
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t y = __shfl_up(before, o, 64);
+        before += lane >= o ? y : 0;
+    }
+    if (lane == 63) wave_rounds[wave] = before;
+    __syncthreads();
+    uint32_t total = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; i++) {
+        before += i < wave ? wave_rounds[i] : 0;
+        total += wave_rounds[i];
+    }
+    before -= own;
+    const uint64_t all = uniform((uint64_t)total * units);
+    const uint32_t w = blockIdx.x;
+    const uint32_t runs = a.alone ? gridDim.x : (uint32_t)max(min((uint64_t)gridDim.x, divide(all, a.least)), (uint64_t)1);
+    auto first_of = [&](uint32_t w) { return all >> 32 ? uniform(w * all / runs) : divide(w * all, runs); };
+    uint64_t x = 0, end;
+    int b, unit, r = 0;
+    if (a.alone) {
+        b = w / (uint32_t)units, unit = w - b * units;
+        end = rounds = span(b, len, lo, past);
+    } else {
+        if (w >= runs) {
+            if (tid == 0) a.cut[w] = Cut{0, 0, 0};
+            return;
+        }
+        x = first_of(w), end = first_of(w + 1);
+        const uint32_t y = (uint32_t)divide(x, units);      // the thread whose sequences hold the run's start
+        if (y >= before && y < before + own) {
+            int i = tid * each;
+            for (;; i++) {
+                const int n = span(i, len, lo, past);
+                if (y < before + n) break;
+                before += n;
+            }
+            start_b = i;
+            start_r = before;
+        }
+        __syncthreads();
+        b = __builtin_amdgcn_readfirstlane(start_b);
+        rounds = span(b, len, lo, past);
+        const uint64_t in = x - (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(start_r) * units;
+        unit = (int)divide(in, rounds), r = (int)(in - (uint64_t)unit * rounds);
+    }
+    Cut cut{0, 0, 0};
+
+    for (;;) {
+    const int n = (int)min(end - x, (uint64_t)(rounds - r));     // this segment's rounds
+    const int hk = unit / a.tiles, ht = unit - hk * a.tiles;
+    const int heads = min(a.G - ht * kTile, kTile);
+    const int c0 = (lo & ~(kTile - 1)) + r * kGrain, hi = past ? c0 : min(c0 + n * kGrain, len);
 
     // ---- queries
     const int64_t head0 = (int64_t)hk * a.G + ht * kTile;
@@ -241,7 +344,6 @@ paged_attention_kernel(AttnArgs a)
 
     const int steps = c0 + kStep * wave < hi ? (hi - c0 - kStep * wave + kGrain - 1) / kGrain : 0;
     // the pool groups of 32 steps at a time, one per lane: lane 2 s + t has tile t of step s
-    const int per_page = a.page / kTile;
     uint32_t grp = 0;
     bool wild = false;
     auto groups = [&](int s0) {
@@ -255,11 +357,18 @@ paged_attention_kernel(AttnArgs a)
         }
         wild = __any(wild);
     };
-    auto load = [&](S &st, int s) {
+    // NB steps are in flight or here.  Step s + NB's loads go into step s's registers as soon as these are
+    // read: its keys before the softmax, its values after the second product.
+    S ring[NB];
+    auto load_keys = [&](S &st, int s) {
         const int i = 2 * (s & 31);
-        st.load(a, __builtin_amdgcn_readlane(grp, i), __builtin_amdgcn_readlane(grp, i + 1), m, g);
+        st.load_keys(a, __builtin_amdgcn_readlane(grp, i), __builtin_amdgcn_readlane(grp, i + 1), m, g);
     };
-    auto compute = [&](S &st, int s) {
+    auto load_values = [&](S &st, int s) {
+        const int i = 2 * (s & 31);
+        st.load_values(a, __builtin_amdgcn_readlane(grp, i), __builtin_amdgcn_readlane(grp, i + 1), m, g);
+    };
+    auto compute = [&](S &st, int s, bool more) {
         const int t0 = c0 + kStep * wave + s * kGrain;
         v4f sc[2];
 #pragma unroll
@@ -280,6 +389,7 @@ paged_attention_kernel(AttnArgs a)
 #pragma unroll
             for (int i = 0; i < 4; i++) sc[t][i] = x[i] * a.scale * (ES == 1 ? st.ks[t][i] : 1.0f);
         }
+        if (more) load_keys(st, s + NB);
         if (t0 < lo || t0 + kStep > hi) {
             // tokens outside: score -inf, and nothing of what their places hold (NaN, Inf) reaches the sums
 #pragma unroll
@@ -354,22 +464,25 @@ paged_attention_kernel(AttnArgs a)
         if (!steps) return;
         groups(0);
         if (wild) return;
-        S cur, nxt;
-        load(cur, 0);
-        for (int s = 0;; s += 2) {
-            if (s + 1 < steps) load(nxt, s + 1);
-            compute(cur, s);
-            if (s + 1 >= steps) break;
-            if (s + 2 < steps) {
-                if (((s + 2) & 31) == 0) {
-                    groups(s + 2);
-                    if (wild) break;
-                }
-                load(cur, s + 2);
+#pragma unroll
+        for (int i = 0; i < NB; i++)
+            if (i < steps) {
+                load_keys(ring[i], i);
+                load_values(ring[i], i);
             }
-            compute(nxt, s + 1);
-            if (s + 2 >= steps) break;
-        }
+        for (int s0 = 0; s0 < steps; s0 += NB)
+#pragma unroll
+            for (int i = 0; i < NB; i++) {
+                const int s = s0 + i;
+                if (s >= steps) break;
+                const bool more = s + NB < steps;
+                if (more && ((s + NB) & 31) == 0) {
+                    groups(s + NB);
+                    if (wild) return;
+                }
+                compute(ring[i], s, more);
+                if (more) load_values(ring[i], s + NB);
+            }
     };
     for (;;) {
         run();
@@ -402,134 +515,95 @@ paged_attention_kernel(AttnArgs a)
     }
     __syncthreads();
     const int quads = D / 4;
-    auto wave_sum = [&](int h, int d4, float &M, float &L) {
-        M = fmaxf(fmaxf(wave_m[0][h], wave_m[1][h]), fmaxf(wave_m[2][h], wave_m[3][h]));
-        const float ref = M == -INFINITY ? 0.0f : M;
+    // a run has two parts: of the unit that it goes on with (0) and of the one that it leaves (1)
+    const bool whole = n == rounds;
+    float *part = whole ? nullptr : a.part + (int64_t)(2 * w + (r == 0)) * a.part_floats;
+    for (int i = tid; i < heads * quads; i += kThreads) {
+        const int h = i / quads, d4 = i - h * quads;
+        const float M = fmaxf(fmaxf(wave_m[0][h], wave_m[1][h]), fmaxf(wave_m[2][h], wave_m[3][h]));
         v4f acc = {0, 0, 0, 0};
-        L = 0.0f;
+        float L = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) {
-            const float e = __builtin_amdgcn_exp2f(wave_m[w][h] - ref);
-            L += wave_l[w][h] * e;
-            const v4f x = *(const v4f *)(smem + (w * heads + h) * LD + 4 * d4);
-#pragma unroll
-            for (int i = 0; i < 4; i++) acc[i] += x[i] * e;
+        for (int v = 0; v < kWaves; v++) join_add(M, L, acc, wave_m[v][h], wave_l[v][h], *(const v4f *)(smem + (v * heads + h) * LD + 4 * d4));
+        if (whole) {
+            finish<DT>(a.out, a.lse, b * (int64_t)a.Hq + head0 + h, D, d4, acc, M, L, len == 0 && !past);
+        } else {
+            *(v4f *)(part + 4 * i) = acc;
+            if (d4 == 0) *(v2f *)(part + heads * D + 2 * h) = v2f{M, L};
         }
-        return acc;
-    };
-    auto finish = [&](int h, int d4, const v4f &acc, float M, float L) {
-        // no token: zeros; tokens whose scores are all -inf: 0 / 0, as softmax
-        const bool none = len == 0 && !past;
-        const float r = none ? 0.0f : 1.0f / L;
-        const int64_t head = b * (int64_t)a.Hq + head0 + h;
-        *(v2i *)(a.out + head * D + 4 * d4) = v2i{(int)pack_half2<DT>(acc[0] * r, acc[1] * r), (int)pack_half2<DT>(acc[2] * r, acc[3] * r)};
-        if (a.lse && d4 == 0) a.lse[head] = none ? -INFINITY : M * kLn2 + logf(L);
-    };
-    if (parts == 1) {
-        for (int i = tid; i < heads * quads; i += kThreads) {
-            const int h = i / quads, d4 = i - h * quads;
-            float M, L;
-            const v4f acc = wave_sum(h, d4, M, L);
-            finish(h, d4, acc, M, L);
-        }
-        return;
     }
+    if (!whole && r == 0) cut = Cut{b, unit, (int)(((x + rounds) * runs - 1) / all - w) + 1};   // (to the last round's run)
 
-    // ---- a part: outputs, then maxima and sums, written and read around the XCDs' own L2s (sc1), so that
-    // the count needs only the wait for the stores
-    constexpr int SC1 = 16;
-    const int64_t unit = id;                                // (sequence, kv head, head tile)
-    float *mine = a.part + (unit * a.splits + split) * a.part_floats;
-    {
-        const __amdgpu_buffer_rsrc_t rs = raw_rsrc(mine);
-        for (int i = tid; i < heads * quads; i += kThreads) {
-            const int h = i / quads, d4 = i - h * quads;
-            float M, L;
-            const v4f acc = wave_sum(h, d4, M, L);
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4i, acc), rs, i * 16, 0, SC1);
-            if (d4 == 0)
-                __builtin_amdgcn_raw_buffer_store_b64(v2i{__float_as_int(M), __float_as_int(L)}, rs,
-                                                      (heads * D + 2 * h) * 4, 0, SC1);
-        }
+    // ---- the run's next unit
+    x += n;
+    if (x >= end) break;
+    r = 0;
+    if (++unit == units) {
+        unit = 0;
+        rounds = span(++b, len, lo, past);
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (tid == 0) arrived = atomicAdd(a.count + unit, 1u);
-    __syncthreads();
-    if (__builtin_amdgcn_readfirstlane(arrived) != (uint32_t)parts - 1) return;
-    // every other workgroup of the unit has counted itself: zero the count for the next launch
-    if (tid == 0) __hip_atomic_store(a.count + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    // The parts' maxima and sums go to LDS (a wave per head turns them into weights), then every load of
-    // the outputs is independent: as many as the registers hold in flight, the parts shared out among
-    // the threads that a narrow unit leaves over.
-    const __amdgpu_buffer_rsrc_t rs = raw_rsrc(a.part + unit * a.splits * a.part_floats);
-    const int pitch = (int)a.part_floats * 4;
-    float *weight = smem, *sums = smem + heads * parts;
-    v4f *red = (v4f *)(smem + (2 * heads * parts + 3) / 4 * 4);
-    for (int i = tid; i < heads * parts; i += kThreads) {
-        const int s = i / heads, h = i - s * heads;
-        const v2i ml = __builtin_amdgcn_raw_buffer_load_b64(rs, (heads * D + 2 * h) * 4 + s * pitch, 0, SC1);
-        weight[h * parts + s] = __int_as_float(ml[0]);
-        sums[h * parts + s] = __int_as_float(ml[1]);
+    __syncthreads();   // LDS is free again
     }
-    __syncthreads();
-    for (int h = wave; h < heads; h += kWaves) {
-        float M = -INFINITY, L = 0.0f;
-        for (int s = lane; s < parts; s += 64) M = fmaxf(M, weight[h * parts + s]);
-        M = wave_max(M);
-        const float ref = M == -INFINITY ? 0.0f : M;
-        for (int s = lane; s < parts; s += 64) {
-            const float e = __builtin_amdgcn_exp2f(weight[h * parts + s] - ref);
-            weight[h * parts + s] = e;
-            L += sums[h * parts + s] * e;
-        }
-        L = wave_add(L);
-        if (lane == 0) wave_m[0][h] = M, wave_l[0][h] = L;
-    }
-    __syncthreads();
-    const int items = heads * quads, sharers = max(1, kThreads / items);
-    const int share = sharers > 1 ? tid / items : 0;
-    for (int i = tid - share * items; i < items && share < sharers; i += kThreads) {
-        const int h = i / quads;
-        v4f acc = {0, 0, 0, 0};
-        constexpr int U = 8;
-        for (int s0 = share; s0 < parts; s0 += U * sharers) {
-            v4i x[U];
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int s = s0 + u * sharers;
-                x[u] = v4i{0, 0, 0, 0};
-                if (s < parts) x[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, i * 16 + s * pitch, 0, SC1);
-            }
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int s = s0 + u * sharers;
-                const float e = s < parts ? weight[h * parts + s] : 0.0f;
-#pragma unroll
-                for (int c = 0; c < 4; c++) acc[c] += __int_as_float(x[u][c]) * e;
-            }
-        }
-        if (sharers == 1) finish(h, i - h * quads, acc, wave_m[0][h], wave_l[0][h]);
-        else red[tid] = acc;
-    }
-    if (sharers == 1) return;
-    __syncthreads();
-    if (tid < items) {
-        const int h = tid / quads;
-        v4f acc = red[tid];
-        for (int k = 1; k < sharers; k++) {
-            const v4f x = red[k * items + tid];
-#pragma unroll
-            for (int c = 0; c < 4; c++) acc[c] += x[c];
-        }
-        finish(h, tid - h * quads, acc, wave_m[0][h], wave_l[0][h]);
-    }
+    if (!a.alone && tid == 0) a.cut[w] = cut;
 }
 
-// ------------------------------------------------------------------ the split
+// Adds up the parts of the units that runs have cut: a workgroup per run and head of a tile.  Part 0 is
+// run w's second, the others the first ones of the runs after it.  A thread has one quad of dims of every
+// 256 / quads-th part, U of them in flight.
+template <int DT>
+__global__ void __launch_bounds__(kThreads)
+join_parts_kernel(AttnArgs a)
+{
+    __shared__ v4f red[kThreads];
+    __shared__ v2f red_ml[kThreads];
+    const uint32_t w = blockIdx.x;
+    const int tid = threadIdx.x, h = blockIdx.y;
+    const Cut cut = a.cut[w];
+    const int hk = cut.unit / a.tiles, ht = cut.unit - hk * a.tiles, heads = min(a.G - ht * kTile, kTile);
+    if (cut.parts == 0 || h >= heads) return;
+    const int quads = a.D / 4, sharers = kThreads / quads, share = tid / quads, d4 = tid - share * quads;
+    const float *first = a.part + (int64_t)(2 * w) * a.part_floats;
+    float M = -INFINITY, L = 0.0f;
+    v4f acc = {0, 0, 0, 0};
+    constexpr int U = 8;
+    for (int s0 = share; s0 < cut.parts && share < sharers; s0 += U * sharers) {
+        v4f y[U];
+        v2f ml[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int s = s0 + u * sharers;
+            const float *part = first + (int64_t)(s == 0 ? 1 : 2 * s) * a.part_floats;
+            y[u] = v4f{0, 0, 0, 0}, ml[u] = v2f{-INFINITY, 0};
+            if (s < cut.parts) {
+                y[u] = *(const v4f *)(part + h * a.D + 4 * d4);
+                ml[u] = *(const v2f *)(part + heads * a.D + 2 * h);
+            }
+        }
+        float top = M;
+#pragma unroll
+        for (int u = 0; u < U; u++) top = fmaxf(top, ml[u][0]);
+        join_move(M, L, acc, top);
+#pragma unroll
+        for (int u = 0; u < U; u++) join_add(M, L, acc, ml[u][0], ml[u][1], y[u]);
+    }
+    red[tid] = acc;
+    red_ml[tid] = v2f{M, L};
+    __syncthreads();
+    if (share) return;
+    for (int k = 1; k < sharers; k++) M = fmaxf(M, red_ml[k * quads + tid][0]);
+    L = 0.0f;
+    acc = v4f{0, 0, 0, 0};
+    for (int k = 0; k < sharers; k++) join_add(M, L, acc, red_ml[k * quads + tid][0], red_ml[k * quads + tid][1], red[k * quads + tid]);
+    finish<DT>(a.out, a.lse, cut.b * (int64_t)a.Hq + (int64_t)hk * a.G + ht * kTile + h, a.D, d4, acc, M, L, false);
+}
+
+// ------------------------------------------------------------------ the launch
+// Workgroups that the chip holds at once (launch bounds: 2 of 4 waves per CU, 1 for 256 dims), no more
+// than the rounds can fill.  A run has `least` rounds at least: shorter ones leave more parts to join
+// than they save.
 struct Plan {
-    int tiles, heads, splits, chunk;
-    int64_t part_floats, bytes;
+    int tiles, least, part_floats;
+    int64_t groups, bytes;
 };
 
 Plan plan(int64_t B, int Hq, int Hkv, int D, int64_t max_len)
@@ -537,28 +611,23 @@ Plan plan(int64_t B, int Hq, int Hkv, int D, int64_t max_len)
     Plan p{};
     const int G = Hq / Hkv;
     p.tiles = (G + kTile - 1) / kTile;
-    p.heads = std::min(G, kTile);
+    const int heads = std::min(G, kTile);
     const int64_t units = B * Hkv * p.tiles;
-    const int64_t rounds = std::max<int64_t>((max_len + kGrain - 1) / kGrain, 1);   // of the longest sequence
-    int64_t splits = 1;
-    if (units * 4 <= kCounterBytes) {
-        const int64_t want = (1024 + units - 1) / units;
-        splits = std::min<int64_t>(std::min<int64_t>(std::max<int64_t>(want, (rounds + 7) / 8), rounds), kMaxSplits);
-    }
-    const int64_t per = (rounds + splits - 1) / splits;
-    p.chunk = (int)(per * kGrain);
-    p.splits = (int)((rounds + per - 1) / per);
-    p.part_floats = (int64_t)p.heads * D + (2 * p.heads + 3) / 4 * 4;
-    p.bytes = p.splits > 1 ? kCounterBytes + units * p.splits * p.part_floats * 4 : 0;
+    const int64_t rounds = std::max<int64_t>((max_len + kGrain - 1) / kGrain, 1) * units;
+    p.least = std::max(1, heads * D / 1024);
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) dev = 0;
+    p.groups = std::min<int64_t>((int64_t)cu_count(dev) * groups_per_cu(D), (rounds + p.least - 1) / p.least);
+    p.part_floats = (heads * (D + 2) + 31) / 32 * 32;   // whole lines
+    // units of one round cannot be cut
+    p.bytes = max_len <= kGrain ? 0 : kCounterBytes + (p.groups * (int64_t)sizeof(Cut) + 255) / 256 * 256 + 2 * p.groups * p.part_floats * 4;
     return p;
 }
 
 template <int DT, int CODES, int DD, bool PART>
 int launch(const AttnArgs &a, int64_t groups, hipStream_t st)
 {
-    // the waves' outputs, then (the joining workgroup) the parts' weights, sums and 256 quads
-    const int heads = std::min(a.G, kTile);
-    const int lds = std::max(kWaves * heads * (DD + 4), (2 * heads * a.splits + 3) / 4 * 4 + 4 * kThreads) * 4;
+    const int lds = kWaves * std::min(a.G, kTile) * (DD + 4) * 4;   // the waves' outputs
     auto *kernel = paged_attention_kernel<DT, CODES, DD, PART>;
     if (lds > 48 * 1024) {
         static bool raised[64] = {};
@@ -570,7 +639,8 @@ int launch(const AttnArgs &a, int64_t groups, hipStream_t st)
             raised[dev] = true;
         }
     }
-    kernel<<<(unsigned)groups, kThreads, lds, st>>>(a);   // at most 65 KB (256 dims), 37 KB (256 splits)
+    kernel<<<(unsigned)groups, kThreads, lds, st>>>(a);
+    if (!a.alone) join_parts_kernel<DT><<<dim3((unsigned)groups, std::min(a.G, kTile)), kThreads, 0, st>>>(a);
     return check_launch("paged_attention");
 }
 
@@ -616,19 +686,21 @@ int psq_paged_attention(int codes, const void *q, int dtype, int64_t q_batch, in
         return set_error(PSQ_E_SHAPE, "%s: queries and output must be 16-byte aligned, query strides multiples of 8", name);
     if (((uintptr_t)block_table | (uintptr_t)lengths | (uintptr_t)lse) & 3)
         return set_error(PSQ_E_SHAPE, "%s: misaligned table, lengths or lse", name);
-    if (B > 65535 || table_cols > 0x3fffffffLL / page_size)
+    if (B > 65535 || table_cols > 0x3fffffffLL / page_size || B * (table_cols * page_size / kGrain + 1) > 0x7fffffffLL)
         return set_error(PSQ_E_SHAPE, "%s: %lld sequences of %lld pages are too many", name, (long long)B, (long long)table_cols);
     if ((uintptr_t)workspace & 255) return set_error(PSQ_E_SHAPE, "%s: the workspace must be 256-byte aligned", name);
     const int64_t cap = table_cols * page_size;
-    Plan p = plan(B, Hq, Hkv, D, std::min(max_len, cap));
-    if (p.splits > 1 && (!workspace || workspace_bytes < p.bytes)) p.splits = 1;
-    const int64_t groups = B * Hkv * p.tiles * p.splits;
+    const Plan p = plan(B, Hq, Hkv, D, std::min(max_len, cap));
+    const bool alone = !p.bytes || !workspace || workspace_bytes < p.bytes;
+    const int64_t groups = alone ? B * Hkv * p.tiles : p.groups;
     if (groups > 0x7fffffffLL) return set_error(PSQ_E_SHAPE, "%s: %lld workgroups are too many", name, (long long)groups);
     if (int e = require_device()) return e;
+    Cut *cut = (Cut *)((uint8_t *)workspace + kCounterBytes);
     const AttnArgs a{(const uint16_t *)q, q_batch, q_head, (const uint8_t *)k_cache, (const uint8_t *)v_cache, k_scale, v_scale,
-                     block_table, table_stride, lengths, (uint16_t *)out, lse, (uint32_t *)workspace,
-                     (float *)((uint8_t *)workspace + kCounterBytes), p.part_floats, (int)num_pages, (int)cap, page_size, Hq, Hkv,
-                     D, Hq / Hkv, p.tiles, p.splits, p.chunk, (int)std::min<int64_t>(window, cap), scale * kLog2e};
+                     block_table, table_stride, lengths, (uint16_t *)out, lse, cut,
+                     (float *)((uint8_t *)cut + (p.groups * sizeof(Cut) + 255) / 256 * 256), p.part_floats, (int)num_pages, (int)cap,
+                     (int)B, page_size, Hq, Hkv, D, Hq / Hkv, p.tiles, (int)std::min<int64_t>(window, cap), p.least, alone,
+                     scale * kLog2e};
     hipStream_t st = (hipStream_t)stream;
     auto go = [&](auto dtc) {
         constexpr int DT = decltype(dtc)::value;
