@@ -486,20 +486,34 @@ def dequant_fp8(q, w_scale, out_dtype=torch.bfloat16, e5m2=None):
 
 
 # ------------------------------------------------------------------ text decoder
-# What a decoder layer does between its quantized linears.  The checks are written out flat and the
-# addresses passed as integers: at one token the host call is most of the time.
+# What a decoder layer does between its quantized linears.  At one token the host call is most of the time,
+# so the checks are written out flat and addresses go to the library as integers (us a call, host side,
+# against the first form with tuples and loops: add_rms_norm HOST_NORM, kv_write HOST_WRITE, kv_read HOST_READ,
+# paged_attention HOST_ATTEND).
 CODES = {None: _native.CODES_NONE, "none": _native.CODES_NONE, "int8": _native.CODES_I8, "fp8": _native.CODES_E4M3}
 _CODE_DTYPES = {torch.int8: _native.CODES_I8, torch.float8_e4m3fn: _native.CODES_E4M3,
                 torch.bfloat16: _native.CODES_NONE, torch.float16: _native.CODES_NONE}
-_HALF = (torch.bfloat16, torch.float16)
+_HALF = {torch.bfloat16: _native.BF16, torch.float16: _native.F16}
+_ROW_DTYPES = (None, torch.int8, torch.float8_e4m3fn)   # of codes
 
 
-def _one_device(name, first, *others):
-    """RuntimeError unless all tensors (None apart) are on the GPU of the first."""
-    device = first.device
-    for t in (first,) + others:
-        if t is not None and (t.device != device or device.type != "cuda"):
-            raise RuntimeError(f"{name}: psquant kernels need tensors of one GPU (got {device}, {t.device})")
+def _raw(index):
+    """The current stream of device `index` as an integer."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def _call(name, fn, *args):
+    """_launch for integer arguments."""
+    if _timer is not None:
+        return _launch(name, fn, *args)
+    status = fn(*args)
+    if status:
+        _native.check(status, name)
+
+
+def _elsewhere(name, *tensors):
+    raise RuntimeError(f"{name}: psquant kernels need tensors of one GPU (got "
+                       f"{', '.join(str(t.device) for t in tensors if t is not None)})")
 
 
 def add_rms_norm(x, weight, eps=1e-6, residual=None, codes=None, rot_group=0, static_scale=None):
@@ -510,75 +524,98 @@ def add_rms_norm(x, weight, eps=1e-6, residual=None, codes=None, rot_group=0, st
     static_scale: fp32 tensor with one element in the place of the rows' own scales.
     Returns (rows [M, K], scale [M] fp32 or None, h or None when there is no residual).
     """
-    _one_device("add_rms_norm", x, weight, residual)
-    code = CODES.get(codes)
+    index = x.get_device()
+    if index < 0 or weight.get_device() != index or (residual is not None and residual.get_device() != index):
+        _elsewhere("add_rms_norm", x, weight, residual)
+    code, dtype = CODES.get(codes), x.dtype
+    dt = _HALF.get(dtype)
     if code is None:
         raise ValueError(f"add_rms_norm: unknown codes {codes!r}")
-    if x.dtype not in _HALF:
-        raise TypeError(f"add_rms_norm: rows must be bf16/f16, got {x.dtype}")
-    if static_scale is not None and not code:
-        raise ValueError("add_rms_norm: a static scale needs codes")
-    x = _rows2d(x)
+    if dt is None:
+        raise TypeError(f"add_rms_norm: rows must be bf16/f16, got {dtype}")
+    if x.dim() != 2:
+        raise ValueError(f"add_rms_norm: rows must be [M, K], got {tuple(x.shape)}")
     M, K = x.shape
     if weight.numel() != K:
         raise ValueError(f"add_rms_norm: weight has {weight.numel()} elements, expected {K}")
+    if not x.is_contiguous() or x.data_ptr() % 16 or K % 8:
+        x = _rows2d(x)
     if not weight.is_contiguous() or weight.data_ptr() % 16:
         weight = torch.empty(K, dtype=weight.dtype, device=weight.device).copy_(weight.reshape(-1))
-    h, ldr = None, 0
+    device, h, ldr = x.device, None, 0
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype != x.dtype:
+        if residual.shape != x.shape or residual.dtype is not dtype:
             raise ValueError(f"add_rms_norm: residual {tuple(residual.shape)} {residual.dtype} does not match the rows")
-        residual = _rows2d(residual)
+        if not residual.is_contiguous() or residual.data_ptr() % 16 or K % 8:
+            residual = _rows2d(residual)
         ldr = residual.stride(0)
-        h = torch.empty(M, K, dtype=x.dtype, device=x.device)
-    scale, st = None, None
-    if code:
-        out = torch.empty(M, K, dtype=torch.int8 if code == _native.CODES_I8 else torch.float8_e4m3fn, device=x.device)
-        scale = torch.empty(M, dtype=torch.float32, device=x.device)
-        if static_scale is not None:
-            st = static_scale.to(device=x.device, dtype=torch.float32).reshape(-1)[:1].contiguous()
-    else:
-        out = torch.empty(M, K, dtype=x.dtype, device=x.device)
-    _launch("add_rms_norm", _native.lib().psq_add_rms_norm, code, x.data_ptr(), _DT[x.dtype], x.stride(0),
-            None if residual is None else residual.data_ptr(), ldr, weight.data_ptr(), _dt(weight, "weight"), eps,
-            None if h is None else h.data_ptr(), K, int(rot_group or 0), None if st is None else st.data_ptr(),
-            out.data_ptr(), K, None if scale is None else scale.data_ptr(), M, K, _stream(x))
+        h = torch.empty((M, K), dtype=dtype, device=device)
+    out = torch.empty((M, K), dtype=_ROW_DTYPES[code] or dtype, device=device)
+    scale = torch.empty((M,), dtype=torch.float32, device=device) if code else None
+    if static_scale is not None:
+        if not code:
+            raise ValueError("add_rms_norm: a static scale needs codes")
+        static_scale = static_scale.to(device=device, dtype=torch.float32).reshape(-1)[:1].contiguous()
+    _call("add_rms_norm", _native.lib().psq_add_rms_norm, code, x.data_ptr(), dt, x.stride(0),
+          None if residual is None else residual.data_ptr(), ldr, weight.data_ptr(), _dt(weight, "weight"), eps,
+          None if h is None else h.data_ptr(), K, int(rot_group or 0), None if static_scale is None else static_scale.data_ptr(),
+          out.data_ptr(), K, scale.data_ptr() if code else None, M, K, _raw(index))
     return out, scale, h
 
 
-def _kv_pools(name, k_cache, v_cache, k_scale, v_scale):
-    """(codes, pages, kv heads, page size, head dim) of a paged cache's pools, checked."""
-    code = _CODE_DTYPES.get(k_cache.dtype)
-    if code is None or v_cache.dtype is not k_cache.dtype:
+def _pools_error(name, k_cache, v_cache, k_scale, v_scale):
+    """Raises what is wrong with a paged cache's pools."""
+    if _CODE_DTYPES.get(k_cache.dtype) is None or v_cache.dtype is not k_cache.dtype:
         raise TypeError(f"{name}: unsupported cache dtypes {k_cache.dtype}, {v_cache.dtype}")
-    shape = k_cache.shape
-    if len(shape) != 4 or v_cache.shape != shape:
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
         raise ValueError(f"{name}: the pools must both be [pages, kv heads, page size, head dim], got "
-                         f"{tuple(shape)}, {tuple(v_cache.shape)}")
+                         f"{tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError(f"{name}: the pools must be contiguous")
-    if code:
-        if k_scale is None or v_scale is None:
-            raise ValueError(f"{name}: a cache of codes needs its scales")
-        for t in (k_scale, v_scale):
-            if t.shape != shape[:3] or t.dtype is not torch.float32 or not t.is_contiguous():
-                raise ValueError(f"{name}: scales must be contiguous fp32 [pages, kv heads, page size]")
-    elif k_scale is not None or v_scale is not None:
+    if _CODE_DTYPES[k_cache.dtype] == _native.CODES_NONE:
         raise ValueError(f"{name}: a 16-bit cache has no scales")
-    return (code,) + tuple(shape)
+    if k_scale is None or v_scale is None:
+        raise ValueError(f"{name}: a cache of codes needs its scales")
+    raise ValueError(f"{name}: scales must be contiguous fp32 [pages, kv heads, page size] on the pools' GPU")
 
 
-def _slots(name, slots, T=None):
+def _pools(name, index, k_cache, v_cache, k_scale, v_scale):
+    """(codes, pools' shape, scales' addresses) of a paged cache on GPU `index`, checked."""
+    if k_cache.get_device() != index or v_cache.get_device() != index or index < 0:
+        _elsewhere(name, k_cache, v_cache)
+    kind, shape = k_cache.dtype, k_cache.shape
+    code = _CODE_DTYPES.get(kind)
+    if (code is None or v_cache.dtype is not kind or len(shape) != 4 or v_cache.shape != shape or not k_cache.is_contiguous()
+            or not v_cache.is_contiguous()):
+        _pools_error(name, k_cache, v_cache, k_scale, v_scale)
+    if not code:
+        if k_scale is not None or v_scale is not None:
+            _pools_error(name, k_cache, v_cache, k_scale, v_scale)
+        return code, shape, None, None
+    if (k_scale is None or v_scale is None or k_scale.shape != shape[:3] or v_scale.shape != shape[:3]
+            or k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32 or not k_scale.is_contiguous()
+            or not v_scale.is_contiguous() or k_scale.get_device() != index or v_scale.get_device() != index):
+        _pools_error(name, k_cache, v_cache, k_scale, v_scale)
+    return code, shape, k_scale.data_ptr(), v_scale.data_ptr()
+
+
+def _slots(name, slots, index, T=None):
+    """slots' address (and the tensor that has it), checked: int64 [tokens] on GPU `index`."""
+    if slots.get_device() != index:
+        _elsewhere(name, slots)
     if slots.dim() != 1 or slots.dtype is not torch.int64 or (T is not None and slots.shape[0] != T):
         raise ValueError(f"{name}: slots must be int64 [tokens], got {slots.dtype} {tuple(slots.shape)}")
-    return slots.contiguous()
+    return slots if slots.is_contiguous() else slots.contiguous()
 
 
-def _heads(name, t, dim):
-    """[tokens, heads, dim] with unit element stride, 16-byte aligned heads: t itself or a packed copy."""
-    if t.stride(2) != 1 or (t.stride(0) | t.stride(1)) % 8 or t.data_ptr() % 16:
+def _heads(t):
+    """(t, token stride, head stride) of [tokens, heads, dim] with unit element stride and 16-byte aligned
+    heads: t itself or a packed copy."""
+    a, b, c = t.stride()
+    if c != 1 or (a | b) & 7 or t.data_ptr() & 15:
         t = torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
-    return t
+        a, b, c = t.stride()
+    return t, a, b
 
 
 def kv_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
@@ -589,37 +626,40 @@ def kv_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
     k_cache, v_cache: [pages, kv heads, page size, head dim], of k's dtype, int8 or float8_e4m3fn;
     k_scale, v_scale: [pages, kv heads, page size] fp32 for codes (scale = max|row| / 127 or / 448).
     """
-    _one_device("kv_write", k, v, slots, k_cache, v_cache, k_scale, v_scale)
-    code, pages, H, page, D = _kv_pools("kv_write", k_cache, v_cache, k_scale, v_scale)
-    if k.dtype not in _HALF or v.dtype is not k.dtype or (not code and k_cache.dtype is not k.dtype):
-        raise TypeError(f"kv_write: keys {k.dtype} and values {v.dtype} do not fit a {k_cache.dtype} cache")
-    if k.dim() != 3 or k.shape != v.shape or k.shape[1] != H or k.shape[2] != D:
-        raise ValueError(f"kv_write: keys {tuple(k.shape)} and values {tuple(v.shape)} must be [tokens, {H}, {D}]")
-    slots = _slots("kv_write", slots, k.shape[0])
-    k, v = _heads("kv_write", k, D), _heads("kv_write", v, D)
-    _launch("kv_write", _native.lib().psq_kv_write, code, k.data_ptr(), v.data_ptr(), _DT[k.dtype], k.stride(0), k.stride(1),
-            v.stride(0), v.stride(1), slots.data_ptr(), k.shape[0], H, D, k_cache.data_ptr(), v_cache.data_ptr(),
-            None if k_scale is None else k_scale.data_ptr(), None if v_scale is None else v_scale.data_ptr(), pages, page,
-            _stream(k))
+    index = k.get_device()
+    code, (pages, H, page, D), ks, vs = _pools("kv_write", index, k_cache, v_cache, k_scale, v_scale)
+    if v.get_device() != index:
+        _elsewhere("kv_write", k, v)
+    dtype, shape = k.dtype, k.shape
+    dt = _HALF.get(dtype)
+    if dt is None or v.dtype is not dtype or (not code and k_cache.dtype is not dtype):
+        raise TypeError(f"kv_write: keys {dtype} and values {v.dtype} do not fit a {k_cache.dtype} cache")
+    if len(shape) != 3 or v.shape != shape or shape[1] != H or shape[2] != D:
+        raise ValueError(f"kv_write: keys {tuple(shape)} and values {tuple(v.shape)} must be [tokens, {H}, {D}]")
+    T = shape[0]
+    slots = _slots("kv_write", slots, index, T)
+    k, k_token, k_head = _heads(k)
+    v, v_token, v_head = _heads(v)
+    _call("kv_write", _native.lib().psq_kv_write, code, k.data_ptr(), v.data_ptr(), dt, k_token, k_head, v_token, v_head,
+          slots.data_ptr(), T, H, D, k_cache.data_ptr(), v_cache.data_ptr(), ks, vs, pages, page, _raw(index))
 
 
 def kv_read(slots, k_cache, v_cache, k_scale=None, v_scale=None, out_dtype=None):
     """Cached tokens back as dense rows: (k, v), each [tokens, kv heads, head dim] of out_dtype (default: the
     cache's dtype, bf16 for codes).  slots as in kv_write; a negative slot reads as zeros."""
-    _one_device("kv_read", slots, k_cache, v_cache, k_scale, v_scale)
-    code, pages, H, page, D = _kv_pools("kv_read", k_cache, v_cache, k_scale, v_scale)
+    index = slots.get_device()
+    code, (pages, H, page, D), ks, vs = _pools("kv_read", index, k_cache, v_cache, k_scale, v_scale)
     if out_dtype is None:
         out_dtype = torch.bfloat16 if code else k_cache.dtype
-    if out_dtype not in _DT:
+    dt = _DT.get(out_dtype)
+    if dt is None:
         raise TypeError(f"kv_read: unsupported dtype {out_dtype}")
-    slots = _slots("kv_read", slots)
+    slots = _slots("kv_read", slots, index)
     T = slots.shape[0]
-    k = torch.empty(T, H, D, dtype=out_dtype, device=slots.device)
-    v = torch.empty(T, H, D, dtype=out_dtype, device=slots.device)
-    _launch("kv_read", _native.lib().psq_kv_read, code, slots.data_ptr(), T, k_cache.data_ptr(), v_cache.data_ptr(),
-            0 if code else _DT[k_cache.dtype], None if k_scale is None else k_scale.data_ptr(),
-            None if v_scale is None else v_scale.data_ptr(), pages, page, H, D, k.data_ptr(), v.data_ptr(), _DT[out_dtype],
-            _stream(slots))
+    k = torch.empty((T, H, D), dtype=out_dtype, device=slots.device)
+    v = torch.empty_like(k)
+    _call("kv_read", _native.lib().psq_kv_read, code, slots.data_ptr(), T, k_cache.data_ptr(), v_cache.data_ptr(),
+          0 if code else _HALF[k_cache.dtype], ks, vs, pages, page, H, D, k.data_ptr(), v.data_ptr(), dt, _raw(index))
     return k, v
 
 
@@ -631,41 +671,44 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, k_scale=None, v_s
     dtype.  block_table: [batch, columns] int32, the page of token t in column t // page_size; lengths:
     [batch] int32, each sequence's tokens, the new one included (0: zeros).  scale: of the scores (default
     head_dim ** -0.5); window: the last tokens that are attended to (0: all).  max_len: about the longest
-    length, which the host plans the split over the length by (default: what the table can hold).
+    length, for the number of workgroups (default: what the table can hold; any value gives right results).
     return_lse: also the natural log of the softmax's denominator, [batch, heads] fp32.
     A sequence that needs a page outside the pool, or more tokens than its table has, gets NaN.
     """
-    _one_device("paged_attention", q, k_cache, v_cache, block_table, lengths, k_scale, v_scale)
-    code, pages, Hk, page, D = _kv_pools("paged_attention", k_cache, v_cache, k_scale, v_scale)
-    if q.dtype not in _HALF or (not code and k_cache.dtype is not q.dtype):
-        raise TypeError(f"paged_attention: {q.dtype} queries do not fit a {k_cache.dtype} cache")
-    if q.dim() != 3 or q.shape[2] != D or q.shape[1] % Hk:
-        raise ValueError(f"paged_attention: queries {tuple(q.shape)} must be [batch, a multiple of {Hk}, {D}]")
-    B, H, _ = q.shape
-    if block_table.dim() != 2 or block_table.shape[0] != B or block_table.dtype is not torch.int32:
+    index = q.get_device()
+    code, (pages, Hk, page, D), ks, vs = _pools("paged_attention", index, k_cache, v_cache, k_scale, v_scale)
+    if block_table.get_device() != index or lengths.get_device() != index:
+        _elsewhere("paged_attention", q, block_table, lengths)
+    dtype, shape = q.dtype, q.shape
+    dt = _HALF.get(dtype)
+    if dt is None or (not code and k_cache.dtype is not dtype):
+        raise TypeError(f"paged_attention: {dtype} queries do not fit a {k_cache.dtype} cache")
+    if len(shape) != 3 or shape[2] != D or shape[1] % Hk:
+        raise ValueError(f"paged_attention: queries {tuple(shape)} must be [batch, a multiple of {Hk}, {D}]")
+    B, H, _ = shape
+    if block_table.dim() != 2 or block_table.dtype is not torch.int32 or block_table.shape[0] != B:
         raise ValueError(f"paged_attention: block_table must be int32 [{B}, columns]")
-    if lengths.shape != (B,) or lengths.dtype is not torch.int32:
+    if lengths.dtype is not torch.int32 or lengths.dim() != 1 or lengths.shape[0] != B:
         raise ValueError(f"paged_attention: lengths must be int32 [{B}]")
-    window = int(window or 0)
-    if window < 0:
+    if window is None or window < 0:
         raise ValueError("paged_attention: window must be 0 or more")
     cols = block_table.shape[1]
-    if block_table.stride(1) != 1 and cols > 1:
+    if not block_table.is_contiguous() and cols > 1 and block_table.stride(1) != 1:
         block_table = block_table.contiguous()
-    lengths = lengths.contiguous()
-    q = _heads("paged_attention", q, D)
-    max_len = cols * page if max_len is None else max(0, int(max_len))
-    if window:
-        max_len = min(max_len, window)
-    lib, stream = _native.lib(), _stream(q)
-    out = torch.empty(B, H, D, dtype=q.dtype, device=q.device)
-    lse = torch.empty(B, H, dtype=torch.float32, device=q.device) if return_lse else None
-    ws, nb = _workspace(q.device, stream.value, lib.psq_paged_attention_workspace_bytes(code, B, H, Hk, D, max_len))
-    _launch("paged_attention", lib.psq_paged_attention, code, q.data_ptr(), _DT[q.dtype], q.stride(0), q.stride(1),
-            k_cache.data_ptr(), v_cache.data_ptr(), None if k_scale is None else k_scale.data_ptr(),
-            None if v_scale is None else v_scale.data_ptr(), pages, page, block_table.data_ptr(), block_table.stride(0), cols,
-            lengths.data_ptr(), B, H, Hk, D, D ** -0.5 if scale is None else float(scale), window, max_len, out.data_ptr(),
-            None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), nb, stream)
+    if not lengths.is_contiguous():
+        lengths = lengths.contiguous()
+    q, q_batch, q_head = _heads(q)
+    max_len = cols * page if max_len is None or max_len < 0 else int(max_len)
+    if window and window < max_len:
+        max_len = int(window)
+    lib, raw, device = _native.lib(), _raw(index), q.device
+    out = torch.empty((B, H, D), dtype=dtype, device=device)
+    lse = torch.empty((B, H), dtype=torch.float32, device=device) if return_lse else None
+    ws, nb = _workspace(device, raw or None, lib.psq_paged_attention_workspace_bytes(code, B, H, Hk, D, max_len))
+    _call("paged_attention", lib.psq_paged_attention, code, q.data_ptr(), dt, q_batch, q_head, k_cache.data_ptr(),
+          v_cache.data_ptr(), ks, vs, pages, page, block_table.data_ptr(), block_table.stride(0), cols, lengths.data_ptr(), B, H,
+          Hk, D, D ** -0.5 if scale is None else scale, window, max_len, out.data_ptr(), lse.data_ptr() if return_lse else None,
+          None if ws is None else ws.data_ptr(), nb, raw)
     return (out, lse) if return_lse else out
 
 
