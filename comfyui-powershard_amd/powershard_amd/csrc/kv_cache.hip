@@ -102,7 +102,9 @@ __device__ __forceinline__ void row16(const uint8_t *pool, const float *scale, i
     if constexpr (CODES == PSQ_CODES_NONE) {
         load16<DT>((const uint16_t *)pool + at * D + e, f);
     } else {
-        const v4i q = *(const v4i *)(pool + at * D + e);
+        // read once: kept out of the caches, which then hold the rows written (65489 x 8 x 128 93 -> 83 us;
+        // non-temporal stores as well: 125)
+        const v4i q = __builtin_nontemporal_load((const v4i *)(pool + at * D + e));
         const float s = scale[at];
 #pragma unroll
         for (int i = 0; i < 4; i++) {

@@ -24,8 +24,9 @@
 // Work is dealt in rounds of 128 tokens (a step of each wave).  The rounds of all units (sequence, kv
 // head, head tile), in their order, are cut into equal runs, one per workgroup, as many workgroups as the
 // chip holds at once: ragged lengths cost no balance, the host needs no lengths, and a unit is cut only
-// where a run ends.  The parts of a cut unit go through the workspace to a second kernel, which adds them
-// up in their order: results do not depend on timing.
+// where a run ends.  A workgroup writes its parts of cut units (two at most) to the workspace and counts
+// itself when its run is done; the last one of a unit, or a second kernel (see plan()), adds the parts up
+// in their order, so results do not depend on timing.
 #include "kv_cache.hpp"
 
 #include <algorithm>
@@ -41,13 +42,14 @@ constexpr int kStep = 32;                       // tokens of a wave's step
 constexpr int kTile = 16;                       // heads of a workgroup; tokens of a group (one page holds it)
 constexpr int kGrain = kStep * kWaves;          // tokens of a workgroup's round
 constexpr int64_t kCounterBytes = 64 * 1024;    // arrival counters of the GEMMs at the workspace's head
+constexpr int SC1 = 16;                         // cache-policy bit sc1 of the buffer intrinsics
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// The unit that a run begins and does not end: its sequence, index in it, and parts (0: no such unit).
-struct Cut { int b, unit, parts; };
+// A cut unit that a run has part of: its sequence, index in it, first run and number of parts.
+struct Cut { int b, unit, first, parts; };
 
-// workgroups that a CU holds at once
-constexpr int groups_per_cu(int D) { return D > 128 ? 1 : D > 64 ? 2 : 3; }
+// workgroups that a CU holds at once (4 waves; 512, 256 and 168 registers a lane)
+constexpr int groups_per_cu(int D, bool codes) { return D > 128 ? (codes ? 2 : 1) : 3; }
 
 struct AttnArgs {
     const uint16_t *q;
@@ -59,13 +61,14 @@ struct AttnArgs {
     const int32_t *lengths;
     uint16_t *out;
     float *lse;
-    Cut *cut;              // one per run
+    uint32_t *count;       // one per run: of the unit that it begins
+    Cut *cut;              // likewise
     float *part;           // two per run
     int part_floats;       // of one part
     int num_pages, cap;    // cap: tokens that a table row has room for
     int B, page, Hq, Hkv, D, G, tiles, window;
-    int least;             // rounds that a workgroup's run has at least
-    int alone;             // no workspace: units stay whole
+    int alone;             // units stay whole, a workgroup each
+    int apart;             // parts are joined by a kernel of their own
     float scale;           // times log2(e)
 };
 
@@ -184,6 +187,65 @@ __device__ __forceinline__ void finish(uint16_t *out, float *lse, int64_t head, 
     if (lse && d4 == 0) lse[head] = none ? -INFINITY : M * kLn2 + logf(L);
 }
 
+// Adds up the parts of heads h0 .. h0 + n - 1 of a cut unit: part 0 is its first run's second, the others the
+// first ones of the runs after it.  A thread has one quad of dims (of every 256 / quads-th part, where
+// these are few), U parts' loads in flight.  smem: 6 KB.
+template <int DT, int U>
+__device__ __forceinline__ void join_parts(const AttnArgs &a, const Cut &cut, int h0, int n, float *smem)
+{
+    const int tid = threadIdx.x;
+    const int hk = cut.unit / a.tiles, ht = cut.unit - hk * a.tiles, heads = min(a.G - ht * kTile, kTile);
+    const int64_t row0 = cut.b * (int64_t)a.Hq + hk * a.G + ht * kTile;
+    const int quads = a.D / 4, first = h0 * quads, items = min(heads - h0, n) * quads, sharers = max(kThreads / max(items, 1), 1);
+    const int share = sharers > 1 ? tid / items : 0;
+    const __amdgpu_buffer_rsrc_t rs = raw_rsrc(a.part + (int64_t)(2 * cut.first) * a.part_floats);
+    const int pitch = a.part_floats * 4, ml_at = heads * a.D * 4;
+    v4f *red = (v4f *)smem;
+    v2f *red_ml = (v2f *)(smem + 4 * kThreads);
+    __syncthreads();   // LDS is free
+    for (int i = tid - share * items; i < items && share < sharers; i += kThreads) {
+        const int q = first + i, h = q / quads;
+        float M = -INFINITY, L = 0.0f;
+        v4f acc = {0, 0, 0, 0};
+        for (int s0 = share; s0 < cut.parts; s0 += U * sharers) {
+            v4i y[U];
+            v2i ml[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int s = s0 + u * sharers, at = (s == 0 ? 1 : 2 * s) * pitch;
+                y[u] = v4i{0, 0, 0, 0}, ml[u] = v2i{(int)0xff800000, 0};   // no part: maximum -inf, sum 0
+                if (s < cut.parts) {
+                    y[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, at + q * 16, 0, SC1);
+                    ml[u] = __builtin_amdgcn_raw_buffer_load_b64(rs, at + ml_at + 8 * h, 0, SC1);
+                }
+            }
+            float top = M;
+#pragma unroll
+            for (int u = 0; u < U; u++) top = fmaxf(top, __int_as_float(ml[u][0]));
+            join_move(M, L, acc, top);
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                join_add(M, L, acc, __int_as_float(ml[u][0]), __int_as_float(ml[u][1]), __builtin_bit_cast(v4f, y[u]));
+        }
+        if (sharers == 1) {
+            finish<DT>(a.out, a.lse, row0 + h, a.D, q - h * quads, acc, M, L, false);
+        } else {
+            red[tid] = acc;
+            red_ml[tid] = v2f{M, L};
+        }
+    }
+    if (sharers == 1) return;
+    __syncthreads();
+    if (tid < items) {
+        const int q = first + tid, h = q / quads;
+        float M = -INFINITY, L = 0.0f;
+        v4f acc = {0, 0, 0, 0};
+        for (int k = 0; k < sharers; k++) M = fmaxf(M, red_ml[k * items + tid][0]);
+        for (int k = 0; k < sharers; k++) join_add(M, L, acc, red_ml[k * items + tid][0], red_ml[k * items + tid][1], red[k * items + tid]);
+        finish<DT>(a.out, a.lse, row0 + h, a.D, q - h * quads, acc, M, L, false);
+    }
+}
+
 // A step's registers.  DD: head dims they are laid out for; PART: D < DD, the rest of a row is not there.
 template <int CODES, int DD, bool PART>
 struct Step {
@@ -244,16 +306,16 @@ struct Step {
 };
 
 template <int DT, int CODES, int DD, bool PART>
-__global__ void __launch_bounds__(kThreads, groups_per_cu(DD))
+__global__ void __launch_bounds__(kThreads, groups_per_cu(DD, CODES != PSQ_CODES_NONE))
 paged_attention_kernel(AttnArgs a)
 {
     using S = Step<CODES, DD, PART>;
-    constexpr int ES = S::ES, DV = S::DV, VW = S::VW, NC = DD / 32, NB = 1;
+    constexpr int ES = S::ES, DV = S::DV, VW = S::VW, NC = DD / 32;
     constexpr int PVT = CODES == PSQ_CODES_NONE ? DT : PSQ_BF16;   // of the second product
     extern __shared__ __attribute__((aligned(16))) float smem[];
     __shared__ float wave_m[kWaves][kTile], wave_l[kWaves][kTile];
     __shared__ uint32_t wave_rounds[kWaves], start_r;
-    __shared__ int start_b;
+    __shared__ int start_b, joins[2];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int m = lane & 15, g = lane >> 4;
@@ -290,7 +352,7 @@ paged_attention_kernel(AttnArgs a)
     before -= own;
     const uint64_t all = uniform((uint64_t)total * units);
     const uint32_t w = blockIdx.x;
-    const uint32_t runs = a.alone ? gridDim.x : (uint32_t)max(min((uint64_t)gridDim.x, divide(all, a.least)), (uint64_t)1);
+    const uint32_t runs = a.alone ? gridDim.x : (uint32_t)max(min((uint64_t)gridDim.x, all), (uint64_t)1);
     auto first_of = [&](uint32_t w) { return all >> 32 ? uniform(w * all / runs) : divide(w * all, runs); };
     uint64_t x = 0, end;
     int b, unit, r = 0;
@@ -299,7 +361,7 @@ paged_attention_kernel(AttnArgs a)
         end = rounds = span(b, len, lo, past);
     } else {
         if (w >= runs) {
-            if (tid == 0) a.cut[w] = Cut{0, 0, 0};
+            if (a.apart && tid == 0) a.cut[w] = Cut{};
             return;
         }
         x = first_of(w), end = first_of(w + 1);
@@ -320,55 +382,67 @@ paged_attention_kernel(AttnArgs a)
         const uint64_t in = x - (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(start_r) * units;
         unit = (int)divide(in, rounds), r = (int)(in - (uint64_t)unit * rounds);
     }
-    Cut cut{0, 0, 0};
+    Cut cut[2] = {};       // what the run has part of: a unit that it goes on with, and one that it leaves
 
-    for (;;) {
-    const int n = (int)min(end - x, (uint64_t)(rounds - r));     // this segment's rounds
-    const int hk = unit / a.tiles, ht = unit - hk * a.tiles;
-    const int heads = min(a.G - ht * kTile, kTile);
-    const int c0 = (lo & ~(kTile - 1)) + r * kGrain, hi = past ? c0 : min(c0 + n * kGrain, len);
-
-    // ---- queries
-    const int64_t head0 = (int64_t)hk * a.G + ht * kTile;
+    // ---- the segment of the run at hand: n rounds of one unit, tokens c0 .. hi - 1
+    int n, hk, ht, heads, c0, hi, steps;
+    int64_t head0;
     v4i qf[NC];
-#pragma unroll
-    for (int c = 0; c < NC; c++) {
-        const int d = ES == 2 ? 32 * c + 8 * g : 64 * (c >> 1) + 16 * g + 8 * (c & 1);
-        qf[c] = v4i{0, 0, 0, 0};
-        if (m < heads && (!PART || d < D)) qf[c] = *(const v4i *)(a.q + b * a.q_batch + (head0 + m) * a.q_head + d);
-    }
-
-    v4f o[DV];
-    float run_m, run_l;
-    bool pair = true;   // probabilities as hi + lo
-
-    const int steps = c0 + kStep * wave < hi ? (hi - c0 - kStep * wave + kGrain - 1) / kGrain : 0;
-    // the pool groups of 32 steps at a time, one per lane: lane 2 s + t has tile t of step s
-    uint32_t grp = 0;
-    bool wild = false;
+    S st;
+    uint32_t grp;          // the pool groups of 32 steps, one per lane: lane 2 s + t has tile t of step s
+    bool wild;             // a page outside the pool
     auto groups = [&](int s0) {
         const int t = c0 + kStep * wave + (s0 + (lane >> 1)) * kGrain + kTile * (lane & 1);
+        bool out = false;
         grp = 0;
         if (t < hi) {
-            const uint32_t n = (uint32_t)t / kTile, col = n / (uint32_t)per_page;
+            const uint32_t i = (uint32_t)t / kTile, col = i / (uint32_t)per_page;
             const int pg = a.table[b * a.table_stride + col];
-            if (pg < 0 || pg >= a.num_pages) wild = true;
-            else grp = ((uint32_t)pg * a.Hkv + hk) * per_page + (n - col * per_page);
+            out = pg < 0 || pg >= a.num_pages;
+            grp = out ? 0 : ((uint32_t)pg * a.Hkv + hk) * per_page + (i - col * per_page);
         }
-        wild = __any(wild);
+        wild = __any(out);
     };
-    // NB steps are in flight or here.  Step s + NB's loads go into step s's registers as soon as these are
-    // read: its keys before the softmax, its values after the second product.
-    S ring[NB];
-    auto load_keys = [&](S &st, int s) {
+    auto load_keys = [&](int s) {
         const int i = 2 * (s & 31);
         st.load_keys(a, __builtin_amdgcn_readlane(grp, i), __builtin_amdgcn_readlane(grp, i + 1), m, g);
     };
-    auto load_values = [&](S &st, int s) {
+    auto load_values = [&](int s) {
         const int i = 2 * (s & 31);
         st.load_values(a, __builtin_amdgcn_readlane(grp, i), __builtin_amdgcn_readlane(grp, i + 1), m, g);
     };
-    auto compute = [&](S &st, int s, bool more) {
+    auto begin = [&]() {   // the first step's loads (no page, no load: the caller looks at wild)
+        wild = false;
+        if (steps) groups(0);
+        if (steps && !wild) {
+            load_keys(0);
+            load_values(0);
+        }
+    };
+    auto open = [&]() {
+        n = (int)min(end - x, (uint64_t)(rounds - r));
+        hk = unit / a.tiles, ht = unit - hk * a.tiles, heads = min(a.G - ht * kTile, kTile);
+        head0 = b * (int64_t)a.Hq + hk * a.G + ht * kTile;
+        c0 = (lo & ~(kTile - 1)) + r * kGrain, hi = past ? c0 : min(c0 + n * kGrain, len);
+        steps = c0 + kStep * wave < hi ? (hi - c0 - kStep * wave + kGrain - 1) / kGrain : 0;
+        const uint16_t *q = a.q + b * a.q_batch + (int64_t)(hk * a.G + ht * kTile + m) * a.q_head;
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            const int d = ES == 2 ? 32 * c + 8 * g : 64 * (c >> 1) + 16 * g + 8 * (c & 1);
+            qf[c] = v4i{0, 0, 0, 0};
+            if (m < heads && (!PART || d < D)) qf[c] = *(const v4i *)(q + d);
+        }
+        begin();
+    };
+    open();
+
+    for (;;) {
+    v4f o[DV];
+    float run_m, run_l;
+    bool pair = true;      // probabilities as hi + lo
+    // The step's keys and values are in flight or here.  The next step's loads go into the same registers
+    // as soon as these are read: its keys before the softmax, its values after the second product.
+    auto compute = [&](int s, bool more) {
         const int t0 = c0 + kStep * wave + s * kGrain;
         v4f sc[2];
 #pragma unroll
@@ -389,7 +463,7 @@ paged_attention_kernel(AttnArgs a)
 #pragma unroll
             for (int i = 0; i < 4; i++) sc[t][i] = x[i] * a.scale * (ES == 1 ? st.ks[t][i] : 1.0f);
         }
-        if (more) load_keys(st, s + NB);
+        if (more) load_keys(s + 1);
         if (t0 < lo || t0 + kStep > hi) {
             // tokens outside: score -inf, and nothing of what their places hold (NaN, Inf) reaches the sums
 #pragma unroll
@@ -457,35 +531,19 @@ paged_attention_kernel(AttnArgs a)
         }
     };
 
-    auto run = [&]() {
+    for (;;) {
 #pragma unroll
         for (int dt = 0; dt < DV; dt++) o[dt] = v4f{0, 0, 0, 0};
         run_m = -INFINITY, run_l = 0.0f;
-        if (!steps) return;
-        groups(0);
-        if (wild) return;
-#pragma unroll
-        for (int i = 0; i < NB; i++)
-            if (i < steps) {
-                load_keys(ring[i], i);
-                load_values(ring[i], i);
+        for (int s = 0; s < steps && !wild; s++) {
+            bool more = s + 1 < steps;
+            if (more && ((s + 1) & 31) == 0) {
+                groups(s + 1);
+                more = !wild;
             }
-        for (int s0 = 0; s0 < steps; s0 += NB)
-#pragma unroll
-            for (int i = 0; i < NB; i++) {
-                const int s = s0 + i;
-                if (s >= steps) break;
-                const bool more = s + NB < steps;
-                if (more && ((s + NB) & 31) == 0) {
-                    groups(s + NB);
-                    if (wild) return;
-                }
-                compute(ring[i], s, more);
-                if (more) load_values(ring[i], s + NB);
-            }
-    };
-    for (;;) {
-        run();
+            compute(s, more);
+            if (more) load_values(s + 1);
+        }
         // An infinite value meets lo = 0 or lo < 0 in the second product: NaN where the sum is infinite.
         // Once more, then, with p as the sum of two equal halves (the precision of one 16-bit number).
         float any = 0.0f;
@@ -493,8 +551,9 @@ paged_attention_kernel(AttnArgs a)
         for (int dt = 0; dt < DV; dt++)
 #pragma unroll
             for (int i = 0; i < 4; i++) any = __builtin_fmaf(o[dt][i], 0.0f, any);
-        if (!pair || !__any(any != any)) break;
+        if (!pair || wild || !__any(any != any)) break;
         pair = false;
+        begin();
     }
     if (wild || past) run_m = 0.0f, run_l = NAN;
 
@@ -506,107 +565,105 @@ paged_attention_kernel(AttnArgs a)
     }
     constexpr int LD = DD + 4;
     if (m < heads) {
-        float *w = smem + (wave * heads + m) * LD;
+        float *row = smem + (wave * heads + m) * LD;
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
             for (int dt = 0; dt < DV; dt += 4)
-                *(v4f *)(w + (4 * g + i) * DV + dt) = v4f{o[dt][i], o[dt + 1][i], o[dt + 2][i], o[dt + 3][i]};
+                *(v4f *)(row + (4 * g + i) * DV + dt) = v4f{o[dt][i], o[dt + 1][i], o[dt + 2][i], o[dt + 3][i]};
     }
-    __syncthreads();
-    const int quads = D / 4;
-    // a run has two parts: of the unit that it goes on with (0) and of the one that it leaves (1)
-    const bool whole = n == rounds;
-    float *part = whole ? nullptr : a.part + (int64_t)(2 * w + (r == 0)) * a.part_floats;
-    for (int i = tid; i < heads * quads; i += kThreads) {
+    // the run's next segment: its first loads travel while this one's sums are put together
+    const bool whole = n == rounds, none = len == 0 && !past;
+    const int quads = D / 4, these = heads;
+    const int64_t row0 = head0;
+    const int slot = r == 0;
+    if (!whole) {
+        auto owner = [&](uint64_t y) { return (int)(all >> 32 ? uniform(((y + 1) * runs - 1) / all) : divide((y + 1) * runs - 1, (uint32_t)all)); };
+        const int first = slot ? (int)w : owner(x - r);
+        cut[slot] = Cut{b, unit, first, owner(x - r + rounds - 1) - first + 1};
+    }
+    x += n;
+    const bool last = x >= end;
+    if (!last) {
+        r = 0;
+        if (++unit == units) {
+            unit = 0;
+            rounds = span(++b, len, lo, past);
+        }
+        open();
+    }
+    stage_barrier();       // (a barrier that leaves loads in flight)
+    const __amdgpu_buffer_rsrc_t part = raw_rsrc(a.part + (int64_t)(2 * w + slot) * a.part_floats);
+    for (int i = tid; i < these * quads; i += kThreads) {
         const int h = i / quads, d4 = i - h * quads;
         const float M = fmaxf(fmaxf(wave_m[0][h], wave_m[1][h]), fmaxf(wave_m[2][h], wave_m[3][h]));
         v4f acc = {0, 0, 0, 0};
         float L = 0.0f;
 #pragma unroll
-        for (int v = 0; v < kWaves; v++) join_add(M, L, acc, wave_m[v][h], wave_l[v][h], *(const v4f *)(smem + (v * heads + h) * LD + 4 * d4));
+        for (int v = 0; v < kWaves; v++) join_add(M, L, acc, wave_m[v][h], wave_l[v][h], *(const v4f *)(smem + (v * these + h) * LD + 4 * d4));
         if (whole) {
-            finish<DT>(a.out, a.lse, b * (int64_t)a.Hq + head0 + h, D, d4, acc, M, L, len == 0 && !past);
+            finish<DT>(a.out, a.lse, row0 + h, D, d4, acc, M, L, none);
         } else {
-            *(v4f *)(part + 4 * i) = acc;
-            if (d4 == 0) *(v2f *)(part + heads * D + 2 * h) = v2f{M, L};
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4i, acc), part, i * 16, 0, SC1);
+            if (d4 == 0)
+                __builtin_amdgcn_raw_buffer_store_b64(v2i{__float_as_int(M), __float_as_int(L)}, part, (these * D + 2 * h) * 4, 0, SC1);
         }
     }
-    if (!whole && r == 0) cut = Cut{b, unit, (int)(((x + rounds) * runs - 1) / all - w) + 1};   // (to the last round's run)
+    if (last) break;
+    stage_barrier();       // LDS is free again
+    }
+    if (a.apart) {         // the second kernel joins
+        if (tid == 0) a.cut[w] = cut[1];
+        return;
+    }
+    if (cut[0].parts + cut[1].parts == 0) return;
 
-    // ---- the run's next unit
-    x += n;
-    if (x >= end) break;
-    r = 0;
-    if (++unit == units) {
-        unit = 0;
-        rounds = span(++b, len, lo, past);
+    // ---- the run's parts are written (around the XCDs' own L2s, sc1: the count needs only the wait for the
+    // stores); the workgroup that counts last adds a unit up
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid < 2) {
+        const int first = tid ? cut[1].first : cut[0].first, parts = tid ? cut[1].parts : cut[0].parts;
+        if (parts) {
+            const bool join = atomicAdd(a.count + first, 1u) == (uint32_t)parts - 1;
+            // every other part has been counted: zero again for the next launch
+            if (join) __hip_atomic_store(a.count + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            joins[tid] = join;
+        } else {
+            joins[tid] = 0;
+        }
     }
-    __syncthreads();   // LDS is free again
-    }
-    if (!a.alone && tid == 0) a.cut[w] = cut;
+    __syncthreads();
+#pragma clang loop unroll(disable)
+    for (int i = 0; i < 2; i++)
+        if (__builtin_amdgcn_readfirstlane(joins[i])) join_parts<DT, DD == 64 ? 8 : 16>(a, i ? cut[1] : cut[0], 0, kTile, smem);
 }
 
-// Adds up the parts of the units that runs have cut: a workgroup per run and head of a tile.  Part 0 is
-// run w's second, the others the first ones of the runs after it.  A thread has one quad of dims of every
-// 256 / quads-th part, U of them in flight.
+// The join as a kernel of its own: a workgroup per run and head of a tile.
 template <int DT>
 __global__ void __launch_bounds__(kThreads)
 join_parts_kernel(AttnArgs a)
 {
-    __shared__ v4f red[kThreads];
-    __shared__ v2f red_ml[kThreads];
-    const uint32_t w = blockIdx.x;
-    const int tid = threadIdx.x, h = blockIdx.y;
-    const Cut cut = a.cut[w];
-    const int hk = cut.unit / a.tiles, ht = cut.unit - hk * a.tiles, heads = min(a.G - ht * kTile, kTile);
-    if (cut.parts == 0 || h >= heads) return;
-    const int quads = a.D / 4, sharers = kThreads / quads, share = tid / quads, d4 = tid - share * quads;
-    const float *first = a.part + (int64_t)(2 * w) * a.part_floats;
-    float M = -INFINITY, L = 0.0f;
-    v4f acc = {0, 0, 0, 0};
-    constexpr int U = 8;
-    for (int s0 = share; s0 < cut.parts && share < sharers; s0 += U * sharers) {
-        v4f y[U];
-        v2f ml[U];
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int s = s0 + u * sharers;
-            const float *part = first + (int64_t)(s == 0 ? 1 : 2 * s) * a.part_floats;
-            y[u] = v4f{0, 0, 0, 0}, ml[u] = v2f{-INFINITY, 0};
-            if (s < cut.parts) {
-                y[u] = *(const v4f *)(part + h * a.D + 4 * d4);
-                ml[u] = *(const v2f *)(part + heads * a.D + 2 * h);
-            }
-        }
-        float top = M;
-#pragma unroll
-        for (int u = 0; u < U; u++) top = fmaxf(top, ml[u][0]);
-        join_move(M, L, acc, top);
-#pragma unroll
-        for (int u = 0; u < U; u++) join_add(M, L, acc, ml[u][0], ml[u][1], y[u]);
-    }
-    red[tid] = acc;
-    red_ml[tid] = v2f{M, L};
-    __syncthreads();
-    if (share) return;
-    for (int k = 1; k < sharers; k++) M = fmaxf(M, red_ml[k * quads + tid][0]);
-    L = 0.0f;
-    acc = v4f{0, 0, 0, 0};
-    for (int k = 0; k < sharers; k++) join_add(M, L, acc, red_ml[k * quads + tid][0], red_ml[k * quads + tid][1], red[k * quads + tid]);
-    finish<DT>(a.out, a.lse, cut.b * (int64_t)a.Hq + (int64_t)hk * a.G + ht * kTile + h, a.D, d4, acc, M, L, false);
+    __shared__ __attribute__((aligned(16))) float smem[6 * kThreads];
+    const Cut cut = a.cut[blockIdx.x];
+    if (cut.parts) join_parts<DT, 8>(a, cut, blockIdx.y, 1, smem);
 }
 
 // ------------------------------------------------------------------ the launch
-// Workgroups that the chip holds at once (launch bounds: 2 of 4 waves per CU, 1 for 256 dims), no more
-// than the rounds can fill.  A run has `least` rounds at least: shorter ones leave more parts to join
-// than they save.
+// As many workgroups as the chip holds, no more than the rounds can fill.  Where units are few (long
+// texts of few users: over 8 parts a unit), parts are joined by a kernel of their own, which spreads a
+// unit's heads over the chip, and two workgroups per CU fill the memory system with fewer parts than
+// three; where units are many, the workgroups of the first kernel join (two or three parts a unit) and
+// a third one per CU covers the gaps between segments.  us, joined apart | inside:
+// 1 x 131071 tokens, 8 kv heads, fp8 62 | 65; 8 x 6000, 1 kv head of 256 dims 22 | 34; 61 x 4096, 8 kv
+// heads, int8 72 | 68; 16 x 8192 (window 1024), 16 kv heads of 64 dims 22.4 | 21.2.
 struct Plan {
-    int tiles, least, part_floats;
-    int64_t groups, bytes;
+    int tiles, part_floats;
+    bool apart;
+    int64_t groups, cuts_at, parts_at, bytes;
 };
 
-Plan plan(int64_t B, int Hq, int Hkv, int D, int64_t max_len)
+Plan plan(int codes, int64_t B, int Hq, int Hkv, int D, int64_t max_len)
 {
     Plan p{};
     const int G = Hq / Hkv;
@@ -614,20 +671,26 @@ Plan plan(int64_t B, int Hq, int Hkv, int D, int64_t max_len)
     const int heads = std::min(G, kTile);
     const int64_t units = B * Hkv * p.tiles;
     const int64_t rounds = std::max<int64_t>((max_len + kGrain - 1) / kGrain, 1) * units;
-    p.least = std::max(1, heads * D / 1024);
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess) dev = 0;
-    p.groups = std::min<int64_t>((int64_t)cu_count(dev) * groups_per_cu(D), (rounds + p.least - 1) / p.least);
+    const int cus = cu_count(dev);
+    const int most = groups_per_cu(D, codes != PSQ_CODES_NONE);
+    p.groups = std::min<int64_t>(cus * std::min(most, 2), rounds);
+    p.apart = p.groups > 8 * units;
+    if (!p.apart) p.groups = std::min<int64_t>(cus * most, rounds);
     p.part_floats = (heads * (D + 2) + 31) / 32 * 32;   // whole lines
+    p.cuts_at = kCounterBytes;
+    p.parts_at = p.cuts_at + (p.groups * (int64_t)sizeof(Cut) + 255) / 256 * 256;
     // units of one round cannot be cut
-    p.bytes = max_len <= kGrain ? 0 : kCounterBytes + (p.groups * (int64_t)sizeof(Cut) + 255) / 256 * 256 + 2 * p.groups * p.part_floats * 4;
+    p.bytes = max_len <= kGrain ? 0 : p.parts_at + 2 * p.groups * p.part_floats * 4;
     return p;
 }
 
 template <int DT, int CODES, int DD, bool PART>
 int launch(const AttnArgs &a, int64_t groups, hipStream_t st)
 {
-    const int lds = kWaves * std::min(a.G, kTile) * (DD + 4) * 4;   // the waves' outputs
+    // the waves' outputs, then (joining) 256 quads with their maxima and sums
+    const int lds = std::max(kWaves * std::min(a.G, kTile) * (DD + 4), 6 * kThreads) * 4;
     auto *kernel = paged_attention_kernel<DT, CODES, DD, PART>;
     if (lds > 48 * 1024) {
         static bool raised[64] = {};
@@ -640,7 +703,7 @@ int launch(const AttnArgs &a, int64_t groups, hipStream_t st)
         }
     }
     kernel<<<(unsigned)groups, kThreads, lds, st>>>(a);
-    if (!a.alone) join_parts_kernel<DT><<<dim3((unsigned)groups, std::min(a.G, kTile)), kThreads, 0, st>>>(a);
+    if (a.apart) join_parts_kernel<DT><<<dim3((unsigned)groups, std::min(a.G, kTile)), kThreads, 0, st>>>(a);
     return check_launch("paged_attention");
 }
 
@@ -662,9 +725,8 @@ extern "C" {
 
 int64_t psq_paged_attention_workspace_bytes(int codes, int64_t B, int Hq, int Hkv, int D, int64_t max_len)
 {
-    (void)codes;
     if (B <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || max_len <= 0 || Hq % Hkv || B > 65535) return 0;
-    return psq::plan(B, Hq, Hkv, D, std::min<int64_t>(max_len, 0x7fffffffLL)).bytes;
+    return psq::plan(codes, B, Hq, Hkv, D, std::min<int64_t>(max_len, 0x7fffffffLL)).bytes;
 }
 
 int psq_paged_attention(int codes, const void *q, int dtype, int64_t q_batch, int64_t q_head, const void *k_cache,
@@ -690,17 +752,16 @@ int psq_paged_attention(int codes, const void *q, int dtype, int64_t q_batch, in
         return set_error(PSQ_E_SHAPE, "%s: %lld sequences of %lld pages are too many", name, (long long)B, (long long)table_cols);
     if ((uintptr_t)workspace & 255) return set_error(PSQ_E_SHAPE, "%s: the workspace must be 256-byte aligned", name);
     const int64_t cap = table_cols * page_size;
-    const Plan p = plan(B, Hq, Hkv, D, std::min(max_len, cap));
+    const Plan p = plan(codes, B, Hq, Hkv, D, std::min(max_len, cap));
     const bool alone = !p.bytes || !workspace || workspace_bytes < p.bytes;
     const int64_t groups = alone ? B * Hkv * p.tiles : p.groups;
     if (groups > 0x7fffffffLL) return set_error(PSQ_E_SHAPE, "%s: %lld workgroups are too many", name, (long long)groups);
     if (int e = require_device()) return e;
-    Cut *cut = (Cut *)((uint8_t *)workspace + kCounterBytes);
     const AttnArgs a{(const uint16_t *)q, q_batch, q_head, (const uint8_t *)k_cache, (const uint8_t *)v_cache, k_scale, v_scale,
-                     block_table, table_stride, lengths, (uint16_t *)out, lse, cut,
-                     (float *)((uint8_t *)cut + (p.groups * sizeof(Cut) + 255) / 256 * 256), p.part_floats, (int)num_pages, (int)cap,
-                     (int)B, page_size, Hq, Hkv, D, Hq / Hkv, p.tiles, (int)std::min<int64_t>(window, cap), p.least, alone,
-                     scale * kLog2e};
+                     block_table, table_stride, lengths, (uint16_t *)out, lse,
+                     (uint32_t *)workspace, (Cut *)((uint8_t *)workspace + p.cuts_at), (float *)((uint8_t *)workspace + p.parts_at),
+                     p.part_floats, (int)num_pages, (int)cap, (int)B, page_size, Hq, Hkv, D, Hq / Hkv, p.tiles,
+                     (int)std::min<int64_t>(window, cap), alone, !alone && p.apart, scale * kLog2e};
     hipStream_t st = (hipStream_t)stream;
     auto go = [&](auto dtc) {
         constexpr int DT = decltype(dtc)::value;

@@ -19,7 +19,8 @@ constexpr int kMaxK = kChunk * kMaxThreads * 2;
 // below this max|h w| a row counts as zero: LIM / max stays finite
 constexpr float kTiny = 0x1p-120f;
 
-template <int DT>
+// 16 elements as fp32.  ONCE: read once, non-temporally (quantize_rows.hip says what that leaves in the caches).
+template <int DT, bool ONCE = false>
 __device__ __forceinline__ void load16(const void *p, float (&v)[16])
 {
     if constexpr (DT == PSQ_F32) {
@@ -29,7 +30,9 @@ __device__ __forceinline__ void load16(const void *p, float (&v)[16])
 #pragma unroll
             for (int j = 0; j < 4; j++) v[4 * i + j] = f[i][j];
     } else {
-        const v4i raw[2] = {((const v4i *)p)[0], ((const v4i *)p)[1]};
+        v4i raw[2];
+        raw[0] = ONCE ? __builtin_nontemporal_load((const v4i *)p) : ((const v4i *)p)[0];
+        raw[1] = ONCE ? __builtin_nontemporal_load((const v4i *)p + 1) : ((const v4i *)p)[1];
         to_f32<DT>(raw, v);
     }
 }
@@ -73,10 +76,10 @@ add_rms_norm_kernel(NormArgs a)
         const int e = (c * T + lc) * kChunk;
         float w[16];
         if (e < a.K) {
-            load16<DT>(a.x + row * a.ldx + e, v[c]);
+            load16<DT, true>(a.x + row * a.ldx + e, v[c]);
             if (a.res) {
                 float r[16];
-                load16<DT>(a.res + row * a.ldr + e, r);
+                load16<DT, true>(a.res + row * a.ldr + e, r);
 #pragma unroll
                 for (int j = 0; j < 16; j++) v[c][j] += r[j];
                 v4i h[2];
