@@ -238,6 +238,19 @@ def requantize_like(template, weight, fmt):
 
 
 # ------------------------------------------------------------------------- module
+class QuantizedRows(NamedTuple):
+    """Input rows as the codes that native W8A8 / fp8 modules multiply (norm.RMSNorm makes them)."""
+    codes: torch.Tensor      # [M, K] int8 or float8_e4m3fn
+    scale: torch.Tensor      # [M] fp32
+    rot_group: int           # ConvRot group that the rows are rotated by
+    shape: tuple             # of the rows they stand for, [..., K]
+    dtype: torch.dtype       # of the rows they stand for
+
+    @property
+    def device(self):
+        return self.codes.device
+
+
 class QuantLinear(nn.Module):
     """Linear whose weight is one QuantizedWeight byte vector (FSDP Shard(0) over bytes)."""
 
@@ -292,6 +305,59 @@ class QuantLinear(nn.Module):
         if activation == "silu_gate" and self.out_features % 2:
             raise ValueError(f"silu_gate needs an even number of output features, got {self.out_features}")
         return self._forward(x, activation)
+
+    def input_codes(self):
+        """("int8" or "fp8", ConvRot group) when the native forward quantizes its rows to that and does
+        nothing else to them, so that forward_codes can take them; else None."""
+        plan = self._ps_qplan
+        if (not self._ps_native or self._ps_full_precision or getattr(self, "_ps_safe", False) or self.in_features % 128
+                or self._ps_compute_dtype not in (torch.bfloat16, torch.float16) or any(s[0].startswith("x:") for s in plan.specs)):
+            return None
+        if plan.layout is qtm.Int8RowwiseLayout:
+            return "int8", plan.fields["convrot_groupsize"] if plan.fields["convrot"] else 0
+        return ("fp8", 0) if plan.layout is qtm.Float8ScaledLayout else None
+
+    def forward_codes(self, rows, activation=None):
+        """self of rows that are quantized already (QuantizedRows as input_codes asks for), activation as
+        in forward_act: the native GEMM alone, the values of the forward on the rows that the codes stand
+        for.  The result has the module's compute dtype."""
+        want = self.input_codes()
+        kind = "int8" if rows.codes.dtype is torch.int8 else "fp8"
+        if want != (kind, rows.rot_group) or rows.codes.shape[1] != self.in_features:
+            raise ValueError(f"forward_codes: {kind} rows [., {rows.codes.shape[1]}] rotated by {rows.rot_group} do not fit "
+                             f"[., {self.in_features}] {want}")
+        dtype = self._ps_compute_dtype
+        out = self._codes_direct(rows, activation)
+        if out is not None:
+            return out
+        qt = unpack(self.qbytes, self._ps_qplan, dtype)
+        bias = None if self.bias is None else self.bias.to(dtype)
+        fused = None if activation == "silu_gate" and self.out_features % 128 else activation
+        out = gemm_codes(rows.codes, rows.scale, qt, bias, dtype, fused)
+        if activation is not None and fused is None:
+            out = apply_activation(out, activation).to(dtype)
+        out = out.reshape(*rows.shape[:-1], out.shape[-1])
+        tracker = getattr(self, "_ps_tracker", None)
+        if tracker is not None:
+            tracker.observe(self._ps_finite_slot, out)
+        return out
+
+    def _codes_direct(self, rows, activation):
+        """forward_codes in one library call, or None where _direct would not take the plain rows."""
+        from . import ops
+        plan, store, bias, dtype = self._ps_qplan, self.qbytes, self.bias, self._ps_compute_dtype
+        (_, code, (N, K), q_at, _), (name, sdtype, _, s_at, s_bytes) = plan.specs[:2]
+        M, weights, count = rows.codes.shape[0], _Q8_WEIGHTS.get(code), s_bytes // 4
+        if (rows.dtype is not dtype or not M or not ops.direct_available() or self.__dict__.get("_ps_tracker") is not None
+                or type(store) not in PLAIN or not store.is_cuda or store.device != rows.device or not store.is_contiguous()
+                or store.numel() < plan.total or store.data_ptr() % 16 or name != "scale" or sdtype is not torch.float32
+                or weights is None or (activation is not None and weights == 2) or (activation == "silu_gate" and N % 128)
+                or (bias is not None and (type(bias) not in PLAIN or bias.dtype is not dtype or bias.device != rows.device
+                                          or bias.numel() != N or not bias.is_contiguous()))):
+            return None
+        base = store.data_ptr()
+        return ops.linear_codes_direct(rows, rows.codes, rows.scale, M, K, weights, base + q_at, base + s_at, int(count > 1), N, bias,
+                                       ops.ACTIVATIONS[activation])
 
     # -- the forward in four steps: compute dtype, the native attempt, the dequantize branch, delivery
     def _dtype_for(self, x):
@@ -505,6 +571,19 @@ def apply_activation(out, activation):
     raise ValueError(f"unsupported activation {activation!r}")
 
 
+def gemm_codes(qx, a_scale, qt, bias, dtype, activation=None):
+    """The W8A8 / fp8 GEMM of quantized rows (activation as in native_linear)."""
+    from . import ops
+    p = qt._params
+    if qt._layout_cls is qtm.Int8RowwiseLayout:
+        return ops.gemm_i8(qx, a_scale, qt._qdata, p.scale, bias, out_dtype=dtype, activation=activation)
+    if qt._qdata.dtype == torch.float8_e5m2 and activation is not None:
+        # e5m2 weights have no fused epilogue: the linear output, rounded, then the activation
+        out = ops.gemm_fp8(qx, a_scale, qt._qdata, p.scale, bias, out_dtype=dtype)
+        return apply_activation(out, activation).to(dtype)
+    return ops.gemm_fp8(qx, a_scale, qt._qdata, p.scale, bias, out_dtype=dtype, activation=activation)
+
+
 def native_linear(rows, qt, bias, fmt, input_scale=None, activation=None):
     """The native GEMM of one format on the gfx950 kernels (replaces F.linear(QuantizedTensor)).
 
@@ -516,17 +595,10 @@ def native_linear(rows, qt, bias, fmt, input_scale=None, activation=None):
     if rows.device.type != "cuda":
         raise RuntimeError("native quantized GEMM needs a GPU tensor")
     layout, p = qt._layout_cls, qt._params
-    if layout is qtm.Int8RowwiseLayout:
-        group = p.convrot_groupsize if p.convrot else 0
-        qx, a_scale = _quantize_input(rows, False, group, input_scale)
-        return ops.gemm_i8(qx, a_scale, qt._qdata, p.scale, bias, out_dtype=rows.dtype, activation=activation)
-    if layout is qtm.Float8ScaledLayout:
-        qx, a_scale = _quantize_input(rows, True, 0, input_scale)
-        if qt._qdata.dtype == torch.float8_e5m2 and activation is not None:
-            # e5m2 weights have no fused epilogue: the linear output, rounded, then the activation
-            out = ops.gemm_fp8(qx, a_scale, qt._qdata, p.scale, bias, out_dtype=rows.dtype)
-            return apply_activation(out, activation).to(rows.dtype)
-        return ops.gemm_fp8(qx, a_scale, qt._qdata, p.scale, bias, out_dtype=rows.dtype, activation=activation)
+    if layout is qtm.Int8RowwiseLayout or layout is qtm.Float8ScaledLayout:
+        int8 = layout is qtm.Int8RowwiseLayout
+        qx, a_scale = _quantize_input(rows, not int8, p.convrot_groupsize if int8 and p.convrot else 0, input_scale)
+        return gemm_codes(qx, a_scale, qt, bias, rows.dtype, activation)
     if layout is qtm.UInt4GroupLayout:
         out = ops.gemm_w4a16(rows, qt._qdata, p.scale, p.zero, p.group_size, bias, out_dtype=rows.dtype)
         if activation is not None:   # weight-only GEMM: the activation stays a separate pass
