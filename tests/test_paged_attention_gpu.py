@@ -97,7 +97,8 @@ TYPES = [("none", torch.bfloat16), ("none", torch.float16), ("int8", torch.bfloa
 
 @pytest.mark.parametrize("codes,dtype", TYPES)
 @pytest.mark.parametrize("Hq,Hk,D,page", [(5, 1, 128, 16), (8, 8, 64, 32), (32, 4, 128, 64), (16, 1, 256, 48), (34, 2, 128, 16),
-                                          (3, 3, 16, 16), (6, 2, 96, 80), (20, 4, 240, 128), (7, 7, 144, 16), (40, 1, 80, 32)])
+                                          (3, 3, 16, 16), (6, 2, 96, 80), (20, 4, 240, 128), (7, 7, 144, 16), (40, 1, 80, 32), (64, 1, 64, 16),
+                                          (33, 1, 256, 32), (96, 2, 128, 64), (130, 1, 48, 16)])
 def test_shapes(gpu, codes, dtype, Hq, Hk, D, page):
     """Head layouts, head dims and pages; lengths of none, one, whole and broken tiles and pages."""
     from powershard_amd import ops
@@ -127,6 +128,17 @@ def test_long_and_wide(gpu, B, lens):
     lens = lens or [(b * 37) % 900 for b in range(B)]
     args = make(lens, 40, 8, 128, 32, "int8", torch.bfloat16, gpu, seed=9)
     check(ops.paged_attention(*args), args)
+
+
+@pytest.mark.parametrize("codes,dtype", [("none", torch.float16), ("int8", torch.bfloat16)])
+@pytest.mark.parametrize("heads,lens", [(17, [5000, 3]), (24, [31, 32, 33, 777]), (64, [3000, 1, 64]), (100, [2049])])
+def test_many_heads_share(gpu, codes, dtype, heads, lens):
+    """More heads to a kv head than a wave has, split over the length."""
+    from powershard_amd import ops
+    args = make(lens, heads, 1, 128, 16, codes, dtype, gpu)
+    check(ops.paged_attention(*args), args)
+    two = make(lens, 2 * heads, 2, 64, 64, codes, dtype, gpu)
+    check(ops.paged_attention(*two, max_len=1), two)
 
 
 @pytest.mark.parametrize("codes,dtype", [("none", torch.bfloat16), ("fp8", torch.float16)])
