@@ -340,7 +340,7 @@ paged_attention_kernel(AttnArgs a)
     };
     int len, lo, rounds;
     bool past;
-    const int each = (a.B + kThreads - 1) / kThreads;       // sequences of a thread
+    const int each = a.alone ? 0 : (a.B + kThreads - 1) / kThreads;   // sequences of a thread
     uint32_t own = 0;
     for (int i = 0; i < each; i++)
         if (tid * each + i < a.B) own += span(tid * each + i, len, lo, past);

@@ -549,7 +549,7 @@ def add_rms_norm(x, weight, eps=1e-6, residual=None, codes=None, rot_group=0, st
         if not residual.is_contiguous() or residual.data_ptr() % 16 or K % 8:
             residual = _rows2d(residual)
         ldr = residual.stride(0)
-        h = torch.empty((M, K), dtype=dtype, device=device)
+        h = torch.empty_like(x, memory_format=torch.contiguous_format)
     out = torch.empty((M, K), dtype=_ROW_DTYPES[code] or dtype, device=device)
     scale = torch.empty((M,), dtype=torch.float32, device=device) if code else None
     if static_scale is not None:
