@@ -64,7 +64,7 @@ struct AttnArgs {
     uint16_t *out;
     float *lse;
     uint32_t *count;       // one per run: of the unit that it begins
-    Cut *cut;              // likewise
+    Cut *cut;              // one per unit, where parts are joined apart
     float *part;           // two per run
     int part_floats;       // of one part
     int num_pages, cap;    // cap: tokens that a table row has room for
@@ -369,10 +369,7 @@ paged_attention_kernel(AttnArgs a)
         b = w / (uint32_t)units, unit = w - b * units;
         end = rounds = span(b, len, lo, past);
     } else {
-        if (w >= runs) {
-            if (a.apart && tid == 0) a.cut[w] = Cut{};
-            return;
-        }
+        if (w >= runs) return;
         x = first_of(w), end = first_of(w + 1);
         const uint32_t y = (uint32_t)divide(x, units);      // the thread whose sequences hold the run's start
         if (y >= before && y < before + own) {
@@ -604,6 +601,7 @@ paged_attention_kernel(AttnArgs a)
         const int first = slot ? (int)w : owner(x - r);
         cut[slot] = Cut{b, unit, first, owner(x - r + rounds - 1) - first + 1};
     }
+    if (a.apart && slot && tid == 0) a.cut[b * units + unit] = whole ? Cut{} : cut[1];   // (its first run says so)
     x += n;
     const bool last = x >= end;
     if (!last) {
@@ -634,11 +632,7 @@ paged_attention_kernel(AttnArgs a)
     if (last) break;
     stage_barrier();       // LDS is free again
     }
-    if (a.apart) {         // the second kernel joins
-        if (tid == 0) a.cut[w] = cut[1];
-        return;
-    }
-    if (cut[0].parts + cut[1].parts == 0) return;
+    if (a.apart || cut[0].parts + cut[1].parts == 0) return;
 
     // ---- the run's parts are written (around the XCDs' own L2s, sc1: the count needs only the wait for the
     // stores); the workgroup that counts last adds a unit up
@@ -661,7 +655,7 @@ paged_attention_kernel(AttnArgs a)
         if (__builtin_amdgcn_readfirstlane(joins[i])) join_parts<DT, DD == 64 ? 8 : 16>(a, i ? cut[1] : cut[0], 0, kTile, smem);
 }
 
-// The join as a kernel of its own: a workgroup per run and head of a tile.
+// The join as a kernel of its own: a workgroup per unit and head of it.
 template <int DT>
 __global__ void __launch_bounds__(kThreads)
 join_parts_kernel(AttnArgs a)
@@ -702,7 +696,7 @@ Plan plan(int codes, int64_t B, int Hq, int Hkv, int D, int64_t max_len)
     if (!p.apart) p.groups = std::min<int64_t>(cus * most, rounds);
     p.part_floats = (heads * (D + 2) + 31) / 32 * 32;   // whole lines
     p.cuts_at = kCounterBytes;
-    p.parts_at = p.cuts_at + (p.groups * (int64_t)sizeof(Cut) + 255) / 256 * 256;
+    p.parts_at = p.cuts_at + (p.apart ? units * (int64_t)sizeof(Cut) + 255 : 0) / 256 * 256;
     // units of one round cannot be cut
     p.bytes = max_len <= kGrain ? 0 : p.parts_at + 2 * p.groups * p.part_floats * 4;
     return p;
@@ -725,7 +719,7 @@ int launch(const AttnArgs &a, int64_t groups, hipStream_t st)
         }
     }
     kernel<<<(unsigned)groups, kThreads, lds, st>>>(a);
-    if (a.apart) join_parts_kernel<DT><<<dim3((unsigned)groups, std::min(a.G, kTile)), kThreads, 0, st>>>(a);
+    if (a.apart) join_parts_kernel<DT><<<dim3((unsigned)(a.B * a.Hkv * a.tiles), std::min(a.G, kTile)), kThreads, 0, st>>>(a);
     return check_launch("paged_attention");
 }
 
