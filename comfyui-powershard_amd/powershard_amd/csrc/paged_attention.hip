@@ -666,13 +666,14 @@ join_parts_kernel(AttnArgs a)
 }
 
 // ------------------------------------------------------------------ the launch
-// As many workgroups as the chip holds, no more than the rounds can fill.  Where units are few (long
-// texts of few users: over 8 parts a unit), parts are joined by a kernel of their own, which spreads a
-// unit's heads over the chip, and two workgroups per CU fill the memory system with fewer parts than
-// three; where units are many, the workgroups of the first kernel join (two or three parts a unit) and
-// a third one per CU covers the gaps between segments.  us, joined apart | inside:
-// 1 x 131071 tokens, 8 kv heads, fp8 62 | 65; 8 x 6000, 1 kv head of 256 dims 22 | 34; 61 x 4096, 8 kv
-// heads, int8 72 | 68; 16 x 8192 (window 1024), 16 kv heads of 64 dims 22.4 | 21.2.
+// As many workgroups as the chip holds, no more than the rounds can fill.  A unit's parts are joined by its
+// last workgroup where one round of loads per thread holds them (few parts, or few dims to a part), else by
+// a kernel of their own, which spreads the unit's heads over the chip; two workgroups per CU then fill the
+// memory system with fewer parts than three.  us a call, joined inside | apart (the second launch is
+// 3.5 us of the host's time, which bounds the small calls): 1 x 2000 tokens, 40 heads on 8, int8 14.0 | 18.7;
+// 1 x 4000, 16 on 16 13.8 | 18.2; 61 x 4096, 40 on 8 63.5 | 65.9; 128 x 8192, 64 on 8, bf16 377 | 386;
+// 4 x 16000, 40 on 8 30.1 | 26.0; 1 x 131071, 40 on 8, fp8 66.6 | 57.9 (3 per CU 58.9); 1 x 30000, 8 on 1
+// 35 | 18; 8 x 6000, 16 on 1, 256 dims 33 | 19.
 struct Plan {
     int tiles, part_floats;
     bool apart;
@@ -691,9 +692,10 @@ Plan plan(int codes, int64_t B, int Hq, int Hkv, int D, int64_t max_len)
     if (hipGetDevice(&dev) != hipSuccess) dev = 0;
     const int cus = cu_count(dev);
     const int most = groups_per_cu(D, codes != PSQ_CODES_NONE);
-    p.groups = std::min<int64_t>(cus * std::min(most, 2), rounds);
-    p.apart = p.groups > 8 * units;
-    if (!p.apart) p.groups = std::min<int64_t>(cus * most, rounds);
+    p.groups = std::min<int64_t>(cus * most, rounds);
+    const int items = heads * D / 4, loads = (D <= 64 ? 8 : 16) * std::max(kThreads / items, 1);   // of join_parts
+    p.apart = p.groups > units * loads || (items > kThreads && p.groups > 4 * units);
+    if (p.apart) p.groups = std::min<int64_t>(cus * std::min(most, 2), rounds);
     p.part_floats = (heads * (D + 2) + 31) / 32 * 32;   // whole lines
     p.cuts_at = kCounterBytes;
     p.parts_at = p.cuts_at + (p.apart ? units * (int64_t)sizeof(Cut) + 255 : 0) / 256 * 256;
