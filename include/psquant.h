@@ -352,9 +352,10 @@ PSQ_API int psq_kv_read(int codes, const int64_t *slots, int64_t T, const void *
  *   t / page_size; columns past a sequence's length (and before its window) are not followed
  *   lengths [B] int32, the tokens of each sequence, the new one included.  0 or less: zeros, lse -inf.
  * A sequence longer than its table, or with a page outside the pool among those it needs, gets NaN.
- * max_len: about the longest length, for the plan (any value gives right results).
+ * max_len: about the longest length, for the number of workgroups (any value gives right results).
  * workspace: NULL (no split over the length), or at least psq_paged_attention_workspace_bytes() bytes
- * with the arrival counters of the _ws GEMMs' workspace (zeroed once; every call leaves them zero). */
+ * with the arrival counters of the _ws GEMMs' workspace (zeroed once; every call leaves them zero; for
+ * this use and theirs alone, by calls that do not overlap). */
 PSQ_API int64_t psq_paged_attention_workspace_bytes(int codes, int64_t B, int Hq, int Hkv, int D, int64_t max_len);
 PSQ_API int psq_paged_attention(int codes, const void *q, int dtype, int64_t q_batch, int64_t q_head, const void *k_cache,
                         const void *v_cache, const float *k_scale, const float *v_scale, int64_t num_pages,

@@ -117,6 +117,20 @@ def test_strided_offset_and_empty_rows(gpu):
     assert q.shape == (0, 512) and scale.shape == (0,) and h.shape == (0, 512)
 
 
+@pytest.mark.parametrize("over", ["x", "residual"])
+def test_sum_in_place(gpu, over):
+    """The sum may be written over x or over the residual."""
+    from powershard_amd import _native, ops
+    x, r, w = _inputs(7, 1024, torch.bfloat16, 23, gpu)
+    q, scale, h = ops.add_rms_norm(x, w, residual=r, codes="int8", rot_group=256)
+    to = x if over == "x" else r
+    q2, s2 = torch.empty_like(q), torch.empty_like(scale)
+    _native.check(_native.lib().psq_add_rms_norm(
+        _native.CODES_I8, x.data_ptr(), _native.BF16, 1024, r.data_ptr(), 1024, w.data_ptr(), _native.F32, 1e-6, to.data_ptr(), 1024,
+        256, None, q2.data_ptr(), 1024, s2.data_ptr(), 7, 1024, torch.cuda.current_stream(gpu).cuda_stream), "add_rms_norm")
+    assert torch.equal(to, h) and torch.equal(q, q2) and torch.equal(scale, s2)
+
+
 def test_feeds_the_gemm(gpu):
     """norm -> int8 GEMM equals the GEMM of the dequantized rows."""
     from powershard_amd import ops
