@@ -130,6 +130,47 @@ def test_long_and_wide(gpu, B, lens):
     check(ops.paged_attention(*args), args)
 
 
+@pytest.mark.parametrize("codes,dtype", [("none", torch.bfloat16), ("int8", torch.float16), ("fp8", torch.bfloat16)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_long_units_that_stay_whole(gpu, codes, dtype, D):
+    """Runs of more steps than a wave looks up pages for at once (4096 tokens a workgroup)."""
+    from powershard_amd import ops
+    args = make([13000, 4096, 4097, 8193], 6, 2, D, 16, codes, dtype, gpu, seed=D)
+    check(ops.paged_attention(*args, max_len=1), args)
+    bad = args[3].clone()
+    bad[0, 700] = -1                       # past the first look-up of its workgroup
+    got = ops.paged_attention(*args[:3], bad, *args[4:], max_len=1)
+    assert got[0].isnan().all() and torch.isfinite(got[1:]).all()
+    assert ops.paged_attention(*args[:3], bad, *args[4:])[0].isnan().all()
+
+
+@pytest.mark.parametrize("B", [256, 257, 300, 1025])
+def test_batches_wider_than_a_workgroup(gpu, B):
+    """The runs are found from the lengths of the whole batch, several to a thread."""
+    from powershard_amd import ops
+    g = seeded(B)
+    lens = [int(n) for n in torch.randint(0, 700, (B,), generator=g)]
+    args = make(lens, 4, 2, 64, 16, "int8", torch.bfloat16, gpu, seed=3)
+    got = ops.paged_attention(*args)
+    check(got, args)
+    assert torch.equal(ops.paged_attention(*args, max_len=1)[0] == 0, got[0] == 0)
+
+
+def test_more_rounds_than_32_bits_times_runs(gpu):
+    """8192 sequences on the same 20000 tokens: 10 million rounds, whose cuts need 64-bit products."""
+    from powershard_amd import ops
+    B, n = 8192, 20000
+    q1, k, v, table, lengths, ks, vs = make([n], 8, 8, 64, 64, "int8", torch.bfloat16, gpu, seed=5)
+    q = torch.randn(B, 8, 64, generator=torch.Generator(device=gpu).manual_seed(1), device=gpu).to(torch.bfloat16)
+    pick = torch.tensor([0, 1, 4000, 8190, 8191], device=gpu)
+    got = ops.paged_attention(q, k, v, table.expand(B, -1), lengths.expand(B), ks, vs)
+    few = (q[pick], k, v, table.expand(5, -1), lengths.expand(5), ks, vs)
+    out, bound, _ = formula(*few)
+    assert ((got[pick].double() - out).abs() <= U16[torch.bfloat16] * out.abs() + 2.0 ** -25 + bound).all()
+    half = ops.paged_attention(q[2048:4096], k, v, table.expand(2048, -1), lengths.expand(2048), ks, vs)
+    assert ((got[2048:4096].double() - half.double()).abs() <= 2 * U16[torch.bfloat16] * half.double().abs() + 1e-3).all()
+
+
 @pytest.mark.parametrize("codes,dtype", [("none", torch.float16), ("int8", torch.bfloat16)])
 @pytest.mark.parametrize("heads,lens", [(17, [5000, 3]), (24, [31, 32, 33, 777]), (64, [3000, 1, 64]), (100, [2049])])
 def test_many_heads_share(gpu, codes, dtype, heads, lens):
