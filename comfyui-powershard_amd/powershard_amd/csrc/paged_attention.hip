@@ -340,23 +340,29 @@ paged_attention_kernel(AttnArgs a)
     };
     int len, lo, rounds;
     bool past;
-    const int each = a.alone ? 0 : (a.B + kThreads - 1) / kThreads;   // sequences of a thread
+    // Each wave scans the lengths for itself where it holds them (64 sequences), else the workgroup does.
+    const bool narrow = a.B <= 64;
+    const int each = a.alone ? 0 : narrow ? 1 : (a.B + kThreads - 1) / kThreads;   // sequences of a thread
+    const int mine_at = narrow ? lane : tid * each;
     uint32_t own = 0;
     for (int i = 0; i < each; i++)
-        if (tid * each + i < a.B) own += span(tid * each + i, len, lo, past);
+        if (mine_at + i < a.B) own += span(mine_at + i, len, lo, past);
     uint32_t before = own;                                  // rounds up to and with this thread's
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         const uint32_t y = __shfl_up(before, o, 64);
         before += lane >= o ? y : 0;
     }
-    if (lane == 63) wave_rounds[wave] = before;
-    __syncthreads();
-    uint32_t total = 0;
+    uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)before, 63);
+    if (!narrow) {
+        if (lane == 63) wave_rounds[wave] = before;
+        __syncthreads();
+        total = 0;
 #pragma unroll
-    for (int i = 0; i < kWaves; i++) {
-        before += i < wave ? wave_rounds[i] : 0;
-        total += wave_rounds[i];
+        for (int i = 0; i < kWaves; i++) {
+            before += i < wave ? wave_rounds[i] : 0;
+            total += wave_rounds[i];
+        }
     }
     before -= own;
     const uint64_t all = uniform((uint64_t)total * units);
@@ -372,20 +378,28 @@ paged_attention_kernel(AttnArgs a)
         if (w >= runs) return;
         x = first_of(w), end = first_of(w + 1);
         const uint32_t y = (uint32_t)divide(x, units);      // the thread whose sequences hold the run's start
-        if (y >= before && y < before + own) {
-            int i = tid * each;
-            for (;; i++) {
-                const int n = span(i, len, lo, past);
-                if (y < before + n) break;
-                before += n;
+        const bool here = y >= before && y < before + own;
+        uint32_t at;
+        if (narrow) {
+            b = __builtin_ctzll(__ballot(here));
+            at = (uint32_t)__builtin_amdgcn_readlane((int)before, b);
+        } else {
+            if (here) {
+                int i = mine_at;
+                for (;; i++) {
+                    const int n = span(i, len, lo, past);
+                    if (y < before + n) break;
+                    before += n;
+                }
+                start_b = i;
+                start_r = before;
             }
-            start_b = i;
-            start_r = before;
+            __syncthreads();
+            b = __builtin_amdgcn_readfirstlane(start_b);
+            at = (uint32_t)__builtin_amdgcn_readfirstlane(start_r);
         }
-        __syncthreads();
-        b = __builtin_amdgcn_readfirstlane(start_b);
         rounds = span(b, len, lo, past);
-        const uint64_t in = x - (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(start_r) * units;
+        const uint64_t in = x - (uint64_t)at * units;
         unit = (int)divide(in, rounds), r = (int)(in - (uint64_t)unit * rounds);
     }
     Cut cut[2] = {};       // what the run has part of: a unit that it goes on with, and one that it leaves
