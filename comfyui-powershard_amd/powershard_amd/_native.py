@@ -9,10 +9,13 @@ The reference loads its own native helper the same way -- a runtime-built ``.so`
 ``extern "C"`` entry points (powershard/ats_memory.py:80-91, ats_allocator.cpp:14-52).
 """
 import ctypes
+import importlib.util
 import os
 import threading
+import warnings
 from pathlib import Path
 
+DIRECT_PATH = Path(__file__).resolve().parent / "lib" / "psq_direct.so"
 LIB_PATH = Path(os.environ.get("PSQUANT_LIB", Path(__file__).resolve().parent / "lib" / "libpsquant.so"))
 ABI_VERSION = 1
 
@@ -60,6 +63,8 @@ SIGNATURES = {
     "psq_flag_nonfinite": (_I, [_P, _I, _I64, _P, ctypes.c_uint64, _P]),
 }
 
+DIRECT_CALLS = ("psq_add_rms_norm", "psq_kv_write", "psq_kv_read", "psq_paged_attention_workspace_bytes", "psq_paged_attention")
+
 
 class NativeLibraryError(ImportError):
     """libpsquant.so is missing or unusable: the native path cannot run."""
@@ -91,6 +96,36 @@ def lib():
                 raise NativeLibraryError(f"{LIB_PATH}: ABI {handle.psq_abi_version()} != {ABI_VERSION}")
             _lib = handle
     return _lib
+
+
+_direct = None
+
+
+def direct():
+    """The module of the decoder operators' direct calls (csrc/direct.cpp), bound to the loaded library, or
+    False where it cannot be used: it belongs to one release of torch, and the calls that it shortens
+    work without it.  A missing or foreign module is named in one warning."""
+    global _direct
+    if _direct is None:
+        handle = lib()
+        with _lock:
+            if _direct is None:
+                _direct = _load_direct(handle)
+    return _direct
+
+
+def _load_direct(handle):
+    import torch
+    try:
+        spec = importlib.util.spec_from_file_location("psq_direct", DIRECT_PATH)
+        module = importlib.util.module_from_spec(spec)
+        if module.TORCH_VERSION != torch.__version__.split("+")[0]:
+            raise ImportError(f"built for torch {module.TORCH_VERSION}, this is {torch.__version__}")
+        module.bind({name: ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in DIRECT_CALLS})
+    except ImportError as error:
+        warnings.warn(f"psquant: {DIRECT_PATH} is not used ({error}): the decoder operators' calls take longer", stacklevel=4)
+        return False
+    return module
 
 
 def available():

@@ -11,6 +11,9 @@ Each ``csrc/*.hip`` compiles to an object under ``_build/``; the objects link in
 * ``-fhip-fp32-correctly-rounded-divide-sqrt``: IEEE division for the per-row 127/absmax.
 * ``-fno-gpu-flush-denormals-to-zero``: fp32 denormals are kept, as on the CPU.
 * ``-Xclang -target-feature -Xclang -packed-fp32-ops``: no packed fp32 VALU instructions.
+
+``csrc/direct.cpp`` (host code only) is built beside it with the host compiler against the installed
+torch's headers: ``lib/psq_direct.so``.
 """
 import argparse
 import concurrent.futures
@@ -23,6 +26,7 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "lib" / "libpsquant.so"
+DIRECT = PKG / "lib" / "psq_direct.so"
 INCLUDE = PKG.parent.parent / "include"
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -52,6 +56,26 @@ def _compile(src):
     return obj
 
 
+def _build_direct():
+    """lib/psq_direct.so, the CPython module of the decoder operators' direct calls."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    tmp = DIRECT.with_suffix(".so.tmp")
+    headers = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"]]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f"-I{INCLUDE}",
+           *(flag for path in headers for flag in ("-isystem", path)), str(CSRC / "direct.cpp"), "-o", str(tmp),
+           f"-L{cpp_extension.TORCH_LIB_PATH}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed for direct.cpp:\n{r.stdout}\n{r.stderr}")
+    if r.stderr:
+        print(r.stderr, file=sys.stderr)
+    os.replace(tmp, DIRECT)
+
+
 def _check_stubs(lib):
     """Fail on an undefined symbol of the library's own namespace.  When the host pass of a .hip
     file rejects a kernel body (a target builtin it cannot check there), clang drops the kernel's
@@ -65,13 +89,16 @@ def _check_stubs(lib):
 
 
 def build(jobs=None, verbose=False):
-    """Compile every csrc/*.hip for gfx950 and link lib/libpsquant.so. Returns the library path."""
+    """Compile every csrc/*.hip for gfx950 and link lib/libpsquant.so, and lib/psq_direct.so beside it.
+    Returns the library's path."""
     BUILD.mkdir(exist_ok=True)
     LIB.parent.mkdir(exist_ok=True)
     srcs = sources()
     jobs = jobs or min(len(srcs), os.cpu_count() or 1, 8)
     with concurrent.futures.ThreadPoolExecutor(jobs) as ex:
+        direct = ex.submit(_build_direct)
         objs = list(ex.map(_compile, srcs))
+        direct.result()
     tmp = LIB.with_suffix(".so.tmp")
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), *map(str, objs)]
     r = subprocess.run(cmd, capture_output=True, text=True)
