@@ -9,6 +9,7 @@ Modules (the first three mirror the reference modules of the same name):
   norm           RMSNorm whose rows go to the quantized linears as codes
   kv_cache       PagedKVCache: a paged key-value cache in 16 bits, int8 or e4m3
   decoder        DecoderLayer: a text decoder layer on the linears, the norm and the cache
-  ops            torch-facing wrappers of the HIP kernels in libpsquant.so
+  ops            torch-facing wrappers of the HIP kernels in libpsquant.so (the decoder operators' shortest
+                 host calls are in psq_direct.so, csrc/direct.cpp)
 """
 __version__ = "0.1.0"
