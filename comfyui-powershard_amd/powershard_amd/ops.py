@@ -506,8 +506,8 @@ def dequant_fp8(q, w_scale, out_dtype=torch.bfloat16, e5m2=None):
 # What a decoder layer does between its quantized linears.  At one token the host call is most of the time.
 # Arguments that need nothing done to them go through _native.direct(), None from there means that they are not
 # such and the checks below see to them; those are written out flat, and addresses go to the library as
-# integers.  Host us a call, general path and direct: add_rms_norm 10.8 and 6.0, kv_write 7.2 and 3.2, kv_read
-# 9.1 and 5.5, paged_attention 12.6 and 7.5 (the launch is 3 of each, an allocation in Python 1.3).
+# integers.  Host us a call, general path and direct: add_rms_norm 11.0 and 6.0, kv_write 7.6 and 3.5, kv_read
+# 9.7 and 5.5, paged_attention 10.4 and 5.0 (the launch is 3 of each, an allocation in Python 1.3).
 CODES = {None: _native.CODES_NONE, "none": _native.CODES_NONE, "int8": _native.CODES_I8, "fp8": _native.CODES_E4M3}
 _CODE_DTYPES = {torch.int8: _native.CODES_I8, torch.float8_e4m3fn: _native.CODES_E4M3,
                 torch.bfloat16: _native.CODES_NONE, torch.float16: _native.CODES_NONE}
