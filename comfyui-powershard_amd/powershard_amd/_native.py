@@ -58,12 +58,14 @@ SIGNATURES = {
     "psq_kv_write": (_I, [_I, _P, _P, _I, _I64, _I64, _I64, _I64, _P, _I64, _I, _I, _P, _P, _P, _P, _I64, _I, _P]),
     "psq_kv_read": (_I, [_I, _P, _I64, _P, _P, _I, _P, _P, _I64, _I, _I, _I, _P, _P, _I, _P]),
     "psq_paged_attention_workspace_bytes": (_I64, [_I, _I64, _I, _I, _I, _I64]),
+    "psq_paged_attention_own_workspace": (_I, [_I, _I64, _I, _I, _I, _I64]),
     "psq_paged_attention": (_I, [_I, _P, _I, _I64, _I64, _P, _P, _P, _P, _I64, _I, _P, _I64, _I64, _P, _I64, _I, _I, _I, _F,
                                  _I64, _I64, _P, _P, _P, _I64, _P]),
     "psq_flag_nonfinite": (_I, [_P, _I, _I64, _P, ctypes.c_uint64, _P]),
 }
 
-DIRECT_CALLS = ("psq_add_rms_norm", "psq_kv_write", "psq_kv_read", "psq_paged_attention_workspace_bytes", "psq_paged_attention")
+DIRECT_CALLS = ("psq_add_rms_norm", "psq_kv_write", "psq_kv_read", "psq_paged_attention_workspace_bytes",
+                "psq_paged_attention_own_workspace", "psq_paged_attention")
 
 
 class NativeLibraryError(ImportError):

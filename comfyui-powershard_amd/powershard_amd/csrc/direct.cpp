@@ -25,6 +25,7 @@ decltype(&psq_add_rms_norm) f_norm;
 decltype(&psq_kv_write) f_write;
 decltype(&psq_kv_read) f_read;
 decltype(&psq_paged_attention_workspace_bytes) f_attend_bytes;
+decltype(&psq_paged_attention_own_workspace) f_attend_own;
 decltype(&psq_paged_attention) f_attend;
 
 // Other threads run while memory is allocated and the kernel is launched (a full queue makes the launch wait).
@@ -224,12 +225,13 @@ PyObject *kv_read(PyObject *, PyObject *const *o, Py_ssize_t n)
 
 // paged_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, scale (None: dim ** -0.5), window,
 //                 max_len (None: the table's), return_lse, the stream's workspace, stream) -> out or (out, lse)
+// Parts that a second launch joins are in memory of the call's own.
 PyObject *attend(PyObject *, PyObject *const *o, Py_ssize_t n)
 {
     return guarded([&]() -> PyObject * {
         Arg q, table, lengths, ws;
         Pools p;
-        if (n != 13 || !f_attend || !f_attend_bytes || !take(o[0], -1, q) || !q.t) return none();
+        if (n != 13 || !f_attend || !f_attend_bytes || !f_attend_own || !take(o[0], -1, q) || !q.t) return none();
         const int64_t index = q.t->get_device();
         if (!p.take_from(o + 1, index) || !take(o[5], index, table) || !table.t || !take(o[6], index, lengths) || !lengths.t || !take(o[11], index, ws))
             return none();
@@ -249,21 +251,24 @@ PyObject *attend(PyObject *, PyObject *const *o, Py_ssize_t n)
             lengths.t->dim() != 1 || lengths.t->size(0) != q.t->size(0) || !lengths.t->is_contiguous() || window < 0)
             return none();
         const int64_t B = q.t->size(0), H = q.t->size(1), cols = table.t->size(1);
-        if (max_len < 0) max_len = cols * p.page;
+        if (max_len < 0 || max_len > cols * p.page) max_len = cols * p.page;
         if (window && window < max_len) max_len = window;
         const int64_t need = f_attend_bytes(p.codes, B, (int)H, p.heads, p.dim, max_len);
-        if (need > 0 && (!ws.t || ws.t->numel() < need)) return none();
+        const bool own = need > 0 && f_attend_own(p.codes, B, (int)H, p.heads, p.dim, max_len);
+        if (need > 0 && !own && (!ws.t || ws.t->numel() < need)) return none();
         const auto opt = at::TensorOptions().device(q.t->device());
-        at::Tensor out, lse;
+        at::Tensor out, lse, parts;
         int status;
         {
             Unlocked unlocked;
+            if (own) parts = at::empty({need}, opt.dtype(at::kByte));
+            const at::Tensor *work = own ? &parts : ws.t;
             out = at::empty({B, H, p.dim}, opt.dtype(q.t->scalar_type()));
             if (want) lse = at::empty({B, H}, opt.dtype(at::kFloat));
             status = f_attend(p.codes, q.t->data_ptr(), dt, q.t->stride(0), q.t->stride(1), p.k.t->data_ptr(), p.v.t->data_ptr(), p.scale(p.ks),
                               p.scale(p.vs), p.pages, (int)p.page, (const int32_t *)table.t->data_ptr(), table.t->stride(0), cols,
                               (const int32_t *)lengths.t->data_ptr(), B, (int)H, p.heads, p.dim, (float)scale, window, max_len, out.data_ptr(),
-                              want ? (float *)lse.data_ptr() : nullptr, need > 0 ? ws.t->data_ptr() : nullptr, need > 0 ? ws.t->numel() : 0,
+                              want ? (float *)lse.data_ptr() : nullptr, need > 0 ? work->data_ptr() : nullptr, need > 0 ? work->numel() : 0,
                               stream);
         }
         return status ? none() : want ? tuple(out, lse) : THPVariable_Wrap(out);
@@ -281,6 +286,7 @@ PyObject *bind(PyObject *, PyObject *d)
     f_write = (decltype(f_write))at("psq_kv_write");
     f_read = (decltype(f_read))at("psq_kv_read");
     f_attend_bytes = (decltype(f_attend_bytes))at("psq_paged_attention_workspace_bytes");
+    f_attend_own = (decltype(f_attend_own))at("psq_paged_attention_own_workspace");
     f_attend = (decltype(f_attend))at("psq_paged_attention");
     if (PyErr_Occurred()) return nullptr;
     Py_RETURN_NONE;

@@ -28,7 +28,9 @@
 // chip holds at once: ragged lengths cost no balance, the host needs no lengths, and a unit is cut only
 // where a run ends.  A workgroup writes its parts of cut units (two at most) to the workspace and counts
 // itself when its run is done; the last one of a unit, or a second kernel (see plan()), adds the parts up
-// in their order, so results do not depend on timing.
+// in their order, so results do not depend on timing.  With the second kernel the workspace carries parts
+// from one launch to the next: another call's kernels between them (a second host thread on the stream) would
+// write over them, so such a call's workspace is its own (psq_paged_attention_own_workspace).
 #include "kv_cache.hpp"
 
 #include <algorithm>
@@ -759,6 +761,12 @@ int64_t psq_paged_attention_workspace_bytes(int codes, int64_t B, int Hq, int Hk
 {
     if (B <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || max_len <= 0 || Hq % Hkv || B > 65535) return 0;
     return psq::plan(codes, B, Hq, Hkv, D, std::min<int64_t>(max_len, 0x7fffffffLL)).bytes;
+}
+
+int psq_paged_attention_own_workspace(int codes, int64_t B, int Hq, int Hkv, int D, int64_t max_len)
+{
+    if (psq_paged_attention_workspace_bytes(codes, B, Hq, Hkv, D, max_len) <= 0) return 0;
+    return psq::plan(codes, B, Hq, Hkv, D, std::min<int64_t>(max_len, 0x7fffffffLL)).apart;
 }
 
 int psq_paged_attention(int codes, const void *q, int dtype, int64_t q_batch, int64_t q_head, const void *k_cache,

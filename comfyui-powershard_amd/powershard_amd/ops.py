@@ -254,7 +254,9 @@ def gemm_fp8(a, a_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16, activa
 
 
 # Workspaces of the weight-only GEMMs (split K) and of paged_attention (split length), one per (device,
-# stream): calls on one stream run in order, so they can share it (calls on two streams would race on its counters).  A call that needs
+# stream): launches on one stream run in order, so calls of one launch can share it, whichever host thread makes
+# them (calls on two streams would race on its counters).  A call of two launches, between which another thread's
+# could come, has memory of its own (paged_attention whose parts a second kernel joins).  A call that needs
 # more gets a larger one (at least twice the size, so a stream is replaced a few times at most), and
 # the replaced buffer is kept until the process ends: a launch captured into a graph keeps the
 # address it was given, which must not be handed out again.  At most _MAX_WS_STREAMS streams per
@@ -719,13 +721,17 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, k_scale=None, v_s
     if not lengths.is_contiguous():
         lengths = lengths.contiguous()
     q, q_batch, q_head = _heads(q)
-    max_len = cols * page if max_len is None or max_len < 0 else int(max_len)
+    max_len = cols * page if max_len is None or max_len < 0 else min(int(max_len), cols * page)
     if window and window < max_len:
         max_len = int(window)
     lib, raw, device = _native.lib(), _raw(index), q.device
     out = torch.empty((B, H, D), dtype=dtype, device=device)
     lse = torch.empty((B, H), dtype=torch.float32, device=device) if return_lse else None
-    ws, nb = _workspace(device, raw or None, lib.psq_paged_attention_workspace_bytes(code, B, H, Hk, D, max_len))
+    nb = lib.psq_paged_attention_workspace_bytes(code, B, H, Hk, D, max_len)
+    if nb > 0 and lib.psq_paged_attention_own_workspace(code, B, H, Hk, D, max_len):
+        ws = torch.empty(nb, dtype=torch.uint8, device=device)   # two launches: the call's own
+    else:
+        ws, nb = _workspace(device, raw or None, nb)
     _call("paged_attention", lib.psq_paged_attention, code, q.data_ptr(), dt, q_batch, q_head, k_cache.data_ptr(),
           v_cache.data_ptr(), ks, vs, pages, page, block_table.data_ptr(), block_table.stride(0), cols, lengths.data_ptr(), B, H,
           Hk, D, D ** -0.5 if scale is None else scale, window, max_len, out.data_ptr(), lse.data_ptr() if return_lse else None,

@@ -355,8 +355,13 @@ PSQ_API int psq_kv_read(int codes, const int64_t *slots, int64_t T, const void *
  * max_len: about the longest length, for the number of workgroups (any value gives right results).
  * workspace: NULL (no split over the length), or at least psq_paged_attention_workspace_bytes() bytes
  * with the arrival counters of the _ws GEMMs' workspace (zeroed once; every call leaves them zero; for
- * this use and theirs alone, by calls that do not overlap). */
+ * this use and theirs alone, by calls that do not overlap).
+ * Where psq_paged_attention_own_workspace() is 1 the call makes two launches and the workspace carries the
+ * parts from the first to the second: nothing else that writes to it may be enqueued in between, from
+ * another host thread on the same stream either.  It needs no zeroed counters then, so memory of the call's own
+ * (any contents) serves.  Both queries take the max_len of the call, at most table_cols * page_size. */
 PSQ_API int64_t psq_paged_attention_workspace_bytes(int codes, int64_t B, int Hq, int Hkv, int D, int64_t max_len);
+PSQ_API int psq_paged_attention_own_workspace(int codes, int64_t B, int Hq, int Hkv, int D, int64_t max_len);
 PSQ_API int psq_paged_attention(int codes, const void *q, int dtype, int64_t q_batch, int64_t q_head, const void *k_cache,
                         const void *v_cache, const float *k_scale, const float *v_scale, int64_t num_pages,
                         int page_size, const int32_t *block_table, int64_t table_stride, int64_t table_cols,
