@@ -82,7 +82,7 @@ kv_write_kernel(KvArgs a)
             mk = __builtin_elementwise_maximum(mk, __shfl_xor(mk, o, 64));
             mv = __builtin_elementwise_maximum(mv, __shfl_xor(mv, o, 64));
         }
-        const bool zk = mk < kKvTiny, zv = mv < kKvTiny;
+        const bool zk = mk < zero_below(LIM), zv = mv < zero_below(LIM);
         const v4i qk = codes16<CODES>(fk, zk ? 0.0f : LIM / mk), qv = codes16<CODES>(fv, zv ? 0.0f : LIM / mv);
         if (here) {
             *(v4i *)(a.kc + at * a.D + e) = qk;

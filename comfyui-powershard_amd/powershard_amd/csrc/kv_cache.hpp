@@ -1,12 +1,9 @@
-// kv_cache.hpp -- what the paged cache's kernels share: its shape, and the codes of a row.
+// kv_cache.hpp -- what the paged cache's kernels share: its shape.
 #pragma once
 
 #include "quantize.hpp"
 
 namespace psq {
-
-// below this max|row| a row counts as zero: LIM / max stays finite
-constexpr float kKvTiny = 0x1p-120f;
 
 // host checks of the pools: sizes, alignment, scales present exactly with codes
 inline int check_kv_cache(const char *name, int codes, const void *k_cache, const void *v_cache, const float *k_scale,

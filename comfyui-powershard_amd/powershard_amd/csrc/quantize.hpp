@@ -97,6 +97,10 @@ __device__ __forceinline__ uint32_t e4m3_codes4(float u0, float u1, float u2, fl
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(clamp(u2), clamp(u3), lo, true);
 }
 
+// Below this maximum a row of the decoder operators counts as zero: LIM / max stays finite
+// (127 2^120 < 2^127, 448 2^119 = 1.75 2^127; 448 2^120 is past fp32).
+constexpr float zero_below(float lim) { return lim == 127.0f ? 0x1p-120f : 0x1p-119f; }
+
 // rot_group 0 (rotk 0) or a power of 4 in [4, 1024] dividing K (rotk = its base-4 log)
 inline int rot_log4(int rot_group, int64_t K, int &rotk)
 {

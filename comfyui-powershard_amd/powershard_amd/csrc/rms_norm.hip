@@ -16,8 +16,6 @@ namespace {
 constexpr int kChunk = 16;
 constexpr int kMaxThreads = 1024;
 constexpr int kMaxK = kChunk * kMaxThreads * 2;
-// below this max|h w| a row counts as zero: LIM / max stays finite
-constexpr float kTiny = 0x1p-120f;
 
 // 16 elements as fp32.  ONCE: read once, non-temporally (quantize_rows.hip says what that leaves in the caches).
 template <int DT, bool ONCE = false>
@@ -119,7 +117,7 @@ add_rms_norm_kernel(NormArgs a)
     }
     const float amax = __uint_as_float(top);
     const float r = 1.0f / __builtin_sqrtf(__builtin_fmaf(total, a.inv_k, a.eps));
-    const bool zero = amax < kTiny;
+    const bool zero = amax < zero_below(LIM);
     const float mul = CODES == PSQ_CODES_NONE ? r * post
                       : a.static_scale        ? (r * post) / *a.static_scale
                       : zero                  ? 0.0f

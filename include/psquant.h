@@ -305,8 +305,8 @@ enum psq_codes { PSQ_CODES_NONE = 0, PSQ_CODES_I8 = 1, PSQ_CODES_E4M3 = 2 };
  *   h = round_x(x + residual)               (residual NULL: h = x; else written to sum)
  *   u = T(h w) 2^-k                         (T as in psq_quantize_rows_i8; rot_group 0: u = h w)
  *   y = u / sqrt(mean(h^2) + eps)           fp32, the mean over the row's K elements
- *   PSQ_CODES_I8 / _E4M3: out = codes of y, scale[m] = max|y| / 127 or / 448 (rows with max|h w| below
- *     2^-120, zero rows among them: codes 0, scale 1); static_scale: *static_scale in its place
+ *   PSQ_CODES_I8 / _E4M3: out = codes of y, scale[m] = max|y| / 127 or / 448 (rows with max|u| 2^k below
+ *     2^-120 or 2^-119, zero rows among them: codes 0, scale 1); static_scale: *static_scale in its place
  *   PSQ_CODES_NONE: out = round_x(y); scale unused
  * The normalized row is never rounded to 16 bits on its way to the codes.  The factor
  * 1 / sqrt(...) > 0 scales y and max|y| alike, so the codes do not depend on it, only the scale does.
@@ -325,7 +325,7 @@ PSQ_API int psq_add_rms_norm(int codes, const void *x, int x_dtype, int64_t ldx,
  * 16 in 16..256, page_size a multiple of 16, the pools contiguous and 16-byte aligned. */
 
 /* Writes T tokens' keys and values, quantized on the way: scale = max|row| / 127 or / 448 (rows below
- * 2^-120: codes 0, scale 1), codes = round(v LIM / max|row|).  A row holding a NaN or Inf gets a
+ * 2^-120 or 2^-119: codes 0, scale 1), codes = round(v LIM / max|row|).  A row holding a NaN or Inf gets a
  * non-finite scale.
  *   k, v [T, Hkv, D] bf16/f16, element strides of tokens and heads (multiples of 8, 16-byte aligned)
  *   slots [T] int64, distinct; a token whose slot is negative or past the pool is not written */

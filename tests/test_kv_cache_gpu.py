@@ -116,6 +116,31 @@ def test_rows_of_zeros_nan_and_inf(gpu, codes):
     assert not torch.isfinite(a[2]).any() and not torch.isfinite(a[3]).any()
 
 
+@pytest.mark.parametrize("codes", ["int8", "fp8"])
+def test_rows_at_the_edge_of_zero(gpu, codes):
+    """Rows whose 127 / max or 448 / max is at the end of fp32: zero rows below the limit, the nearest codes from
+    there on, and never a code from a product of zero and infinity."""
+    from powershard_amd import ops
+    k, v, ks, vs = make_pools(1, 1, 16, 64, codes, torch.bfloat16, gpu, fill=0x7F)
+    tops = [2.0 ** -121, 2.0 ** -120, 1.5 * 2.0 ** -120, 1.75 * 2.0 ** -120, 2.0 ** -119, 1.5 * 2.0 ** -119, 2.0 ** -110]
+    x = torch.zeros(len(tops), 1, 64)
+    x[:, 0, 1::3] = torch.tensor(tops)[:, None]
+    x[:, 0, 2::3] = -0.25 * torch.tensor(tops)[:, None]
+    x = x.to(torch.bfloat16).to(gpu)
+    slots = torch.arange(len(tops), device=gpu)
+    ops.kv_write(x, x, slots, k, v, ks, vs)
+    kind, lim = CODES[codes]
+    limit = 2.0 ** -120 if codes == "int8" else 2.0 ** -119
+    got = by_slot(k)[slots].float().cpu()
+    for i, top in enumerate(tops):
+        want = (x[i].float().cpu().double() / top * lim).float() if top >= limit else torch.zeros(1, 64)
+        want = want.round() if codes == "int8" else want.to(kind).float()
+        assert torch.equal(got[i], want), top
+        assert float(by_slot(ks)[i, 0]) == (float(torch.tensor(top) / lim) if top >= limit else 1.0)
+    seen, _ = ops.kv_read(slots, k, v, ks, vs, out_dtype=torch.float32)
+    assert ((seen - x.float()).abs().cpu() <= torch.tensor([t / 100 if t >= limit else t for t in tops])[:, None, None]).all()
+
+
 def test_strides_and_empty(gpu):
     """Slices of a fused projection, misaligned rows, broadcast heads, no tokens."""
     from powershard_amd import ops

@@ -101,6 +101,28 @@ def test_rows_of_zeros_nan_and_inf(gpu, codes):
     assert torch.equal(q[3:4].view(torch.uint8), same.view(torch.uint8)) and scale[3] == s[0]
 
 
+@pytest.mark.parametrize("codes", ["int8", "fp8"])
+@pytest.mark.parametrize("rot", [0, 16])
+def test_rows_at_the_edge_of_zero(gpu, codes, rot):
+    """Rows whose 127 / max or 448 / max is at the end of fp32: zero rows below the limit, the nearest codes from
+    there on.  (One element per group of 16: its transform has the element's size everywhere.)"""
+    from powershard_amd import ops
+    tops = [2.0 ** -121, 2.0 ** -120, 1.5 * 2.0 ** -120, 1.75 * 2.0 ** -120, 2.0 ** -119, 1.5 * 2.0 ** -119, 2.0 ** -110]
+    x = torch.zeros(len(tops), 64)
+    x[:, 16] = torch.tensor(tops)
+    x[:, 37] = -0.25 * torch.tensor(tops)
+    x = x.to(torch.bfloat16).to(gpu)
+    w = torch.ones(64, device=gpu)
+    q, scale, _ = ops.add_rms_norm(x, w, eps=1.0, codes=codes, rot_group=0 if codes == "fp8" else rot)
+    limit = 2.0 ** -120 if codes == "int8" else 2.0 ** -119
+    y = _formula(x, w, 1.0, rot if codes == "int8" else 0)
+    for i, top in enumerate(tops):
+        if top >= limit:
+            _check_codes(q[i:i + 1], scale[i:i + 1], y[i:i + 1], codes)
+        else:
+            assert (q[i].float() == 0).all() and scale[i] == 1, top
+
+
 def test_strided_offset_and_empty_rows(gpu):
     from powershard_amd import ops
     x, r, w = _inputs(5, 512, torch.bfloat16, 21, gpu)
