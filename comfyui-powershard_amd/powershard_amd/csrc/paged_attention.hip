@@ -21,7 +21,9 @@
 // int8 and e4m3 codes are exact in bf16 (and f16), so they enter the products as they are; key scales
 // multiply the fp32 scores, value scales the fp32 probabilities.  A probability enters its product as a
 // pair of 16-bit numbers, p = hi + lo, two instructions each: 16 bits of it or more take part, and the
-// matrix units stay far below what the loads leave them.
+// matrix units stay far below what the loads leave them.  bf16 pairs hold them over fp32's range.  f16 pairs end
+// at 2^-24, so with f16 values p, and the sums over it, are held 2^15 times as large (p <= 1): 16 bits of it down to
+// 2^-30, and no more than 2^-40 lost below.
 //
 // Work is dealt in rounds of 128 tokens (a step of each wave).  The rounds of all units (sequence, kv
 // head, head tile), in their order, are cut into equal runs, one per workgroup, as many workgroups as the
@@ -47,6 +49,7 @@ constexpr int kTile = 16;                       // heads of a workgroup; tokens 
 constexpr int kGrain = kStep * kWaves;          // tokens of a workgroup's round
 constexpr int64_t kCounterBytes = 64 * 1024;    // arrival counters of the GEMMs at the workspace's head
 constexpr int SC1 = 16;                         // cache-policy bit sc1 of the buffer intrinsics
+constexpr float kF16Unit = 0x1p15f;             // of probabilities with f16 values
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // A cut unit that a run has part of: its sequence, index in it, first run and number of parts.
@@ -74,6 +77,7 @@ struct AttnArgs {
     int alone;             // units stay whole, a workgroup each
     int apart;             // parts are joined by a kernel of their own
     float scale;           // times log2(e)
+    float per_unit;        // 1 / the unit that probabilities are held in
 };
 
 // Two fp32 values whose low 16 bits are zero as a packed bf16 pair.
@@ -190,12 +194,11 @@ __device__ __forceinline__ void join_add(float M, float &L, v4f &acc, float m, f
 // Four dims of a head's output from the sums at maximum M (in units of log2), and its lse.  none: no
 // token, zeros (tokens whose scores are all -inf: 0 / 0, as softmax).
 template <int DT>
-__device__ __forceinline__ void finish(uint16_t *out, float *lse, int64_t head, int D, int d4, const v4f &acc, float M, float L,
-                                       bool none)
+__device__ __forceinline__ void finish(const AttnArgs &a, int64_t head, int D, int d4, const v4f &acc, float M, float L, bool none)
 {
     const float r = none ? 0.0f : 1.0f / L;
-    *(v2i *)(out + head * D + 4 * d4) = v2i{(int)pack_half2<DT>(acc[0] * r, acc[1] * r), (int)pack_half2<DT>(acc[2] * r, acc[3] * r)};
-    if (lse && d4 == 0) lse[head] = none ? -INFINITY : M * kLn2 + logf(L);
+    *(v2i *)(a.out + head * D + 4 * d4) = v2i{(int)pack_half2<DT>(acc[0] * r, acc[1] * r), (int)pack_half2<DT>(acc[2] * r, acc[3] * r)};
+    if (a.lse && d4 == 0) a.lse[head] = none ? -INFINITY : M * kLn2 + logf(L * a.per_unit);
 }
 
 // Adds up the parts of heads h0 .. h0 + n - 1 of a cut unit: part 0 is its first run's second, the others the
@@ -239,7 +242,7 @@ __device__ __forceinline__ void join_parts(const AttnArgs &a, const Cut &cut, in
                 join_add(M, L, acc, __int_as_float(ml[u][0]), __int_as_float(ml[u][1]), __builtin_bit_cast(v4f, y[u]));
         }
         if (sharers == 1) {
-            finish<DT>(a.out, a.lse, row0 + h, a.D, q - h * quads, acc, M, L, false);
+            finish<DT>(a, row0 + h, a.D, q - h * quads, acc, M, L, false);
         } else {
             red[tid] = acc;
             red_ml[tid] = v2f{M, L};
@@ -253,7 +256,7 @@ __device__ __forceinline__ void join_parts(const AttnArgs &a, const Cut &cut, in
         v4f acc = {0, 0, 0, 0};
         for (int k = 0; k < sharers; k++) M = fmaxf(M, red_ml[k * items + tid][0]);
         for (int k = 0; k < sharers; k++) join_add(M, L, acc, red_ml[k * items + tid][0], red_ml[k * items + tid][1], red[k * items + tid]);
-        finish<DT>(a.out, a.lse, row0 + h, a.D, q - h * quads, acc, M, L, false);
+        finish<DT>(a, row0 + h, a.D, q - h * quads, acc, M, L, false);
     }
 }
 
@@ -529,6 +532,7 @@ paged_attention_kernel(AttnArgs a)
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             p[j] = __builtin_amdgcn_exp2f(sc[j >> 2][j & 3] - ref);
+            if constexpr (PVT == PSQ_F16) p[j] *= kF16Unit;
             run_l += p[j];
             if constexpr (ES == 1) p[j] *= st.vs[j >> 2][j & 3];
         }
@@ -638,7 +642,7 @@ paged_attention_kernel(AttnArgs a)
 #pragma unroll
         for (int v = 0; v < kWaves; v++) join_add(M, L, acc, wave_m[v][h], wave_l[v][h], *(const v4f *)(smem + (v * these + h) * LD + 4 * d4));
         if (whole) {
-            finish<DT>(a.out, a.lse, row0 + h, D, d4, acc, M, L, none);
+            finish<DT>(a, row0 + h, D, d4, acc, M, L, none);
         } else {
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4i, acc), part, i * 16, 0, SC1);
             if (d4 == 0)
@@ -801,7 +805,8 @@ int psq_paged_attention(int codes, const void *q, int dtype, int64_t q_batch, in
                      block_table, table_stride, lengths, (uint16_t *)out, lse,
                      (uint32_t *)workspace, (Cut *)((uint8_t *)workspace + p.cuts_at), (float *)((uint8_t *)workspace + p.parts_at),
                      p.part_floats, (int)num_pages, (int)cap, (int)B, page_size, Hq, Hkv, D, Hq / Hkv, p.tiles,
-                     (int)std::min<int64_t>(window, cap), alone, !alone && p.apart, scale * kLog2e};
+                     (int)std::min<int64_t>(window, cap), alone, !alone && p.apart, scale * kLog2e,
+                     codes == PSQ_CODES_NONE && dtype == PSQ_F16 ? 1.0f / kF16Unit : 1.0f};
     hipStream_t st = (hipStream_t)stream;
     auto go = [&](auto dtc) {
         constexpr int DT = decltype(dtc)::value;

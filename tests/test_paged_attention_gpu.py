@@ -198,6 +198,39 @@ def test_window_and_scale(gpu, codes, dtype, window):
     assert (err <= U16[dtype] * want[0].abs() + 2.0 ** -25 + want[1]).all()
 
 
+@pytest.mark.parametrize("codes,dtype", TYPES)
+@pytest.mark.parametrize("gap", [11.0, 14.0, 17.0, 17.5, 20.0])
+@pytest.mark.parametrize("max_len", [None, 1])
+def test_small_probabilities(gpu, codes, dtype, gap, max_len):
+    """A first token that takes nearly all weight and has the value 0, before a long tail whose scores are `gap`
+    lower: the tail's values are all that the output has."""
+    from powershard_amd import ops
+    D, page, lens = 64, 16, [5000, 40, 700]
+    args = make(lens, 4, 2, D, page, codes, dtype, gpu, seed=int(gap))
+    q, k, v, table, lengths, ks, vs = args
+    q.zero_()
+    q[..., 0] = 8.0
+    for t in (k, v):
+        if codes != "none":
+            t.view(torch.uint8)[:] = torch.where(t.float().isnan(), 0, t.view(torch.uint8))
+    k[..., 0] = 0
+    for b in range(3):
+        first = int(table[b, 0])
+        v[first, :, 0] = 0
+        k[first, :, 0, 0] = 1
+        if ks is not None:
+            ks[first, :, 0] = gap
+            vs[first, :, 0] = 1.0
+        else:
+            k[first, :, 0, 0] = gap
+    args = (q, k, v.abs() if codes != "int8" else v.clamp(min=0), table, lengths, ks, vs) if codes != "fp8" else \
+        (q, k, (v.view(torch.uint8) & 0x7F).view(v.dtype), table, lengths, ks, vs)
+    got, lse = ops.paged_attention(*args, max_len=max_len, return_lse=True)
+    check(got, args)
+    want = formula(*args)[2]
+    assert ((lse.double() - want).abs() <= 1e-4 + 1e-5 * want.abs()).all()
+
+
 def test_values_that_are_not_finite(gpu):
     """A NaN in a token's key or value reaches its kv head's outputs and no others; scores of -inf get no
     weight; a sequence of only such scores is NaN, as softmax is."""
