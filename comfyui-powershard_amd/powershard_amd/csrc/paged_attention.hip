@@ -471,6 +471,17 @@ paged_attention_kernel(AttnArgs a)
 
     for (;;) {
     v4f o[DV];
+    constexpr int LD = DD + 4;
+    auto place = [&]() {   // o to the wave's rows of the LDS
+        if (m < heads) {
+            float *row = smem + (wave * heads + m) * LD;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int dt = 0; dt < DV; dt += 4)
+                    *(v4f *)(row + (4 * g + i) * DV + dt) = v4f{o[dt][i], o[dt + 1][i], o[dt + 2][i], o[dt + 3][i]};
+        }
+    };
     float run_m, run_l;
     bool pair = true;      // probabilities as hi + lo
     // The step's keys and values are in flight or here.  The next step's loads go into the same registers
@@ -584,7 +595,8 @@ paged_attention_kernel(AttnArgs a)
             if (more) load_values(s + 1);
         }
         // An infinite value meets lo = 0 or lo < 0 in the second product: NaN where the sum is infinite.
-        // Once more, then, with p as the sum of two equal halves (the precision of one 16-bit number).
+        // Once more, then, with p as the sum of two equal halves (the precision of one 16-bit number), for the
+        // sums that were NaN; the others wait in the wave's part of the LDS, which is free until its sums go there.
         float any = 0.0f;
 #pragma unroll
         for (int dt = 0; dt < DV; dt++)
@@ -592,6 +604,7 @@ paged_attention_kernel(AttnArgs a)
             for (int i = 0; i < 4; i++) any = __builtin_fmaf(o[dt][i], 0.0f, any);
         if (!pair || wild || !__any(any != any)) break;
         pair = false;
+        place();
         begin();
     }
     if (wild || past) run_m = 0.0f, run_l = NAN;
@@ -602,15 +615,18 @@ paged_attention_kernel(AttnArgs a)
         wave_m[wave][m] = run_m;
         wave_l[wave][m] = run_l;
     }
-    constexpr int LD = DD + 4;
-    if (m < heads) {
-        float *row = smem + (wave * heads + m) * LD;
+    if (!pair) {
+        float *row = smem + (wave * heads + m) * LD + 4 * g * DV;
+        if (m < heads)
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+            for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int dt = 0; dt < DV; dt += 4)
-                *(v4f *)(row + (4 * g + i) * DV + dt) = v4f{o[dt][i], o[dt + 1][i], o[dt + 2][i], o[dt + 3][i]};
+                for (int dt = 0; dt < DV; dt++) {
+                    const float first = row[i * DV + dt];
+                    o[dt][i] = first == first ? first : o[dt][i];
+                }
     }
+    place();
     // the run's next segment: its first loads travel while this one's sums are put together
     const bool whole = n == rounds, none = len == 0 && !past;
     const int quads = D / 4, these = heads;

@@ -254,6 +254,33 @@ def test_values_that_are_not_finite(gpu):
     assert got[3, 2:].isnan().all() and torch.isfinite(got[3, :2]).all()
 
 
+@pytest.mark.parametrize("codes,dtype", [t for t in TYPES if t[0] != "int8"])
+@pytest.mark.parametrize("D", [64, 96, 128, 144, 256])
+@pytest.mark.parametrize("max_len", [None, 1])
+def test_sums_beside_an_infinite_one(gpu, codes, dtype, D, max_len):
+    """An infinite value (e4m3, which has none: a NaN) in one dim of a token: that dim is infinite, and the other
+    dims are as near to the formula as ever."""
+    from powershard_amd import ops
+    args = make([300, 5000, 33], 6, 2, D, 16, codes, dtype, gpu, seed=D)
+    v, table = args[2], args[3]
+    for b, (token, dim) in enumerate([(200, 5), (4999, D - 1), (0, 0)]):
+        at = v[table[b, token // 16], 1, token % 16]
+        if codes == "fp8":
+            at.view(torch.uint8)[dim] = 0x7F
+        else:
+            at[dim] = float("-inf") if b == 1 else float("inf")
+    got = ops.paged_attention(*args, max_len=max_len).double()
+    out, bound, _ = formula(*args)
+    wild = torch.zeros_like(out, dtype=torch.bool)
+    for b, dim in enumerate([5, D - 1, 0]):
+        wild[b, 3:, dim] = True
+    assert torch.equal(~torch.isfinite(got), wild)
+    if codes != "fp8":
+        assert torch.equal(got[wild], out[wild])
+    err = (got - out).abs()
+    assert (err <= U16[dtype] * out.abs() + 2.0 ** -25 + bound)[~wild].all()
+
+
 def test_tables_that_lead_nowhere(gpu):
     """A page outside the pool, or a length past the table, makes its sequence NaN and touches nothing else."""
     from powershard_amd import ops
