@@ -259,7 +259,9 @@ def gemm_fp8(a, a_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16, activa
 # could come, has memory of its own (paged_attention whose parts a second kernel joins).  A call that needs
 # more gets a larger one (at least twice the size, so a stream is replaced a few times at most), and
 # the replaced buffer is kept until the process ends: a launch captured into a graph keeps the
-# address it was given, which must not be handed out again.  At most _MAX_WS_STREAMS streams per
+# address it was given, which must not be handed out again.  None is made or replaced during a capture: a
+# captured call without one that is large enough runs unsplit.  Replays of a graph use the workspace of the stream
+# that captured it, so they must not overlap with each other or with that stream's calls.  At most _MAX_WS_STREAMS streams per
 # device get one; calls on further streams run without a workspace (the data-parallel tiles: the
 # same results, the split of K left out).  For capture and for callers that cannot allocate at all,
 # psq_gemm_w4a16_noalloc uses the library's own static scratch instead.
@@ -277,6 +279,8 @@ def _workspace(device, stream, nbytes):
     if ws is None and sum(1 for d, _ in _workspaces if d == device.index) >= _MAX_WS_STREAMS:
         return None, 0
     if ws is None or ws.numel() < nbytes:
+        if torch.cuda.is_current_stream_capturing():
+            return None, 0   # (the zeros would be the graph's: later calls would find counters that only its replays zero)
         size = max(nbytes, _WS_MIN_BYTES, 2 * ws.numel() if ws is not None else 0)
         if ws is not None:
             _retired_workspaces.append(ws)
