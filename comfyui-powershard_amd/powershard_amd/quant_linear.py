@@ -28,6 +28,7 @@ import contextlib
 import dataclasses
 import itertools
 import json
+import math
 import threading
 import warnings
 from typing import NamedTuple
@@ -250,6 +251,21 @@ class QuantizedRows(NamedTuple):
     def device(self):
         return self.codes.device
 
+    def check(self):
+        """ValueError unless the parts belong together."""
+        q, s = self.codes, self.scale
+        if q.dtype not in (torch.int8, torch.float8_e4m3fn) or q.dim() != 2:
+            raise ValueError(f"quantized rows must be int8 or float8_e4m3fn [M, K], got {q.dtype} {tuple(q.shape)}")
+        if s.dtype is not torch.float32 or s.shape != q.shape[:1] or s.device != q.device:
+            raise ValueError(f"quantized rows {tuple(q.shape)} on {q.device} need fp32 scales [M], got {s.dtype} {tuple(s.shape)} on {s.device}")
+        if self.shape[-1] != q.shape[1] or math.prod(self.shape[:-1]) != q.shape[0]:
+            raise ValueError(f"quantized rows {tuple(q.shape)} do not stand for rows {tuple(self.shape)}")
+
+    def plain(self):
+        """Whether codes and scales lie in memory as the library's dense rows do."""
+        q, s = self.codes, self.scale
+        return type(q) in PLAIN and type(s) in PLAIN and q.is_contiguous() and s.is_contiguous() and q.data_ptr() % 16 == 0
+
 
 class QuantLinear(nn.Module):
     """Linear whose weight is one QuantizedWeight byte vector (FSDP Shard(0) over bytes)."""
@@ -322,6 +338,7 @@ class QuantLinear(nn.Module):
         in forward_act: the native GEMM alone, the values of the forward on the rows that the codes stand
         for.  The result has the module's compute dtype."""
         want = self.input_codes()
+        rows.check()
         kind = "int8" if rows.codes.dtype is torch.int8 else "fp8"
         if want != (kind, rows.rot_group) or rows.codes.shape[1] != self.in_features:
             raise ValueError(f"forward_codes: {kind} rows [., {rows.codes.shape[1]}] rotated by {rows.rot_group} do not fit "
@@ -348,7 +365,7 @@ class QuantLinear(nn.Module):
         plan, store, bias, dtype = self._ps_qplan, self.qbytes, self.bias, self._ps_compute_dtype
         (_, code, (N, K), q_at, _), (name, sdtype, _, s_at, s_bytes) = plan.specs[:2]
         M, weights, count = rows.codes.shape[0], _Q8_WEIGHTS.get(code), s_bytes // 4
-        if (rows.dtype is not dtype or not M or not ops.direct_available() or self.__dict__.get("_ps_tracker") is not None
+        if (rows.dtype is not dtype or not M or not rows.plain() or not ops.direct_available() or self.__dict__.get("_ps_tracker") is not None
                 or type(store) not in PLAIN or not store.is_cuda or store.device != rows.device or not store.is_contiguous()
                 or store.numel() < plan.total or store.data_ptr() % 16 or name != "scale" or sdtype is not torch.float32
                 or weights is None or (activation is not None and weights == 2) or (activation == "silu_gate" and N % 128)

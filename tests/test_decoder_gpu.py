@@ -237,3 +237,27 @@ def test_step_in_a_graph(gpu):
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("fmt,opts", Q8)
+def test_forward_codes_of_rows_in_other_layouts(gpu, fmt, opts):
+    """Codes and scales that are slices, broadcasts or off 16 bytes have the values of dense ones."""
+    from powershard_amd import ops
+    from powershard_amd.quant_linear import QuantizedRows
+    layer, _, _ = make_layer(512, 96, fmt, opts, torch.bfloat16, True, gpu, seed=5)
+    kind, group = layer.input_codes()
+    x = heavy_rows(7, 512, 6).to(gpu)
+    q, scale = ops.quantize_rows(x, fp8=fmt == "fp8", rot_group=group)
+    rows = QuantizedRows(q, scale, group, (7, 512), torch.bfloat16)
+    want = layer.forward_codes(rows)
+    wide = torch.zeros(7, 1024, dtype=torch.uint8, device=gpu)
+    wide[:, 512:] = q.view(torch.uint8)
+    odd = torch.zeros(7 * 512 + 1, dtype=torch.uint8, device=gpu)[1:].view(7, 512)
+    odd.copy_(q.view(torch.uint8))
+    for codes in (wide[:, 512:].view(q.dtype), odd.view(q.dtype)):
+        assert torch.equal(layer.forward_codes(rows._replace(codes=codes)), want)
+    apart = torch.zeros(14, device=gpu)
+    apart[::2] = scale
+    assert torch.equal(layer.forward_codes(rows._replace(scale=apart[::2])), want)
+    one = rows._replace(codes=q[:1].expand(7, 512), scale=scale[:1].expand(7))
+    assert torch.equal(layer.forward_codes(one), want[:1].expand(7, 96))
