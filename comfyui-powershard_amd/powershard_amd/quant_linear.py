@@ -261,6 +261,13 @@ class QuantizedRows(NamedTuple):
         if self.shape[-1] != q.shape[1] or math.prod(self.shape[:-1]) != q.shape[0]:
             raise ValueError(f"quantized rows {tuple(q.shape)} do not stand for rows {tuple(self.shape)}")
 
+    def dequantize(self):
+        """The rows that the codes stand for: shape, dtype."""
+        x = self.codes.float() * self.scale[:, None]
+        if self.rot_group:   # rows H, and H H^T = I
+            x = (x.reshape(-1, self.rot_group) @ qtm.regular_hadamard(self.rot_group, x.device).T).reshape(x.shape)
+        return x.to(self.dtype).reshape(self.shape)
+
     def plain(self):
         """Whether codes and scales lie in memory as the library's dense rows do."""
         q, s = self.codes, self.scale
@@ -325,8 +332,12 @@ class QuantLinear(nn.Module):
     def input_codes(self):
         """("int8" or "fp8", ConvRot group) when the native forward quantizes its rows to that and does
         nothing else to them, so that forward_codes can take them; else None."""
+        return self._codes_of() if self._ps_native else None
+
+    def _codes_of(self):
+        """input_codes of the module as it is configured, whether or not its native forward failed since."""
         plan = self._ps_qplan
-        if (not self._ps_native or self._ps_full_precision or getattr(self, "_ps_safe", False) or self.in_features % 128
+        if (self._ps_full_precision or getattr(self, "_ps_safe", False) or self.in_features % 128
                 or self._ps_compute_dtype not in (torch.bfloat16, torch.float16) or any(s[0].startswith("x:") for s in plan.specs)):
             return None
         if plan.layout is qtm.Int8RowwiseLayout:
@@ -336,28 +347,28 @@ class QuantLinear(nn.Module):
     def forward_codes(self, rows, activation=None):
         """self of rows that are quantized already (QuantizedRows as input_codes asks for), activation as
         in forward_act: the native GEMM alone, the values of the forward on the rows that the codes stand
-        for.  The result has the module's compute dtype."""
-        want = self.input_codes()
+        for.  The result has the module's compute dtype, a text-encoder module's (follow_input) the rows'.
+        A module whose native forward failed, now or before, dequantizes rows and weight, as the forward does."""
+        want = self._codes_of()
         rows.check()
         kind = "int8" if rows.codes.dtype is torch.int8 else "fp8"
         if want != (kind, rows.rot_group) or rows.codes.shape[1] != self.in_features:
             raise ValueError(f"forward_codes: {kind} rows [., {rows.codes.shape[1]}] rotated by {rows.rot_group} do not fit "
                              f"[., {self.in_features}] {want}")
         dtype = self._ps_compute_dtype
-        out = self._codes_direct(rows, activation)
+        out = self._codes_direct(rows, activation) if self._ps_native else None
         if out is not None:
             return out
-        qt = unpack(self.qbytes, self._ps_qplan, dtype)
-        bias = None if self.bias is None else self.bias.to(dtype)
-        fused = None if activation == "silu_gate" and self.out_features % 128 else activation
-        out = gemm_codes(rows.codes, rows.scale, qt, bias, dtype, fused)
+        if self._ps_native:
+            qt = unpack(self.qbytes, self._ps_qplan, dtype)
+            bias = None if self.bias is None else self.bias.to(dtype)
+            fused = None if activation == "silu_gate" and self.out_features % 128 else activation
+            out = self._native_or_none(lambda: gemm_codes(rows.codes, rows.scale, qt, bias, dtype, fused))
+        if out is None:
+            return self._forward(rows.dequantize(), activation).to(rows.dtype if self._ps_follow_input else dtype)
         if activation is not None and fused is None:
             out = apply_activation(out, activation).to(dtype)
-        out = out.reshape(*rows.shape[:-1], out.shape[-1])
-        tracker = getattr(self, "_ps_tracker", None)
-        if tracker is not None:
-            tracker.observe(self._ps_finite_slot, out)
-        return out
+        return self._deliver(out, rows)
 
     def _codes_direct(self, rows, activation):
         """forward_codes in one library call, or None where _direct would not take the plain rows."""
@@ -392,15 +403,20 @@ class QuantLinear(nn.Module):
             return None, False
         # the fused gate pairs 64-column blocks: other widths take the gate as a separate pass
         act = None if activation == "silu_gate" and self.out_features % 128 else activation
+        out = self._native_or_none(lambda: native_linear(rows, qt, bias, self._ps_qplan.fmt, extras.get("input_scale"), act))
+        return out, out is not None and act is not None
+
+    def _native_or_none(self, call):
+        """call(), or None when it fails: the module dequantizes from then on, with one warning."""
         try:
-            return native_linear(rows, qt, bias, self._ps_qplan.fmt, extras.get("input_scale"), act), act is not None
+            return call()
         except torch.cuda.OutOfMemoryError:
             raise
         except NATIVE_FAILURES as error:
             warnings.warn(f"PowerShard: native {self._ps_qplan.fmt} GEMM unavailable ({error}); the module "
                           f"switches to dequantize")
             self._ps_native = False
-            return None, False
+            return None
 
     def _dequantized(self, rows, qt, bias):
         """F.linear on the dequantized weight; the V100 "FP16 safe" mode computes it in fp32."""
@@ -410,7 +426,7 @@ class QuantLinear(nn.Module):
 
     def _deliver(self, out, x):
         out = out.reshape(*x.shape[:-1], out.shape[-1])
-        if self._ps_follow_input and x.is_floating_point() and out.dtype != x.dtype:
+        if self._ps_follow_input and x.dtype.is_floating_point and out.dtype != x.dtype:
             out = out.to(x.dtype)  # text encoder: the FP32 graph is not narrowed to bf16 by the native kernel
         tracker = getattr(self, "_ps_tracker", None)
         if tracker is not None:

@@ -261,3 +261,20 @@ def test_forward_codes_of_rows_in_other_layouts(gpu, fmt, opts):
     assert torch.equal(layer.forward_codes(rows._replace(scale=apart[::2])), want)
     one = rows._replace(codes=q[:1].expand(7, 512), scale=scale[:1].expand(7))
     assert torch.equal(layer.forward_codes(one), want[:1].expand(7, 96))
+
+
+@pytest.mark.parametrize("fmt,opts", Q8)
+@pytest.mark.parametrize("activation", [None, "silu_gate"])
+def test_forward_codes_follows_the_rows_dtype(gpu, fmt, opts, activation):
+    """A text-encoder module gives back the dtype of the rows, as its forward does."""
+    from powershard_amd import ops
+    from powershard_amd.quant_linear import QuantizedRows
+    layer, _, _ = make_layer(512, 256, fmt, opts, torch.bfloat16, True, gpu, seed=5, follow_input=True)
+    kind, group = layer.input_codes()
+    x = heavy_rows(3, 512, 6).to(gpu)
+    q, scale = ops.quantize_rows(x, fp8=fmt == "fp8", rot_group=group)
+    for dtype in (torch.float16, torch.float32, torch.bfloat16):
+        got = layer.forward_codes(QuantizedRows(q, scale, group, (3, 512), dtype), activation)
+        want = layer(x) if activation is None else layer.forward_act(x, activation)
+        assert got.dtype is dtype and torch.equal(got, want.to(dtype))
+    assert layer._ps_native
