@@ -203,14 +203,14 @@ __device__ __forceinline__ void finish(const AttnArgs &a, int64_t head, int D, i
 
 // Adds up the parts of heads h0 .. h0 + n - 1 of a cut unit: part 0 is its first run's second, the others the
 // first ones of the runs after it.  A thread has one quad of dims (of every 256 / quads-th part, where
-// these are few), U parts' loads in flight.  smem: 6 KB.
+// these are few), U parts' loads in flight.  h0 is one of the unit's heads.  smem: 6 KB.
 template <int DT, int U>
 __device__ __forceinline__ void join_parts(const AttnArgs &a, const Cut &cut, int h0, int n, float *smem)
 {
     const int tid = threadIdx.x;
     const int hk = cut.unit / a.tiles, ht = cut.unit - hk * a.tiles, heads = min(a.G - ht * kTile, kTile);
     const int64_t row0 = cut.b * (int64_t)a.Hq + hk * a.G + ht * kTile;
-    const int quads = a.D / 4, first = h0 * quads, items = min(heads - h0, n) * quads, sharers = max(kThreads / max(items, 1), 1);
+    const int quads = a.D / 4, first = h0 * quads, items = min(heads - h0, n) * quads, sharers = max(kThreads / items, 1);
     const int share = sharers > 1 ? tid / items : 0;
     const __amdgpu_buffer_rsrc_t rs = raw_rsrc(a.part + (int64_t)(2 * cut.first) * a.part_floats);
     const int pitch = a.part_floats * 4, ml_at = heads * a.D * 4;
@@ -698,7 +698,8 @@ join_parts_kernel(AttnArgs a)
 {
     __shared__ __attribute__((aligned(16))) float smem[6 * kThreads];
     const Cut cut = a.cut[blockIdx.x];
-    if (cut.parts) join_parts<DT, 8>(a, cut, blockIdx.y, 1, smem);
+    const int heads = a.G - cut.unit % a.tiles * kTile;   // the last tile of a kv head may have fewer than the grid
+    if (cut.parts && (int)blockIdx.y < heads) join_parts<DT, 8>(a, cut, blockIdx.y, 1, smem);
 }
 
 // ------------------------------------------------------------------ the launch

@@ -182,6 +182,19 @@ def test_many_heads_share(gpu, codes, dtype, heads, lens):
     check(ops.paged_attention(*two, max_len=1), two)
 
 
+@pytest.mark.parametrize("heads", [17, 20, 31, 33, 47])
+@pytest.mark.parametrize("D", [16, 64, 128, 256])
+def test_last_tiles_of_few_heads_joined_apart(gpu, heads, D):
+    """The second kernel's grid has 16 heads for every tile; the last one of a kv head has fewer."""
+    from powershard_amd import _native, ops
+    args = make([40000, 5000], heads, 1, D, 16, "int8", torch.bfloat16, gpu)
+    assert _native.lib().psq_paged_attention_own_workspace(_native.CODES_I8, 2, heads, 1, D, args[3].shape[1] * 16) == 1
+    got, lse = ops.paged_attention(*args, return_lse=True)
+    check(got, args)
+    want = formula(*args)[2]
+    assert ((lse.double() - want).abs() <= 1e-4 + 1e-5 * want.abs()).all()
+
+
 @pytest.mark.parametrize("codes,dtype", [("none", torch.bfloat16), ("fp8", torch.float16)])
 @pytest.mark.parametrize("window", [1, 16, 100, 1000, 100000])
 def test_window_and_scale(gpu, codes, dtype, window):
