@@ -83,14 +83,26 @@ class DecoderLayer(nn.Module):
     def prompt(self, x, h, cache, layer, seq, slots):
         """The newest tokens of a sequence, x [tokens, hidden], whose slots cache.extend gave.  h: the
         residual stream (None in front of the first layer).  (x, h) for the next layer."""
+        return self(x, h, cache, layer, slots, seq=seq)
+
+    def step(self, x, h, cache, layer, slots, table):
+        """One new token of each sequence, x [batch, hidden]; table: cache.table(seqs) with it counted."""
+        return self(x, h, cache, layer, slots, table=table)
+
+    def forward(self, x, h, cache, layer, slots, seq=None, table=None):
+        """prompt (seq) or step (table), as a module call: a sharded layer gathers its weights in its hooks."""
+        if (seq is None) == (table is None):
+            raise ValueError("a decoder layer takes a prompt's sequence or a step's table")
+        return self._step(x, h, cache, layer, slots, table) if seq is None else self._prompt(x, h, cache, layer, seq, slots)
+
+    def _prompt(self, x, h, cache, layer, seq, slots):
         first = cache.length(seq) - x.shape[0]
         q, k, v, h = self._projections(x, h, torch.arange(first, first + x.shape[0], device=x.device))
         cache.write(layer, k, v, slots)
         # (fp32: the values that the codes stand for, as the step's attention takes them)
         return self._rest(prompt_attention(q, *cache.read(layer, cache.slots(seq), torch.float32), first), h)
 
-    def step(self, x, h, cache, layer, slots, table):
-        """One new token of each sequence, x [batch, hidden]; table: cache.table(seqs) with it counted."""
+    def _step(self, x, h, cache, layer, slots, table):
         block_table, lengths, longest = table
         q, k, v, h = self._projections(x, h, lengths - 1)
         cache.write(layer, k, v, slots)

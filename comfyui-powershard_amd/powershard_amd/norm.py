@@ -22,9 +22,8 @@ def rows_for(linears):
 
 
 def linear(module, rows, activation=None):
-    """module(rows) for rows as RMSNorm returns them; activation as in QuantLinear.forward_act."""
-    if isinstance(rows, QuantizedRows):
-        return module.forward_codes(rows, activation)
+    """module(rows) for rows as RMSNorm returns them, the module's hooks included; activation as in
+    QuantLinear.forward_act."""
     return module(rows) if activation is None else module.forward_act(rows, activation)
 
 

@@ -306,9 +306,9 @@ class QuantLinear(nn.Module):
         return f"{self.in_features}, {self.out_features}, format={self._ps_qplan.fmt}, native={self._ps_native}"
 
     def forward(self, x, into=None):
-        """self(x).  into (an MLP's result rows, [x rows, out_features]): memory that the native
-        kernels may write the output to, in its dtype; the caller copies when another tensor comes
-        back."""
+        """self(x); x may be QuantizedRows (forward_codes).  into (an MLP's result rows, [x rows, out_features]):
+        memory that the native kernels may write the output to, in its dtype; the caller copies when another
+        tensor comes back."""
         return self._forward(x, None, into)
 
     def forward_act(self, x, activation="gelu_tanh"):
@@ -331,8 +331,8 @@ class QuantLinear(nn.Module):
 
     def input_codes(self):
         """("int8" or "fp8", ConvRot group) when the native forward quantizes its rows to that and does
-        nothing else to them, so that forward_codes can take them; else None."""
-        return self._codes_of() if self._ps_native else None
+        nothing else to them, so that forward_codes can take them; else None (a replaced forward among them)."""
+        return self._codes_of() if self._ps_native and "forward" not in self.__dict__ else None
 
     def _codes_of(self):
         """input_codes of the module as it is configured, whether or not its native forward failed since."""
@@ -506,6 +506,8 @@ class QuantLinear(nn.Module):
             out = self._direct(x, activation, into)
             if out is not None:
                 return out
+        if type(x) is QuantizedRows:
+            return self.forward_codes(x, activation)
         dtype = self._dtype_for(x)
         qt, extras = unpack(self.qbytes, self._ps_qplan, dtype, with_extras=True)
         rows = x.reshape(-1, x.shape[-1]).to(dtype)

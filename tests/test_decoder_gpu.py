@@ -278,3 +278,22 @@ def test_forward_codes_follows_the_rows_dtype(gpu, fmt, opts, activation):
         want = layer(x) if activation is None else layer.forward_act(x, activation)
         assert got.dtype is dtype and torch.equal(got, want.to(dtype))
     assert layer._ps_native
+
+
+def test_layers_and_linears_run_their_hooks(gpu):
+    """prompt and step are module calls, and the linears are called as modules with the norm's codes."""
+    from powershard_amd.kv_cache import PagedKVCache
+    from powershard_amd.quant_linear import QuantizedRows
+    layers, _ = decoder("int8", ROT, gpu, layers=1)
+    calls, x = [], heavy_rows(5, HIDDEN, 61, outlier_frac=0).to(gpu)
+    cache = PagedKVCache(1, 4, 16, KV, DIM, device=gpu)
+    seq = cache.open()
+    layer = layers[0]
+    layer.register_forward_pre_hook(lambda m, args: calls.append("layer"))
+    layer.q_proj.register_forward_pre_hook(lambda m, args: calls.append(type(args[0])))
+    with torch.no_grad():
+        run_prompt(layers, cache, seq, x)
+        run_step(layers, cache, [seq], x[:1])
+    assert calls == ["layer", QuantizedRows] * 2
+    with pytest.raises(ValueError):
+        layer(x, None, cache, 0, cache.slots(seq))

@@ -96,3 +96,23 @@ def test_out_of_memory_is_not_a_native_failure(monkeypatch):
     with pytest.raises(torch.cuda.OutOfMemoryError):
         module.forward_codes(rows())
     assert module._ps_native
+
+
+def test_the_module_call_takes_codes_and_runs_its_hooks():
+    """norm.linear calls the module: hooks (a sharded layer's among them) run around forward_codes, and a replaced
+    forward is given rows, not codes."""
+    from powershard_amd.norm import linear, rows_for
+    module = layer("int8", opts={"convrot": False})
+    weight = quantized_from_float(torch.randn(64, 128), module._ps_qplan.fmt, convrot=False)
+    module.qbytes = torch.nn.Parameter(pack(weight, module._ps_qplan, "cpu"), requires_grad=False)
+    module.bias = None
+    seen = []
+    module.register_forward_pre_hook(lambda m, args: seen.append(type(args[0])))
+    module.register_forward_hook(lambda m, args, out: seen.append(out.shape))
+    with pytest.warns(UserWarning, match="switches to dequantize"):
+        linear(module, rows())
+    assert seen == [QuantizedRows, (2, 3, 64)]
+    module._ps_native = True
+    assert rows_for([module]) == ("int8", 0)
+    module.forward = lambda x: x
+    assert rows_for([module]) is None
