@@ -13,13 +13,15 @@ Each ``csrc/*.hip`` compiles to an object under ``_build/``; the objects link in
 * ``-Xclang -target-feature -Xclang -packed-fp32-ops``: no packed fp32 VALU instructions.
 
 ``csrc/direct.cpp`` (host code only) is built beside it with the host compiler against the installed
-torch's headers: ``lib/psq_direct.so``.
+torch's headers: ``lib/psq_direct.so``.  The library works without it (the decoder operators' calls take longer), so
+where that fails (no host compiler, no torch headers) the build says so and goes on.
 """
 import argparse
 import concurrent.futures
 import os
 import subprocess
 import sys
+import warnings
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -57,6 +59,15 @@ def _compile(src):
 
 
 def _build_direct():
+    """lib/psq_direct.so, or a warning and no such file: one of another build would not fit the library."""
+    try:
+        _compile_direct()
+    except Exception as error:   # whatever the compiler or torch's build helpers run into
+        DIRECT.unlink(missing_ok=True)
+        warnings.warn(f"psquant: {DIRECT.name} was not built: {error}")
+
+
+def _compile_direct():
     """lib/psq_direct.so, the CPython module of the decoder operators' direct calls."""
     import sysconfig
 

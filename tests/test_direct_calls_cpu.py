@@ -30,3 +30,16 @@ def test_a_foreign_module_is_not_used(monkeypatch, tmp_path):
 def test_bind_takes_a_dict():
     from powershard_amd._native import DIRECT_CALLS, SIGNATURES
     assert set(DIRECT_CALLS) <= set(SIGNATURES)
+
+
+@pytest.mark.parametrize("compiler", ["/no/such/compiler", "false"])
+def test_the_library_builds_without_a_host_compiler(monkeypatch, tmp_path, compiler):
+    """The module is optional: its build fails with a warning, and leaves none of an earlier build."""
+    from powershard_amd import build_lib
+    old = tmp_path / "psq_direct.so"
+    old.write_bytes(b"of another build")
+    monkeypatch.setattr(build_lib, "DIRECT", old)
+    monkeypatch.setenv("CXX", compiler)
+    with pytest.warns(UserWarning, match="was not built"):
+        build_lib._build_direct()
+    assert not old.exists()
