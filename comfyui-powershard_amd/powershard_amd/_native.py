@@ -11,6 +11,7 @@ The reference loads its own native helper the same way -- a runtime-built ``.so`
 import ctypes
 import importlib.util
 import os
+import sys
 import threading
 import warnings
 from pathlib import Path
@@ -105,8 +106,8 @@ _direct = None
 
 def direct():
     """The module of the decoder operators' direct calls (csrc/direct.cpp), bound to the loaded library, or
-    False where it cannot be used: it belongs to one release of torch, and the calls that it shortens
-    work without it.  A missing or foreign module is named in one warning."""
+    False where it cannot be used: it belongs to one release of torch and of Python, and the calls that it
+    shortens work without it.  A missing or foreign module is named in one warning."""
     global _direct
     if _direct is None:
         handle = lib()
@@ -123,6 +124,8 @@ def _load_direct(handle):
         module = importlib.util.module_from_spec(spec)
         if module.TORCH_VERSION != torch.__version__.split("+")[0]:
             raise ImportError(f"built for torch {module.TORCH_VERSION}, this is {torch.__version__}")
+        if module.PYTHON_VERSION != sys.hexversion >> 16:
+            raise ImportError(f"built for Python {module.PYTHON_VERSION >> 8}.{module.PYTHON_VERSION & 255}, this is {sys.version.split()[0]}")
         module.bind({name: ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in DIRECT_CALLS})
     except ImportError as error:
         warnings.warn(f"psquant: {DIRECT_PATH} is not used ({error}): the decoder operators' calls take longer", stacklevel=4)

@@ -308,6 +308,7 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "psq_direct", nullptr, -1, methods,
 PyMODINIT_FUNC PyInit_psq_direct(void)
 {
     PyObject *m = PyModule_Create(&module);
-    if (m && PyModule_AddStringConstant(m, "TORCH_VERSION", TORCH_VERSION) < 0) Py_CLEAR(m);
+    if (m && (PyModule_AddStringConstant(m, "TORCH_VERSION", TORCH_VERSION) < 0 || PyModule_AddIntConstant(m, "PYTHON_VERSION", PY_VERSION_HEX >> 16) < 0))
+        Py_CLEAR(m);
     return m;
 }

@@ -32,6 +32,15 @@ def test_bind_takes_a_dict():
     assert set(DIRECT_CALLS) <= set(SIGNATURES)
 
 
+def test_belongs_to_this_python(monkeypatch):
+    import sys
+    assert _native.direct().PYTHON_VERSION == sys.hexversion >> 16
+    monkeypatch.setattr(_native, "_direct", None)
+    monkeypatch.setattr(_native.sys, "hexversion", sys.hexversion + (1 << 16))
+    with pytest.warns(UserWarning, match="built for Python"):
+        assert _native.direct() is False
+
+
 @pytest.mark.parametrize("compiler", ["/no/such/compiler", "false"])
 def test_the_library_builds_without_a_host_compiler(monkeypatch, tmp_path, compiler):
     """The module is optional: its build fails with a warning, and leaves none of an earlier build."""
