@@ -267,6 +267,7 @@ def gemm_fp8(a, a_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16, activa
 # psq_gemm_w4a16_noalloc uses the library's own static scratch instead.
 _workspaces = {}
 _retired_workspaces = []
+_workspaces_lock = threading.Lock()
 _MAX_WS_STREAMS = 16
 _WS_MIN_BYTES = 1 << 20
 
@@ -276,17 +277,28 @@ def _workspace(device, stream, nbytes):
         return None, 0
     key = (device.index, stream)
     ws = _workspaces.get(key)
-    if ws is None and sum(1 for d, _ in _workspaces if d == device.index) >= _MAX_WS_STREAMS:
-        return None, 0
     if ws is None or ws.numel() < nbytes:
-        if torch.cuda.is_current_stream_capturing():
-            return None, 0   # (the zeros would be the graph's: later calls would find counters that only its replays zero)
-        size = max(nbytes, _WS_MIN_BYTES, 2 * ws.numel() if ws is not None else 0)
-        if ws is not None:
-            _retired_workspaces.append(ws)
-        ws = torch.zeros(size, dtype=torch.uint8, device=device)   # counter words zero once; calls leave them so
-        _workspaces[key] = ws
+        with _workspaces_lock:
+            ws = _larger_workspace(key, device, nbytes)
+        if ws is None:
+            return None, 0
     return ws, ws.numel()
+
+
+def _larger_workspace(key, device, nbytes):
+    ws = _workspaces.get(key)
+    if ws is not None and ws.numel() >= nbytes:   # another thread was first
+        return ws
+    if ws is None and sum(1 for d, _ in _workspaces if d == device.index) >= _MAX_WS_STREAMS:
+        return None
+    if torch.cuda.is_current_stream_capturing():
+        return None   # (the zeros would be the graph's: later calls would find counters that only its replays zero)
+    size = max(nbytes, _WS_MIN_BYTES, 2 * ws.numel() if ws is not None else 0)
+    if ws is not None:
+        _retired_workspaces.append(ws)
+    ws = torch.zeros(size, dtype=torch.uint8, device=device)   # counter words zero once; calls leave them so
+    _workspaces[key] = ws
+    return ws
 
 
 def gemm_w4a16(x, wq, w_scale, w_zero, group_size, bias=None, out_dtype=None):
