@@ -499,6 +499,8 @@ def dequant_i8_rows(q, w_scale, rot_group=0, out_dtype=torch.bfloat16):
     if w_scale.dtype is not torch.float32 or not w_scale.is_contiguous():
         w_scale = w_scale.to(torch.float32).contiguous()
     N, K = q.shape
+    if w_scale.numel() != N:
+        raise ValueError(f"dequant_i8_rows: {w_scale.numel()} scales for {N} rows")
     out = torch.empty((N, K), dtype=out_dtype, device=q.device)
     _call("dequant_i8_rows", _native.lib().psq_dequant_i8_rows, q.data_ptr(), w_scale.data_ptr(), N, K, int(rot_group or 0),
           out.data_ptr(), _dt(out, "out"), _raw(q.get_device()))

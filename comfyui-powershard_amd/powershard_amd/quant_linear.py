@@ -379,7 +379,8 @@ class QuantLinear(nn.Module):
         if (rows.dtype is not dtype or not M or not rows.plain() or not ops.direct_available() or self.__dict__.get("_ps_tracker") is not None
                 or type(store) not in PLAIN or not store.is_cuda or store.device != rows.device or not store.is_contiguous()
                 or store.numel() < plan.total or store.data_ptr() % 16 or name != "scale" or sdtype is not torch.float32
-                or weights is None or (activation is not None and weights == 2) or (activation == "silu_gate" and N % 128)
+                or weights is None or (count != N and (count != 1 or not weights))
+                or (activation is not None and weights == 2) or (activation == "silu_gate" and N % 128)
                 or (bias is not None and (type(bias) not in PLAIN or bias.dtype is not dtype or bias.device != rows.device
                                           or bias.numel() != N or not bias.is_contiguous()))):
             return None

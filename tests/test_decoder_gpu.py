@@ -297,3 +297,22 @@ def test_layers_and_linears_run_their_hooks(gpu):
     assert calls == ["layer", QuantizedRows] * 2
     with pytest.raises(ValueError):
         layer(x, None, cache, 0, cache.slots(seq))
+
+
+def test_int8_scales_are_counted(gpu):
+    """A kernel reads one scale per int8 row: fewer are refused (forward_codes: one warning first, as the forward)."""
+    from powershard_amd import ops
+    from powershard_amd import quant_tensor as qtm
+    from powershard_amd.quant_linear import QuantizedRows, QuantPlan, pack
+    q = torch.ones(96, 512, dtype=torch.int8, device=gpu)
+    with pytest.raises(ValueError):
+        ops.dequant_i8_rows(q, torch.ones(1, device=gpu))
+    with pytest.raises(ValueError):
+        ops.dequant_i8_rows(q, torch.ones(97, 1, device=gpu))
+    layer, _, _ = make_layer(512, 96, "int8", {"convrot": False}, torch.bfloat16, True, gpu, seed=5)
+    weight = qtm.QuantizedWeight(q, qtm.Int8RowwiseLayout, qtm.Int8RowwiseParams(torch.ones(1, device=gpu)))
+    layer._ps_qplan = QuantPlan.of(weight, layer._ps_qplan.fmt, {})
+    layer.qbytes = nn.Parameter(pack(weight, layer._ps_qplan, gpu), requires_grad=False)
+    rows = QuantizedRows(q[:5].clone(), torch.ones(5, device=gpu), 0, (5, 512), torch.bfloat16)
+    with pytest.warns(UserWarning, match="switches to dequantize"), pytest.raises(ValueError):
+        layer.forward_codes(rows)
