@@ -3,7 +3,7 @@
 // At one token the host's part of a call is longer than its kernel, and in Python most of it is the checks
 // of up to eight tensors, the allocations and the foreign call's 16 to 27 arguments.  Host time of a call of ops.py,
 // its general path and through here: add_rms_norm (x + residual, int8) 11.0 and 6.0 us, kv_write 7.6 and 3.5,
-// kv_read 9.7 and 5.5, paged_attention 10.4 and 5.0 (with a second launch for the join 13.9 and 7.8).
+// kv_read 9.7 and 5.5, paged_attention 10.4 and 5.0 (with a second launch for the join, and memory for its parts, 15.0 and 8.1).
 //
 // The functions take what ops.py was called with and the current stream, and return None whenever the
 // arguments are not plainly what the library takes (another type or layout, a copy to make, something to

@@ -5,7 +5,7 @@
 // Bound by the cache's bytes: each key and value is read once for the G = Hq / Hkv heads that share it.
 // A workgroup of 4 waves takes a run of tokens of one sequence and kv head, for up to 16 of its heads
 // (more heads to a kv head: more workgroups, which find the cache's lines in the last-level cache; waves of
-// one workgroup side by side on the same tokens measured slower, 16 x 8192, 64 heads on one 32 | 42 us,
+// one workgroup side by side on the same tokens measured slower, 16 x 8192, 64 heads on one 32 | 42 us (28 now),
 // their runs being shorter and their parts longer); its waves take steps of 32 tokens in turn, and each keeps a running maximum, sum and output of its own
 // (no barrier inside the run).  Everything goes from memory to registers in the layout that the matrix
 // instructions read (16x16x32, fp32 accumulation), with no LDS and no cross-lane move of keys, values or
@@ -710,7 +710,12 @@ join_parts_kernel(AttnArgs a)
 // 3.5 us of the host's time, which bounds the small calls): 1 x 2000 tokens, 40 heads on 8, int8 14.0 | 18.7;
 // 1 x 4000, 16 on 16 13.8 | 18.2; 61 x 4096, 40 on 8 63.5 | 65.9; 128 x 8192, 64 on 8, bf16 377 | 386;
 // 4 x 16000, 40 on 8 30.1 | 26.0; 1 x 131071, 40 on 8, fp8 66.6 | 57.9 (3 per CU 58.9); 1 x 30000, 8 on 1
-// 35 | 18; 8 x 6000, 16 on 1, 256 dims 33 | 19.
+// 35 | 18; 8 x 6000, 16 on 1, 256 dims 33 | 19.  At the limit of one round, 8 heads of 128 dims, int8, 4000
+// tokens: 12 parts a unit 20.1 | 20.2, 16 18.7 | 19.0, 24 16.8 | 15.7.
+// Where a part has more quads of dims than a workgroup threads, these take turns, and the limit is 4 parts a
+// unit: 16 heads of 256 dims, int8, 4000 tokens, 3 parts 89.2 | 85.5, 4 63.9 | 63.2, 5 64.7 | 57.4, 8 40.7 | 37.2,
+// 12 39.1 | 29.7 (1500 tokens, 4 32.1 | 31.8, 5 39.9 | 32.6); 5 heads of 256 dims 4 59.1 | 58.4, 5 54.2 | 51.0; 16 heads
+// of 128 dims 4 48.9 | 53.4, 5 45.5 | 46.8, 8 29.1 | 31.6, 12 22.8 | 21.2 (1500 tokens, 4 24.2 | 29.1, 5 27.8 | 26.3).
 struct Plan {
     int tiles, part_floats;
     bool apart;
@@ -731,7 +736,7 @@ Plan plan(int codes, int64_t B, int Hq, int Hkv, int D, int64_t max_len)
     const int most = groups_per_cu(D, codes != PSQ_CODES_NONE);
     p.groups = std::min<int64_t>(cus * most, rounds);
     const int items = heads * D / 4, loads = (D <= 64 ? 8 : 16) * std::max(kThreads / items, 1);   // of join_parts
-    p.apart = p.groups > units * loads || (items > kThreads && p.groups > 4 * units);
+    p.apart = p.groups > units * (items > kThreads ? 4 : loads);
     if (p.apart) p.groups = std::min<int64_t>(cus * std::min(most, 2), rounds);
     p.part_floats = (heads * (D + 2) + 31) / 32 * 32;   // whole lines
     p.cuts_at = kCounterBytes;

@@ -310,7 +310,8 @@ enum psq_codes { PSQ_CODES_NONE = 0, PSQ_CODES_I8 = 1, PSQ_CODES_E4M3 = 2 };
  *   PSQ_CODES_NONE: out = round_x(y); scale unused
  * The normalized row is never rounded to 16 bits on its way to the codes.  The factor
  * 1 / sqrt(...) > 0 scales y and max|y| alike, so the codes do not depend on it, only the scale does.
- * A row holding a NaN or Inf gets a NaN scale (codes) or NaN elements.
+ * A row holding a NaN or Inf gets a NaN scale (codes) or NaN elements.  A static scale stays as it is, and a NaN
+ * product takes the lower code bound, as in psq_quantize_rows_i8.
  *   x, residual, sum [M, K] bf16/f16 (ldx, ldr, lds elements, multiples of 8, 16-byte aligned; sum may
  *   be x or residual), weight [K] (weight_dtype, 16-byte aligned), out [M, K] (ldo elements, a multiple
  *   of 16; of 8 for PSQ_CODES_NONE), K a multiple of 16, at most 32768. */
