@@ -57,6 +57,8 @@ SIGNATURES = {
     "psq_dequant_e5m2": (_I, [_P, _P, _I, _I64, _I64, _P, _I, _P]),
     "psq_add_rms_norm": (_I, [_I, _P, _I, _I64, _P, _I64, _P, _I, _F, _P, _I64, _I, _P, _P, _I64, _P, _I64, _I64, _P]),
     "psq_kv_write": (_I, [_I, _P, _P, _I, _I64, _I64, _I64, _I64, _P, _I64, _I, _I, _P, _P, _P, _P, _I64, _I, _P]),
+    "psq_rope_kv_write": (_I, [_I, _P, _P, _P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I, _I, _I64, _P, _P, _I, _I, _P, _I64,
+                               _I, _I, _I, _P, _P, _P, _P, _I64, _I, _P, _P]),
     "psq_kv_read": (_I, [_I, _P, _I64, _P, _P, _I, _P, _P, _I64, _I, _I, _I, _P, _P, _I, _P]),
     "psq_paged_attention_workspace_bytes": (_I64, [_I, _I64, _I, _I, _I, _I64]),
     "psq_paged_attention_own_workspace": (_I, [_I, _I64, _I, _I, _I, _I64]),

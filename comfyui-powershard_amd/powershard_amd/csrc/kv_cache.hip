@@ -23,34 +23,6 @@ struct KvArgs {
     int H, D, page;
 };
 
-template <int DT>
-__device__ __forceinline__ void load16(const uint16_t *p, float (&f)[16])
-{
-    const v4i raw[2] = {((const v4i *)p)[0], ((const v4i *)p)[1]};
-    to_f32<DT>(raw, f);
-}
-
-// row of the pools that slot s of head h occupies
-__device__ __forceinline__ int64_t pool_row(int64_t s, uint32_t h, const KvArgs &a)
-{
-    const int64_t p = s >> 32 ? s / a.page : (int64_t)((uint32_t)s / (uint32_t)a.page);
-    return (p * a.H + h) * a.page + (s - p * a.page);
-}
-
-// 16 codes of f at mul
-template <int CODES>
-__device__ __forceinline__ v4i codes16(const float (&f)[16], float mul)
-{
-    v4i q;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float u0 = f[4 * i] * mul, u1 = f[4 * i + 1] * mul, u2 = f[4 * i + 2] * mul, u3 = f[4 * i + 3] * mul;
-        if constexpr (CODES == PSQ_CODES_I8) q[i] = (int)i8_codes4(u0, u1, u2, u3, kRoundMagic);
-        else q[i] = (int)e4m3_codes4(u0, u1, u2, u3);
-    }
-    return q;
-}
-
 // L lanes per row (the power of two that covers D / 16), rows = (token, head)
 template <int DT, int CODES, int L>
 __global__ void __launch_bounds__(kThreads)
@@ -62,7 +34,7 @@ kv_write_kernel(KvArgs a)
     if (t >= a.T) return;   // all lanes of a row leave together
     const int64_t s = a.slots[t];
     if (s < 0 || s >= a.nslots) return;
-    const int64_t at = pool_row(s, h, a);
+    const int64_t at = pool_row(s, h, a.H, a.page);
     const uint16_t *k = a.k + t * a.k_token + h * a.k_head + e, *v = a.v + t * a.v_token + h * a.v_head + e;
     const bool here = e < a.D;
     if constexpr (CODES == PSQ_CODES_NONE) {
@@ -149,7 +121,7 @@ kv_read_kernel(KvArgs a, void *k, void *v)
     const int64_t s = a.slots[t];
     float fk[16] = {}, fv[16] = {};
     if (s >= 0 && s < a.nslots) {
-        const int64_t at = pool_row(s, h, a);
+        const int64_t at = pool_row(s, h, a.H, a.page);
         row16<DT, CODES>(a.kc, a.ks, at, a.D, e, fk);
         row16<DT, CODES>(a.vc, a.vs, at, a.D, e, fv);
     }

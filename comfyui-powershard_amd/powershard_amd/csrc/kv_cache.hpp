@@ -1,9 +1,38 @@
-// kv_cache.hpp -- what the paged cache's kernels share: its shape.
+// kv_cache.hpp -- what the paged cache's kernels share: its shape, rows of 16 elements, codes.
 #pragma once
 
 #include "quantize.hpp"
 
 namespace psq {
+
+// 16 elements of DT (16-byte aligned) as fp32
+template <int DT>
+__device__ __forceinline__ void load16(const uint16_t *p, float (&f)[16])
+{
+    const v4i raw[2] = {((const v4i *)p)[0], ((const v4i *)p)[1]};
+    to_f32<DT>(raw, f);
+}
+
+// row of the pools that slot s of head h occupies
+__device__ __forceinline__ int64_t pool_row(int64_t s, uint32_t h, int heads, int page)
+{
+    const int64_t p = s >> 32 ? s / page : (int64_t)((uint32_t)s / (uint32_t)page);
+    return (p * heads + h) * page + (s - p * page);
+}
+
+// 16 codes of f at mul
+template <int CODES>
+__device__ __forceinline__ v4i codes16(const float (&f)[16], float mul)
+{
+    v4i q;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float u0 = f[4 * i] * mul, u1 = f[4 * i + 1] * mul, u2 = f[4 * i + 2] * mul, u3 = f[4 * i + 3] * mul;
+        if constexpr (CODES == PSQ_CODES_I8) q[i] = (int)i8_codes4(u0, u1, u2, u3, kRoundMagic);
+        else q[i] = (int)e4m3_codes4(u0, u1, u2, u3);
+    }
+    return q;
+}
 
 // host checks of the pools: sizes, alignment, scales present exactly with codes
 inline int check_kv_cache(const char *name, int codes, const void *k_cache, const void *v_cache, const float *k_scale,

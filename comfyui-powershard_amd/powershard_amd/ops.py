@@ -675,6 +675,57 @@ def kv_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
           slots.data_ptr(), T, H, D, k_cache.data_ptr(), v_cache.data_ptr(), ks, vs, pages, page, _raw(index))
 
 
+def rope_kv_write(q, k, v, positions, inv_freq, slots, k_cache, v_cache, k_scale=None, v_scale=None, axes=None, interleaved=False):
+    """kv_write of keys turned to their positions, and the turned queries [tokens, heads, head dim].
+
+    q: [tokens, heads, head dim], k, v, slots and the pools as in kv_write.  inv_freq: [pairs] float64 (other
+    types are converted on each call), the angle per position of each pair, pairs a multiple of 8; pair i is
+    the elements i and i + pairs of a row, 2 i and 2 i + 1 when interleaved; elements from 2 * pairs on stay as
+    they are.  positions: [tokens] int32 or int64, or [n, tokens] with axes, [pairs] int32: which of the n
+    positions (time, height and width, say) turns each pair.  Angles are worked out in
+    fp64; keys are turned in fp32 and quantized from there.
+    """
+    index = q.get_device()
+    code, (pages, H, page, D), ks, vs = _pools("rope_kv_write", index, k_cache, v_cache, k_scale, v_scale)
+    for t in (k, v, positions, inv_freq) + (() if axes is None else (axes,)):
+        if t.get_device() != index:
+            _elsewhere("rope_kv_write", q, t)
+    dtype, shape = q.dtype, k.shape
+    dt = _HALF.get(dtype)
+    if dt is None or k.dtype is not dtype or v.dtype is not dtype or (not code and k_cache.dtype is not dtype):
+        raise TypeError(f"rope_kv_write: queries {dtype}, keys {k.dtype} and values {v.dtype} do not fit a {k_cache.dtype} cache")
+    if len(shape) != 3 or v.shape != shape or shape[1] != H or shape[2] != D:
+        raise ValueError(f"rope_kv_write: keys {tuple(shape)} and values {tuple(v.shape)} must be [tokens, {H}, {D}]")
+    T = shape[0]
+    if q.dim() != 3 or q.shape[0] != T or q.shape[2] != D:
+        raise ValueError(f"rope_kv_write: queries {tuple(q.shape)} must be [{T}, heads, {D}]")
+    if inv_freq.dim() != 1 or not 0 < 2 * inv_freq.shape[0] <= D or inv_freq.shape[0] % 8:
+        raise ValueError(f"rope_kv_write: inv_freq {tuple(inv_freq.shape)} must have a multiple of 8 pairs, at most {D // 2}")
+    pairs = inv_freq.shape[0]
+    if positions.dtype not in (torch.int32, torch.int64) or positions.shape[-1:] != (T,) or positions.dim() != (1 if axes is None else 2):
+        raise ValueError(f"rope_kv_write: positions must be int32 or int64 [{T}], or [n, {T}] with axes, got {positions.dtype} "
+                         f"{tuple(positions.shape)}")
+    if axes is not None and (axes.dtype is not torch.int32 or axes.shape != (pairs,) or positions.shape[0] == 0):
+        raise ValueError(f"rope_kv_write: axes must be int32 [{pairs}] for one row of positions or more")
+    slots = _slots("rope_kv_write", slots, index, T)
+    if inv_freq.dtype is not torch.float64 or not inv_freq.is_contiguous():
+        inv_freq = inv_freq.to(torch.float64).contiguous()
+    if positions.stride(-1) != 1:
+        positions = positions.contiguous()
+    if axes is not None and not axes.is_contiguous():
+        axes = axes.contiguous()
+    q, q_token, q_head = _heads(q)
+    k, k_token, k_head = _heads(k)
+    v, v_token, v_head = _heads(v)
+    out = torch.empty(q.shape, dtype=dtype, device=q.device)
+    _call("rope_kv_write", _native.lib().psq_rope_kv_write, code, q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, q_token, q_head, k_token,
+          k_head, v_token, v_head, positions.data_ptr(), 64 if positions.dtype is torch.int64 else 32,
+          1 if axes is None else positions.shape[0], 0 if axes is None else positions.stride(0), None if axes is None else axes.data_ptr(),
+          inv_freq.data_ptr(), 2 * pairs, int(bool(interleaved)), slots.data_ptr(), T, q.shape[1], H, D, k_cache.data_ptr(),
+          v_cache.data_ptr(), ks, vs, pages, page, out.data_ptr(), _raw(index))
+    return out
+
+
 def kv_read(slots, k_cache, v_cache, k_scale=None, v_scale=None, out_dtype=None):
     """Cached tokens back as dense rows: (k, v), each [tokens, kv heads, head dim] of out_dtype (default: the
     cache's dtype, bf16 for codes).  slots as in kv_write; a negative slot reads as zeros."""

@@ -334,6 +334,25 @@ PSQ_API int psq_kv_write(int codes, const void *k, const void *v, int dtype, int
                  int64_t v_head, const int64_t *slots, int64_t T, int Hkv, int D, void *k_cache, void *v_cache,
                  float *k_scale, float *v_scale, int64_t num_pages, int page_size, void *stream);
 
+/* psq_kv_write with the positions turned on the way: queries and keys are rotated by pairs, then keys and values
+ * appended.  For pair i of a row, i < rotary / 2, elements (i, i + rotary / 2), or (2 i, 2 i + 1) with interleaved:
+ *   t = position * inv_freq[i];  (a, b) <- (a cos t - b sin t, b cos t + a sin t)
+ * elements past `rotary` stay as they are.  t is worked out in fp64 and its whole turns are dropped before it is rounded
+ * (positions up to 2^31 lose nothing that fp32 sines would show); sines and products are fp32.  Queries are rounded once to their type; keys in a cache of codes are not rounded before
+ * they are quantized (in a 16-bit one they are rounded once).
+ *   q [T, Hq, D], k, v [T, Hkv, D] bf16/f16 (element strides as in psq_kv_write), q_out [T, Hq, D] dense
+ *   positions: T integers of positions_bits (32 or 64), `axes` rows of them axis_stride elements apart;
+ *   pair_axis [rotary / 2] int32: the axis whose position turns each pair (values outside 0 .. axes - 1: the
+ *   nearest axis), NULL for one axis
+ *   inv_freq [rotary / 2] fp64; rotary a multiple of 16, at most D
+ * Queries of tokens whose slot is negative or past the pool are turned all the same. */
+PSQ_API int psq_rope_kv_write(int codes, const void *q, const void *k, const void *v, int dtype, int64_t q_token,
+                      int64_t q_head, int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head,
+                      const void *positions, int positions_bits, int axes, int64_t axis_stride, const int32_t *pair_axis,
+                      const double *inv_freq, int rotary, int interleaved, const int64_t *slots, int64_t T, int Hq,
+                      int Hkv, int D, void *k_cache, void *v_cache, float *k_scale, float *v_scale, int64_t num_pages,
+                      int page_size, void *q_out, void *stream);
+
 /* Reads T tokens back as dense rows: k, v [T, Hkv, D] of out_dtype (bf16, f16 or f32), round_out(code *
  * scale).  cache_dtype: the elements of a PSQ_CODES_NONE cache.  A slot that is negative or past the
  * pool reads as zeros. */
