@@ -64,6 +64,10 @@ SIGNATURES = {
     "psq_paged_attention_own_workspace": (_I, [_I, _I64, _I, _I, _I, _I64]),
     "psq_paged_attention": (_I, [_I, _P, _I, _I64, _I64, _P, _P, _P, _P, _I64, _I, _P, _I64, _I64, _P, _I64, _I, _I, _I, _F,
                                  _I64, _I64, _P, _P, _P, _I64, _P]),
+    "psq_paged_prompt_attention": (_I, [_I, _P, _I, _I64, _I64, _P, _P, _P, _P, _I64, _I, _P, _I64, _I64, _P, _P, _I64, _I64, _I, _I, _I,
+                                        _F, _I64, _I64, _I64, _P, _P, _P, _I64, _P]),
+    "psq_paged_tree_attention": (_I, [_I, _P, _I, _I64, _I64, _P, _P, _P, _P, _I64, _I, _P, _I64, _I64, _P, _P, _P, _I64, _I, _I, _I, _I,
+                                      _F, _I64, _I64, _I64, _P, _P, _P, _I64, _P]),
     "psq_flag_nonfinite": (_I, [_P, _I, _I64, _P, ctypes.c_uint64, _P]),
 }
 

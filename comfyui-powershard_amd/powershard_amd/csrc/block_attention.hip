@@ -1,0 +1,102 @@
+// block_attention.hip -- the entry points of the attention of prompts and of trees of drafts over the paged
+// cache (the kernel is in block_attention.hpp): checks of arguments, and the launch.
+#include "block_attention.hpp"
+
+namespace psq {
+namespace block {
+namespace {
+
+// Fills in and checks everything but the rows' own arguments; a.T, a.N and a.B are set.
+int check(const char *name, Args &a, int codes, const void *q, int dtype, int64_t q_token, int64_t q_head, const void *k_cache,
+          const void *v_cache, const float *k_scale, const float *v_scale, int64_t num_pages, int page_size, const int32_t *block_table,
+          int64_t table_stride, int64_t table_cols, const int32_t *lengths, int64_t B, int64_t T, int Hq, int Hkv, int D, float scale,
+          int64_t window, int64_t sinks, int64_t max_len, void *out, float *lse, const void *workspace, int64_t workspace_bytes)
+{
+    if (B < 0 || T < 0 || Hq < 0 || table_cols < 0 || window < 0 || sinks < 0 || max_len < 0 || workspace_bytes < 0)
+        return set_error(PSQ_E_ARG, "%s: negative size", name);
+    if (dtype != PSQ_BF16 && dtype != PSQ_F16) return set_error(PSQ_E_ARG, "%s: queries must be bf16 or f16 (dtype %d)", name, dtype);
+    if (sinks && !window) return set_error(PSQ_E_ARG, "%s: sinks are of a window", name);
+    if (int e = check_kv_cache(name, codes, k_cache, v_cache, k_scale, v_scale, num_pages, page_size, Hkv, D)) return e;
+    if (T == 0 || Hq == 0) return PSQ_OK;
+    if (!q || !out || (B && !lengths) || (B && table_cols && !block_table)) return set_error(PSQ_E_ARG, "%s: null pointer", name);
+    if (Hq % Hkv || Hq > 65535) return set_error(PSQ_E_SHAPE, "%s: %d heads do not share %d kv heads", name, Hq, Hkv);
+    if (((uintptr_t)q | (uintptr_t)out) & 15 || (q_token | q_head) & 7)
+        return set_error(PSQ_E_SHAPE, "%s: queries and output must be 16-byte aligned, query strides multiples of 8", name);
+    if (((uintptr_t)block_table | (uintptr_t)lengths | (uintptr_t)lse) & 3)
+        return set_error(PSQ_E_SHAPE, "%s: misaligned table, lengths or lse", name);
+    if (B > 65535 || table_cols > 0x3fffffffLL / page_size)
+        return set_error(PSQ_E_SHAPE, "%s: %lld sequences of %lld pages are too many", name, (long long)B, (long long)table_cols);
+    // (a rows' number, and that of a workgroup, in 31 bits)
+    if (T > 0x3fffffffLL / Hq) return set_error(PSQ_E_SHAPE, "%s: %lld tokens of %d heads are too many", name, (long long)T, Hq);
+    if ((uintptr_t)workspace & 255) return set_error(PSQ_E_SHAPE, "%s: the workspace must be 256-byte aligned", name);
+    a.q = (const uint16_t *)q, a.q_token = q_token, a.q_head = q_head;
+    a.kc = (const uint8_t *)k_cache, a.vc = (const uint8_t *)v_cache, a.ks = k_scale, a.vs = v_scale;
+    a.table = block_table, a.table_stride = table_stride, a.lengths = lengths;
+    a.out = (uint16_t *)out, a.lse = lse;
+    a.num_pages = (int)num_pages, a.cols = (int)table_cols, a.B = (int)B, a.T = (int)T, a.page = page_size;
+    a.Hq = Hq, a.Hkv = Hkv, a.D = D, a.G = Hq / Hkv;
+    const int64_t far = 0x3fffffff;    // past any length
+    a.window = (int)std::min(window, far), a.sinks = (int)std::min(sinks, far);
+    a.flip = scale < 0 ? 0x8000 : 0, a.mute = scale == 0;
+    a.scale = a.mute ? 1.0f : fabsf(scale) * kLog2e;
+    return 1;
+}
+
+int run(int codes, int dtype, const Args &a, int64_t groups, hipStream_t st)
+{
+    if (int e = require_device()) return e;
+    const unsigned g = (unsigned)groups;
+    if (codes == PSQ_CODES_I8) return dtype == PSQ_BF16 ? launch_bf16_i8(a, g, st) : launch_f16_i8(a, g, st);
+    if (codes == PSQ_CODES_E4M3) return dtype == PSQ_BF16 ? launch_bf16_fp8(a, g, st) : launch_f16_fp8(a, g, st);
+    return dtype == PSQ_BF16 ? launch_bf16(a, g, st) : launch_f16(a, g, st);
+}
+
+}  // namespace
+}  // namespace block
+}  // namespace psq
+
+extern "C" {
+
+int psq_paged_prompt_attention(int codes, const void *q, int dtype, int64_t q_token, int64_t q_head, const void *k_cache,
+                               const void *v_cache, const float *k_scale, const float *v_scale, int64_t num_pages, int page_size,
+                               const int32_t *block_table, int64_t table_stride, int64_t table_cols, const int32_t *starts,
+                               const int32_t *lengths, int64_t B, int64_t T, int Hq, int Hkv, int D, float scale, int64_t window,
+                               int64_t sinks, int64_t max_len, void *out, float *lse, void *workspace, int64_t workspace_bytes, void *stream)
+{
+    using namespace psq;
+    using namespace psq::block;
+    const char *name = "paged_prompt_attention";
+    Args a{};
+    const int e = check(name, a, codes, q, dtype, q_token, q_head, k_cache, v_cache, k_scale, v_scale, num_pages, page_size, block_table,
+                        table_stride, table_cols, lengths, B, T, Hq, Hkv, D, scale, window, sinks, max_len, out, lse, workspace, workspace_bytes);
+    if (e <= 0) return e;
+    if (!starts) return set_error(PSQ_E_ARG, "%s: null pointer", name);
+    if ((uintptr_t)starts & 3) return set_error(PSQ_E_SHAPE, "%s: misaligned starts", name);
+    a.starts = starts;
+    return run(codes, dtype, a, Hkv * ((T * a.G) / kRows + B + 1), (hipStream_t)stream);
+}
+
+int psq_paged_tree_attention(int codes, const void *q, int dtype, int64_t q_token, int64_t q_head, const void *k_cache,
+                             const void *v_cache, const float *k_scale, const float *v_scale, int64_t num_pages, int page_size,
+                             const int32_t *block_table, int64_t table_stride, int64_t table_cols, const int32_t *lengths,
+                             const int32_t *parents, const int32_t *drafts, int64_t B, int N, int Hq, int Hkv, int D, float scale,
+                             int64_t window, int64_t sinks, int64_t max_len, void *out, float *lse, void *workspace, int64_t workspace_bytes,
+                             void *stream)
+{
+    using namespace psq;
+    using namespace psq::block;
+    const char *name = "paged_tree_attention";
+    if (N < 0) return set_error(PSQ_E_ARG, "%s: negative size", name);
+    if (N > 64) return set_error(PSQ_E_SHAPE, "%s: %d drafts, at most 64", name, N);
+    Args a{};
+    const int e = check(name, a, codes, q, dtype, q_token, q_head, k_cache, v_cache, k_scale, v_scale, num_pages, page_size, block_table,
+                        table_stride, table_cols, lengths, B, B < 0 ? -1 : B * N, Hq, Hkv, D, scale, window, sinks, max_len, out, lse, workspace,
+                        workspace_bytes);
+    if (e <= 0) return e;
+    if (!parents) return set_error(PSQ_E_ARG, "%s: null pointer", name);
+    if (((uintptr_t)parents | (uintptr_t)drafts) & 3) return set_error(PSQ_E_SHAPE, "%s: misaligned parents or drafts", name);
+    a.N = N, a.parents = parents, a.drafts = drafts;
+    return run(codes, dtype, a, Hkv * B * ((N * a.G + kRows - 1) / kRows), (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,4 @@
+// block_attention_bf16.hip -- the kernels of block_attention.hpp for bf16 rows on 16-bit caches.
+#include "block_attention.hpp"
+
+int psq::block::launch_bf16(const Args &a, unsigned groups, hipStream_t st) { return launch_dim<PSQ_BF16, PSQ_CODES_NONE>(a, groups, st); }

@@ -80,46 +80,6 @@ struct AttnArgs {
     float per_unit;        // 1 / the unit that probabilities are held in
 };
 
-// Two fp32 values whose low 16 bits are zero as a packed bf16 pair.
-__device__ __forceinline__ uint32_t pack_exact_bf16(float lo, float hi)
-{
-    return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
-}
-
-template <int B>
-__device__ __forceinline__ float i8_byte_f32(uint32_t w)
-{
-    float f;
-    if constexpr (B == 0)
-        asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(f) : "v"(w));
-    else if constexpr (B == 1)
-        asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(f) : "v"(w));
-    else if constexpr (B == 2)
-        asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(f) : "v"(w));
-    else
-        asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(f) : "v"(w));
-    return f;
-}
-
-// Bytes 2 H and 2 H + 1 of w, codes, as a packed pair of DT.
-template <int DT, int CODES, int H>
-__device__ __forceinline__ uint32_t code_pair(uint32_t w)
-{
-    if constexpr (CODES == PSQ_CODES_E4M3) {
-        if constexpr (DT == PSQ_BF16)
-            return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.0f, H != 0));
-        else
-            return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, H != 0));
-    } else if constexpr (DT == PSQ_BF16) {
-        return pack_exact_bf16(i8_byte_f32<2 * H>(w), i8_byte_f32<2 * H + 1>(w));
-    } else {
-        // the biased byte under the f16 exponent of 1024 is 1152 + q (integers to 2048 are exact)
-        const uint32_t h = __builtin_amdgcn_perm(0x64646464u, w ^ 0x80808080u, H ? 0x04030402u : 0x04010400u);
-        const f16x2_t q = __builtin_bit_cast(f16x2_t, h) - f16x2_t{(_Float16)1152.0f, (_Float16)1152.0f};
-        return __builtin_bit_cast(uint32_t, q);
-    }
-}
-
 template <int DT>
 __device__ __forceinline__ v4f mfma(const v4i &a, const v4i &b, const v4f &c)
 {

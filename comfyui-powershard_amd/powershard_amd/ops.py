@@ -808,6 +808,96 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, k_scale=None, v_s
     return (out, lse) if return_lse else out
 
 
+def _rows_on_cache(name, q, rows, k_cache, v_cache, block_table, lengths, k_scale, v_scale, window, sinks, *others):
+    """Checked arguments that the attention of prompts and of trees have in common; rows: q's dims in front of [heads, dim]."""
+    index = q.get_device()
+    code, (pages, Hk, page, D), ks, vs = _pools(name, index, k_cache, v_cache, k_scale, v_scale)
+    for t in (block_table, lengths) + others:
+        if t.get_device() != index:
+            _elsewhere(name, q, t)
+    dt = _HALF.get(q.dtype)
+    if dt is None or (not code and k_cache.dtype is not q.dtype):
+        raise TypeError(f"{name}: {q.dtype} queries do not fit a {k_cache.dtype} cache")
+    if q.dim() != rows + 2 or q.shape[-1] != D or q.shape[-2] % Hk:
+        raise ValueError(f"{name}: queries {tuple(q.shape)} must be [{'tokens' if rows == 1 else 'batch, drafts'}, a multiple of {Hk}, {D}]")
+    if lengths.dtype is not torch.int32 or lengths.dim() != 1:
+        raise ValueError(f"{name}: lengths must be int32 [batch]")
+    B = lengths.shape[0]
+    if block_table.dim() != 2 or block_table.dtype is not torch.int32 or block_table.shape[0] != B:
+        raise ValueError(f"{name}: block_table must be int32 [{B}, columns]")
+    if window is None or window < 0 or sinks is None or sinks < 0 or (sinks and not window):
+        raise ValueError(f"{name}: window and sinks must be 0 or more, sinks with a window")
+    if block_table.shape[1] > 1 and block_table.stride(1) != 1:
+        block_table = block_table.contiguous()
+    return index, code, dt, (pages, Hk, page, D), ks, vs, block_table, lengths if lengths.is_contiguous() else lengths.contiguous()
+
+
+def paged_prompt_attention(q, k_cache, v_cache, block_table, starts, lengths, k_scale=None, v_scale=None, scale=None, window=0, sinks=0,
+                           max_len=None, return_lse=False):
+    """Attention of a batch of prompts, or of parts of them, over the paged cache that holds them: [tokens, heads, dim].
+
+    q: [tokens, heads, head dim] bf16/f16; rows starts[b] .. starts[b + 1] - 1 are the newest tokens of sequence b, its
+    last ones.  starts: [batch + 1] int32 from 0, not decreasing; rows from the last one on get zeros.  lengths: [batch]
+    int32, the new tokens included.  A token sees those in front of it and itself; with a window, of these the last
+    `window` and the first `sinks` of the sequence.  The cache, scale, max_len and return_lse (lse [tokens, heads]) as
+    in paged_attention.
+    A row that sees a token whose page is outside the pool, or past the table, gets NaN.
+    """
+    name = "paged_prompt_attention"
+    index, code, dt, (pages, Hk, page, D), ks, vs, block_table, lengths = _rows_on_cache(
+        name, q, 1, k_cache, v_cache, block_table, lengths, k_scale, v_scale, window, sinks, starts)
+    (T, H, _), B, cols = q.shape, lengths.shape[0], block_table.shape[1]
+    if starts.dtype is not torch.int32 or starts.shape != (B + 1,):
+        raise ValueError(f"{name}: starts must be int32 [{B + 1}]")
+    if not starts.is_contiguous():
+        starts = starts.contiguous()
+    q, q_token, q_head = _heads(q)
+    max_len = cols * page if max_len is None or max_len < 0 else min(int(max_len), cols * page)
+    out = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((T, H), dtype=torch.float32, device=q.device) if return_lse else None
+    _call(name, _native.lib().psq_paged_prompt_attention, code, q.data_ptr(), dt, q_token, q_head, k_cache.data_ptr(), v_cache.data_ptr(),
+          ks, vs, pages, page, block_table.data_ptr(), block_table.stride(0), cols, starts.data_ptr(), lengths.data_ptr(), B, T, H, Hk, D,
+          D ** -0.5 if scale is None else scale, window, sinks, max_len, out.data_ptr(), lse.data_ptr() if return_lse else None, None, 0,
+          _raw(index))
+    return (out, lse) if return_lse else out
+
+
+def paged_tree_attention(q, k_cache, v_cache, block_table, lengths, parents, k_scale=None, v_scale=None, drafts=None, scale=None,
+                         window=0, sinks=0, max_len=None, return_lse=False):
+    """Attention of a tree of drafted tokens per sequence over the paged cache that holds them: [batch, n, heads, dim].
+
+    q: [batch, n, heads, head dim] bf16/f16, n up to 64.  The last n tokens of a sequence (of its length, lengths[b]) are its
+    drafts, draft i at place lengths[b] - n + i of the cache; drafts: [batch] int32, how many of the n there are
+    (in place of n; rows past them get zeros).  parents: [batch, n] int32: the draft that each one goes on from, an
+    earlier one, or -1 (every other value means that too): the text in front.  A draft sees that text, the drafts on its
+    way from there and itself.  Its position is the text's length plus the number of drafts in front of it on its way;
+    window and sinks count positions.  The rest as in paged_prompt_attention (lse [batch, n, heads]).
+    """
+    name = "paged_tree_attention"
+    index, code, dt, (pages, Hk, page, D), ks, vs, block_table, lengths = _rows_on_cache(
+        name, q, 2, k_cache, v_cache, block_table, lengths, k_scale, v_scale, window, sinks, parents, *(() if drafts is None else (drafts,)))
+    (B, N, H, _), cols = q.shape, block_table.shape[1]
+    if lengths.shape[0] != B or parents.dtype is not torch.int32 or parents.shape != (B, N):
+        raise ValueError(f"{name}: lengths and parents must be int32 [{B}] and [{B}, {N}]")
+    if N > 64:
+        raise ValueError(f"{name}: {N} drafts, at most 64")
+    if drafts is not None and (drafts.dtype is not torch.int32 or drafts.shape != (B,)):
+        raise ValueError(f"{name}: drafts must be int32 [{B}]")
+    if not parents.is_contiguous():
+        parents = parents.contiguous()
+    if drafts is not None and not drafts.is_contiguous():
+        drafts = drafts.contiguous()
+    q, q_token, q_head = _heads(q.reshape(B * N, H, D))
+    max_len = cols * page if max_len is None or max_len < 0 else min(int(max_len), cols * page)
+    out = torch.empty((B, N, H, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, N, H), dtype=torch.float32, device=q.device) if return_lse else None
+    _call(name, _native.lib().psq_paged_tree_attention, code, q.data_ptr(), dt, q_token, q_head, k_cache.data_ptr(), v_cache.data_ptr(),
+          ks, vs, pages, page, block_table.data_ptr(), block_table.stride(0), cols, lengths.data_ptr(), parents.data_ptr(),
+          None if drafts is None else drafts.data_ptr(), B, N, H, Hk, D, D ** -0.5 if scale is None else scale, window, sinks, max_len,
+          out.data_ptr(), lse.data_ptr() if return_lse else None, None, 0, _raw(index))
+    return (out, lse) if return_lse else out
+
+
 # ------------------------------------------------------------------ checks
 # Non-finite flags, one per (device, stream), with the last ticket handed out: a call raises the
 # flag to its ticket when it finds a NaN or Inf, and the flag is never cleared.

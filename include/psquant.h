@@ -389,6 +389,39 @@ PSQ_API int psq_paged_attention(int codes, const void *q, int dtype, int64_t q_b
                         int64_t max_len, void *out, float *lse, void *workspace, int64_t workspace_bytes,
                         void *stream);
 
+/* Attention of new tokens of a batch of sequences, prompts or parts of them, over the cache that holds them:
+ *   rows starts[b] .. starts[b + 1] - 1 of q are the newest tokens of sequence b, its last ones; the token at position
+ *   p sees the tokens t <= p, with a window those with t > p - window or t < sinks
+ * Products, scales and statistics as in psq_paged_attention; a probability enters the second product as one
+ * 16-bit number (the sum of two for f16 rows on codes).
+ *   q [T, Hq, D] bf16/f16 (element strides of tokens and heads), out [T, Hq, D] dense; lse NULL or [T, Hq]
+ *   starts [B + 1] int32, not decreasing, from 0; rows from starts[B] on: zeros, lse -inf
+ *   lengths [B] int32: each sequence's tokens, the new ones included (shorter than its rows: the rows in front
+ *   of position 0 get zeros, lse -inf)
+ * A row that sees a token whose page is outside the pool, or past its table, gets NaN.  A value that is not finite
+ * reaches only the rows that see it.
+ * max_len: about the longest length, for the number of workgroups (any value gives right results).
+ * workspace: NULL. */
+PSQ_API int psq_paged_prompt_attention(int codes, const void *q, int dtype, int64_t q_token, int64_t q_head,
+                               const void *k_cache, const void *v_cache, const float *k_scale, const float *v_scale,
+                               int64_t num_pages, int page_size, const int32_t *block_table, int64_t table_stride,
+                               int64_t table_cols, const int32_t *starts, const int32_t *lengths, int64_t B, int64_t T,
+                               int Hq, int Hkv, int D, float scale, int64_t window, int64_t sinks, int64_t max_len,
+                               void *out, float *lse, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Attention of a tree of drafted tokens per sequence over the cache that holds them: q [B N, Hq, D], rows b N .. are the
+ * drafts of sequence b, its last tokens (draft i in place lengths[b] - drafts[b] + i).  Draft i goes on from draft
+ * parents[b][i] < i, or from the text (-1; so does every other value).  It sees the text in front of the drafts, the drafts on its way and
+ * itself; its position is the text's length plus its depth, and a window and sinks count positions.
+ *   parents [B, N] int32 dense, N <= 64; drafts NULL (N each) or [B] int32, at most N: rows past them get zeros, lse
+ *   -inf, as do all rows of an empty sequence.  The rest as in psq_paged_prompt_attention. */
+PSQ_API int psq_paged_tree_attention(int codes, const void *q, int dtype, int64_t q_token, int64_t q_head,
+                             const void *k_cache, const void *v_cache, const float *k_scale, const float *v_scale,
+                             int64_t num_pages, int page_size, const int32_t *block_table, int64_t table_stride,
+                             int64_t table_cols, const int32_t *lengths, const int32_t *parents, const int32_t *drafts,
+                             int64_t B, int N, int Hq, int Hkv, int D, float scale, int64_t window, int64_t sinks,
+                             int64_t max_len, void *out, float *lse, void *workspace, int64_t workspace_bytes, void *stream);
+
 /* ---------------------------------------------------------------- checks */
 
 /* Raises *flag (a device word) to max(*flag, ticket) when any of the n elements of x (bf16 / f16
