@@ -64,6 +64,9 @@ SIGNATURES = {
     "psq_paged_attention_own_workspace": (_I, [_I, _I64, _I, _I, _I, _I64]),
     "psq_paged_attention": (_I, [_I, _P, _I, _I64, _I64, _P, _P, _P, _P, _I64, _I, _P, _I64, _I64, _P, _I64, _I, _I, _I, _F,
                                  _I64, _I64, _P, _P, _P, _I64, _P]),
+    "psq_paged_attention_sinks": (_I, [_I, _P, _I, _I64, _I64, _P, _P, _P, _P, _I64, _I, _P, _I64, _I64, _P, _I64, _I, _I, _I, _F,
+                                       _I64, _I64, _I64, _P, _P, _P, _I64, _P]),
+    "psq_paged_block_workspace_bytes": (_I64, [_I64, _I64, _I, _I, _I, _I, _I64, _I64, _I64]),
     "psq_paged_prompt_attention": (_I, [_I, _P, _I, _I64, _I64, _P, _P, _P, _P, _I64, _I, _P, _I64, _I64, _P, _P, _I64, _I64, _I, _I, _I,
                                         _F, _I64, _I64, _I64, _P, _P, _P, _I64, _P]),
     "psq_paged_tree_attention": (_I, [_I, _P, _I, _I64, _I64, _P, _P, _P, _P, _I64, _I, _P, _I64, _I64, _P, _P, _P, _I64, _I, _I, _I, _I,
@@ -72,7 +75,7 @@ SIGNATURES = {
 }
 
 DIRECT_CALLS = ("psq_add_rms_norm", "psq_kv_write", "psq_kv_read", "psq_paged_attention_workspace_bytes",
-                "psq_paged_attention_own_workspace", "psq_paged_attention")
+                "psq_paged_attention_own_workspace", "psq_paged_attention_sinks")
 
 
 class NativeLibraryError(ImportError):

@@ -17,6 +17,11 @@
 // A probability enters the second product as one 16-bit number (off by half a step, as the output is), with f16
 // rows on codes, whose values are bf16, as the sum of two.
 //
+// Many tiles of rows: a workgroup each, those with most keys first.  Few: the key tiles of all units (sequence, kv
+// head, tile of rows), in their order, are cut into equal runs, one per workgroup, as many as the chip holds: the
+// host needs no lengths.  A workgroup leaves its parts of cut units (two at most) in the workspace, and a second
+// kernel adds them up in their order.
+//
 // Tiles that all rows of a wave see whole take no masks.  In the others a masked score is -inf whatever its key
 // holds.  A masked value would still poison a row if it were infinite or NaN (0 * inf): sums that come out NaN are
 // worked out once more, carefully, with the values that are not finite taken out of the product and counted for
@@ -50,6 +55,9 @@ struct Args {
     const int32_t *lengths, *starts, *parents, *drafts;
     uint16_t *out;
     float *lse;
+    float *part;           // two per run: of the unit that it goes on with, of the one that it leaves
+    int runs;              // 0: units stay whole
+    int least;             // key tiles of a run, at least
     int num_pages, cols, B, T, N, page, Hq, Hkv, D, G;   // T: tokens of q; N: drafts per sequence (0: prompts)
     int window, sinks;
     int flip;              // of the queries' sign bits (0x8000: negative scale)
@@ -178,6 +186,37 @@ struct Layout {
     static __device__ __forceinline__ int vx(int r) { return DD == 64 ? (r >> 1 & 1) << 2 : (r & 3) << 2; }
 };
 
+// A part: sums of 4 dims of a row, [dims / 4][rows], then the rows' maxima (log2) and sums of weights (-1: sees nothing).
+template <int DD>
+constexpr int part_floats() { return kRows * (DD + 2); }
+
+// Runs: the key tiles of all units laid end to end, a sequence's units (kv head, tile of rows) with as many each.
+struct Runs {
+    uint32_t all, runs;
+    __device__ __forceinline__ uint32_t first(uint32_t w) const { return (uint32_t)uniform64((uint64_t)w * all / runs); }
+    __device__ __forceinline__ uint32_t owner(uint32_t x) const { return (uint32_t)uniform64((((uint64_t)x + 1) * runs - 1) / all); }
+    static __device__ __forceinline__ uint64_t uniform64(uint64_t x)
+    {
+        return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
+    }
+};
+
+__device__ __forceinline__ int key_tiles(const Args &a, const Seq &s) { return max(keys_of(a, s, 0, s.n * a.G - 1).count(), 1); }
+
+__device__ __forceinline__ uint32_t weight_of(const Args &a, int b)
+{
+    const Seq s = sequence(a, b);
+    return s.n ? (uint32_t)row_tiles(a, s) * a.Hkv * key_tiles(a, s) : 0;
+}
+
+__device__ __forceinline__ Runs runs_of(const Args &a, int count)
+{
+    Runs r;
+    r.all = sum_of(count, [&](int b) { return weight_of(a, b); });
+    r.runs = min((uint32_t)a.runs, max(r.all / (uint32_t)a.least, 1u));
+    return r;
+}
+
 enum { WHOLE, EDGE, CAREFUL };
 
 template <int DT, int CODES, int DD, bool PART>
@@ -196,19 +235,53 @@ block_attention_kernel(Args a)
     const int n = lane & 31, h = lane >> 5;
     const int D = PART ? a.D : DD, per_page = a.page / kGroup;
 
-    // ---- the workgroup's tile of rows
+    // ---- the workgroup's units
     const int count = a.N ? a.B : a.B + 1;
-    auto tiles_of = [&](int b) { return (uint32_t)row_tiles(a, sequence(a, b)); };
-    const uint32_t all = sum_of(count, tiles_of), units = all * a.Hkv;
-    if (blockIdx.x >= units) return;
-    // Workgroups of an XCD share a kv head's keys and values in its L2; the rows that see most go first.
-    const uint32_t rank = (uint32_t)xcd_rank(blockIdx.x, units), hk = rank / all;
-    uint32_t before;
-    const uint32_t place = all - 1 - (rank - hk * all);
-    const int b = __builtin_amdgcn_readfirstlane(find(count, place, before, tiles_of));
+    int b, r0, first = 0, tiles = 0;       // key tiles first .. of the unit's list are the workgroup's
+    uint32_t hk, x = 0, end = 0;
+    Runs runs{};
+    if (!a.runs) {
+        auto tiles_of = [&](int b) { return (uint32_t)row_tiles(a, sequence(a, b)); };
+        const uint32_t all = sum_of(count, tiles_of), units = all * a.Hkv;
+        if (blockIdx.x >= units) return;
+        // Workgroups of an XCD share a kv head's keys and values in its L2; the rows that see most go first.
+        const uint32_t rank = (uint32_t)xcd_rank(blockIdx.x, units);
+        hk = rank / all;
+        uint32_t before;
+        const uint32_t place = all - 1 - (rank - hk * all);
+        b = __builtin_amdgcn_readfirstlane(find(count, place, before, tiles_of));
+        r0 = (int)(place - before) * kRows;
+    } else {
+        runs = runs_of(a, count);
+        const uint32_t w = (uint32_t)xcd_rank(blockIdx.x, a.runs);
+        if (w >= runs.runs) return;
+        x = runs.first(w), end = runs.first(w + 1);
+    }
+
+    do {
+    bool whole = true;
+    if (a.runs) {
+        uint32_t before;
+        b = __builtin_amdgcn_readfirstlane(find(count, x, before, [&](int b) { return weight_of(a, b); }));
+        const Seq s = sequence(a, b);
+        const uint32_t each = (uint32_t)key_tiles(a, s), per = (uint32_t)row_tiles(a, s), unit = (x - before) / each;
+        hk = unit / per, r0 = (int)(unit - hk * per) * kRows;
+        first = (int)(x - before - unit * each);
+        tiles = (int)min(each - first, end - x);
+        whole = tiles == (int)each;
+        x += tiles;
+    }
     const Seq s = sequence(a, b);
-    const int r0 = (int)(place - before) * kRows, rows = min(s.n * a.G - r0, kRows);
-    const Keys keys = keys_of(a, s, r0, r0 + rows - 1);
+    const int rows = min(s.n * a.G - r0, kRows);
+    const Keys keys = a.runs ? keys_of(a, s, 0, s.n * a.G - 1) : keys_of(a, s, r0, r0 + rows - 1);
+    const Keys own = keys_of(a, s, r0, r0 + rows - 1);
+    const int last = min(first + (a.runs ? tiles : keys.count()), keys.count());
+    // the next tile of the list from i on that these rows need
+    auto next_of = [&](int i) {
+        const int t = i < last ? keys.tile(i) : own.hi;
+        if (t >= own.hi) return last;
+        return t >= own.lo || t * kKeys < a.sinks ? i : min(i + own.lo - t, last);
+    };
 
     // ---- the lane's row
     const int wrow = r0 + 32 * wave, row = wrow + n, mine = min(max(rows - 32 * wave, 0), 32);
@@ -270,7 +343,7 @@ block_attention_kernel(Args a)
     int base = 0;
     auto look = [&](int i) {
         base = i;
-        const int j = i + (lane >> 2), t = j < keys.count() ? keys.tile(j) * kKeys + kGroup * (lane & 3) : s.len;
+        const int j = i + (lane >> 2), t = j < last ? keys.tile(j) * kKeys + kGroup * (lane & 3) : s.len;
         bool in = t < s.len, out = false;
         grp = 0;
         if (in) {
@@ -494,24 +567,25 @@ block_attention_kernel(Args a)
 #pragma unroll
             for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
         run_m = -INFINITY, run_l = 0.0f;
-        const int last = keys.count();
         uint8_t *buf = smem, *other = smem + L::BUFFER;
         uint32_t astray = 0;
         __syncthreads();                       // LDS is free
-        if (last > 0) {
-            look(0);
-            stage(0, buf);
+        int i = next_of(first);
+        if (i < last) {
+            look(i);
+            stage(i, buf);
             astray = (uint32_t)wild & 15;
             deliver(buf);
         }
-        for (int i = 0; i < last; i++) {
+        while (i < last) {
+            const int j = next_of(i + 1);
             wait_vmcnt<0>();
             stage_barrier();                   // the tile is here, and the one before it is done with
             uint32_t next = 0;
-            if (i + 1 < last) {
-                if (i + 1 - base >= kLook) look(i + 1);
-                stage(i + 1, other);
-                next = (uint32_t)(wild >> (4 * (i + 1 - base))) & 15;
+            if (j < last) {
+                if (j - base >= kLook) look(j);
+                stage(j, other);
+                next = (uint32_t)(wild >> (4 * (j - base))) & 15;
             }
             const int t0 = keys.tile(i) * kKeys, t1 = t0 + kKeys - 1;
             if (mine > 0 && t0 <= any_hi && (t1 >= any_lo || t0 < a.sinks)) {
@@ -519,8 +593,8 @@ block_attention_kernel(Args a)
                 else if (t1 <= full_hi && (t0 >= full_lo || t1 < a.sinks) && !astray) compute(std::integral_constant<int, WHOLE>{}, t0, 0, buf);
                 else compute(std::integral_constant<int, EDGE>{}, t0, astray, buf);
             }
-            if (i + 1 < last) deliver(other);
-            astray = next;
+            if (j < last) deliver(other);
+            astray = next, i = j;
             std::swap(buf, other);
         }
         if (careful) break;
@@ -534,21 +608,91 @@ block_attention_kernel(Args a)
         careful = true;
     }
 
-    // ---- the rows' outputs
+    // ---- the rows' outputs, or the part of them
     run_l = half_sum(run_l);
-    if (!valid) return;
+    const float top = run_m * a.scale - (PVT == PSQ_F16 ? kF16Unit : 0);     // (in log2, the weights' unit taken off)
     const int64_t at = (int64_t)(s.first + token) * a.Hq + head;
-    const float r = pos < 0 ? 0.0f : 1.0f / run_l;    // (sees nothing: zeros)
+    if (valid && whole) {
+        const float r = pos < 0 ? 0.0f : 1.0f / run_l;    // (sees nothing: zeros)
 #pragma unroll
-    for (int d = 0; d < ND; d++)
+        for (int d = 0; d < ND; d++)
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const int dim = 32 * d + 2 * i + 4 * h;
-            if (!PART || dim < D)
-                *(v2i *)(a.out + at * D + dim) = v2i{(int)pack_half2<DT>(o[d][i] * r, o[d][i + 1] * r), (int)pack_half2<DT>(o[d][i + 2] * r, o[d][i + 3] * r)};
+            for (int i = 0; i < 16; i += 4) {
+                const int dim = 32 * d + 2 * i + 4 * h;
+                if (!PART || dim < D)
+                    *(v2i *)(a.out + at * D + dim) = v2i{(int)pack_half2<DT>(o[d][i] * r, o[d][i + 1] * r), (int)pack_half2<DT>(o[d][i + 2] * r, o[d][i + 3] * r)};
+            }
+        if (a.lse && h == 0) a.lse[at] = pos < 0 ? -INFINITY : top * kLn2 + logf(run_l);
+    } else if (valid) {
+        float *part = a.part + (2 * (int64_t)xcd_rank(blockIdx.x, a.runs) + (first == 0)) * part_floats<DD>();
+        const int r = 32 * wave + n;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                ((v4f *)part)[(8 * d + i / 2 + h) * kRows + r] = v4f{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
+        if (h == 0) part[kRows * DD + r] = top, part[kRows * (DD + 1) + r] = pos < 0 ? -1.0f : run_l;
+    }
+    } while (x < end);
+}
+
+// Adds up the parts of a cut unit: a workgroup has 1024 / DD of its rows, a thread one row's 4 dims.
+template <int DT, int DD>
+__global__ void __launch_bounds__(kThreads)
+join_kernel(Args a)
+{
+    constexpr int kJoin = 1024 / DD, U = 8;
+    const int count = a.N ? a.B : a.B + 1;
+    auto units_of = [&](int b) { return (uint32_t)row_tiles(a, sequence(a, b)) * a.Hkv; };
+    if (blockIdx.x >= sum_of(count, units_of)) return;
+    uint32_t before;
+    const int b = __builtin_amdgcn_readfirstlane(find(count, blockIdx.x, before, units_of));
+    const Seq s = sequence(a, b);
+    const uint32_t unit = blockIdx.x - before, each = (uint32_t)key_tiles(a, s), per = (uint32_t)row_tiles(a, s), hk = unit / per;
+    const int r0 = (int)(unit - hk * per) * kRows, r = (int)blockIdx.y * kJoin + (threadIdx.x & (kJoin - 1)), quad = threadIdx.x / kJoin;
+    const Runs runs = runs_of(a, count);
+    const uint32_t x = sum_of(b, [&](int b) { return weight_of(a, b); }) + unit * each;
+    const uint32_t w0 = runs.owner(x), parts = runs.owner(x + each - 1) - w0 + 1;
+    if (parts == 1 || r0 + r >= s.n * a.G || 4 * quad >= a.D) return;
+    float M = -INFINITY, L = 0.0f;
+    v4f acc = {0, 0, 0, 0};
+    bool none = false;
+    for (uint32_t p0 = 0; p0 < parts; p0 += U) {
+        v4f y[U];
+        float m[U], l[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint32_t p = p0 + u;
+            y[u] = v4f{0, 0, 0, 0}, m[u] = -INFINITY, l[u] = 0.0f;
+            if (p < parts) {
+                const float *part = a.part + (2 * (int64_t)(w0 + p) + (p == 0)) * part_floats<DD>();
+                y[u] = ((const v4f *)part)[quad * kRows + r];
+                m[u] = part[kRows * DD + r], l[u] = part[kRows * (DD + 1) + r];
+            }
         }
-    if (a.lse && h == 0)
-        a.lse[at] = pos < 0 ? -INFINITY : (run_m * a.scale - (PVT == PSQ_F16 ? kF16Unit : 0)) * kLn2 + logf(run_l);
+        float to = M;
+#pragma unroll
+        for (int u = 0; u < U; u++) to = fmaxf(to, m[u]);
+        // (2^-126 and not less: an infinite sum stays one)
+        auto scale_to = [&](float from) { return fmaxf(__builtin_amdgcn_exp2f(from - (to == -INFINITY ? 0.0f : to)), 0x1p-126f); };
+        const float e = scale_to(M);
+        L *= e, M = to;
+#pragma unroll
+        for (int c = 0; c < 4; c++) acc[c] *= e;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const float f = scale_to(m[u]);
+            none |= l[u] < 0.0f;
+            L += l[u] * f;
+#pragma unroll
+            for (int c = 0; c < 4; c++) acc[c] += y[u][c] * f;
+        }
+    }
+    const int row = r0 + r, token = row / a.G;
+    const int64_t at = (int64_t)(s.first + token) * a.Hq + (int)hk * a.G + (row - token * a.G);
+    const float i = none ? 0.0f : 1.0f / L;
+    *(v2i *)(a.out + at * a.D + 4 * quad) = v2i{(int)pack_half2<DT>(acc[0] * i, acc[1] * i), (int)pack_half2<DT>(acc[2] * i, acc[3] * i)};
+    if (a.lse && quad == 0) a.lse[at] = none ? -INFINITY : M * kLn2 + logf(L);
 }
 
 template <int DT, int CODES, int DD, bool PART>
@@ -564,7 +708,8 @@ int launch(const Args &a, unsigned groups, hipStream_t st)
             return set_error(PSQ_E_DEVICE, "block attention: cannot raise the LDS size");
         raised[dev] = true;
     }
-    kernel<<<groups, kThreads, lds, st>>>(a);
+    kernel<<<a.runs ? a.runs : groups, kThreads, lds, st>>>(a);
+    if (a.runs) join_kernel<DT, DD><<<dim3(groups, kRows / (1024 / DD)), kThreads, 0, st>>>(a);
     return check_launch("block attention");
 }
 

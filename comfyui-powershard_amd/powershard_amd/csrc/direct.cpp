@@ -26,7 +26,7 @@ decltype(&psq_kv_write) f_write;
 decltype(&psq_kv_read) f_read;
 decltype(&psq_paged_attention_workspace_bytes) f_attend_bytes;
 decltype(&psq_paged_attention_own_workspace) f_attend_own;
-decltype(&psq_paged_attention) f_attend;
+decltype(&psq_paged_attention_sinks) f_attend;
 
 // Other threads run while memory is allocated and the kernel is launched (a full queue makes the launch wait).
 struct Unlocked {
@@ -224,14 +224,14 @@ PyObject *kv_read(PyObject *, PyObject *const *o, Py_ssize_t n)
 }
 
 // paged_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, scale (None: dim ** -0.5), window,
-//                 max_len (None: the table's), return_lse, the stream's workspace, stream) -> out or (out, lse)
+//                 max_len (None: the table's), return_lse, the stream's workspace, stream, sinks (may be left out)) -> out or (out, lse)
 // Parts that a second launch joins are in memory of the call's own.
 PyObject *attend(PyObject *, PyObject *const *o, Py_ssize_t n)
 {
     return guarded([&]() -> PyObject * {
         Arg q, table, lengths, ws;
         Pools p;
-        if (n != 13 || !f_attend || !f_attend_bytes || !f_attend_own || !take(o[0], -1, q) || !q.t) return none();
+        if ((n != 13 && n != 14) || !f_attend || !f_attend_bytes || !f_attend_own || !take(o[0], -1, q) || !q.t) return none();
         const int64_t index = q.t->get_device();
         if (!p.take_from(o + 1, index) || !take(o[5], index, table) || !table.t || !take(o[6], index, lengths) || !lengths.t || !take(o[11], index, ws))
             return none();
@@ -240,6 +240,7 @@ PyObject *attend(PyObject *, PyObject *const *o, Py_ssize_t n)
         long long max_len = o[9] == Py_None ? -1 : PyLong_AsLongLong(o[9]);
         const int want = PyObject_IsTrue(o[10]);
         void *stream = PyLong_AsVoidPtr(o[12]);
+        const long long sinks = n == 14 ? PyLong_AsLongLong(o[13]) : 0;
         if (PyErr_Occurred()) {
             PyErr_Clear();
             return none();
@@ -248,11 +249,11 @@ PyObject *attend(PyObject *, PyObject *const *o, Py_ssize_t n)
         if (dt < 0 || (!p.codes && p.k.t->scalar_type() != q.t->scalar_type()) || !rows_of_heads(*q.t) || q.t->size(2) != p.dim || p.heads <= 0 ||
             q.t->size(1) % p.heads || q.t->size(1) > 0x7fffffff || table.t->scalar_type() != at::kInt || table.t->dim() != 2 ||
             table.t->size(0) != q.t->size(0) || (table.t->size(1) > 1 && table.t->stride(1) != 1) || lengths.t->scalar_type() != at::kInt ||
-            lengths.t->dim() != 1 || lengths.t->size(0) != q.t->size(0) || !lengths.t->is_contiguous() || window < 0)
+            lengths.t->dim() != 1 || lengths.t->size(0) != q.t->size(0) || !lengths.t->is_contiguous() || window < 0 || sinks < 0 || (sinks && !window))
             return none();
         const int64_t B = q.t->size(0), H = q.t->size(1), cols = table.t->size(1);
         if (max_len < 0 || max_len > cols * p.page) max_len = cols * p.page;
-        if (window && window < max_len) max_len = window;
+        if (window && window < max_len && sinks < max_len - window) max_len = window + sinks;
         const int64_t need = f_attend_bytes(p.codes, B, (int)H, p.heads, p.dim, max_len);
         const bool own = need > 0 && f_attend_own(p.codes, B, (int)H, p.heads, p.dim, max_len);
         if (need > 0 && !own && (!ws.t || ws.t->numel() < need)) return none();
@@ -267,7 +268,7 @@ PyObject *attend(PyObject *, PyObject *const *o, Py_ssize_t n)
             if (want) lse = at::empty({B, H}, opt.dtype(at::kFloat));
             status = f_attend(p.codes, q.t->data_ptr(), dt, q.t->stride(0), q.t->stride(1), p.k.t->data_ptr(), p.v.t->data_ptr(), p.scale(p.ks),
                               p.scale(p.vs), p.pages, (int)p.page, (const int32_t *)table.t->data_ptr(), table.t->stride(0), cols,
-                              (const int32_t *)lengths.t->data_ptr(), B, (int)H, p.heads, p.dim, (float)scale, window, max_len, out.data_ptr(),
+                              (const int32_t *)lengths.t->data_ptr(), B, (int)H, p.heads, p.dim, (float)scale, window, sinks, max_len, out.data_ptr(),
                               want ? (float *)lse.data_ptr() : nullptr, need > 0 ? work->data_ptr() : nullptr, need > 0 ? work->numel() : 0,
                               stream);
         }
@@ -287,7 +288,7 @@ PyObject *bind(PyObject *, PyObject *d)
     f_read = (decltype(f_read))at("psq_kv_read");
     f_attend_bytes = (decltype(f_attend_bytes))at("psq_paged_attention_workspace_bytes");
     f_attend_own = (decltype(f_attend_own))at("psq_paged_attention_own_workspace");
-    f_attend = (decltype(f_attend))at("psq_paged_attention");
+    f_attend = (decltype(f_attend))at("psq_paged_attention_sinks");
     if (PyErr_Occurred()) return nullptr;
     Py_RETURN_NONE;
 }

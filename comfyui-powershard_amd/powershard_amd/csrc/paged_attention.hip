@@ -78,6 +78,7 @@ struct AttnArgs {
     int apart;             // parts are joined by a kernel of their own
     float scale;           // times log2(e)
     float per_unit;        // 1 / the unit that probabilities are held in
+    int sinks;
 };
 
 template <int DT>
@@ -279,7 +280,8 @@ struct Step {
     }
 };
 
-template <int DT, int CODES, int DD, bool PART>
+// SINKS: a window's sinks (a kernel of its own: 61 x 4096 int8 without a window 55.5 us with one for both, 54.7 so)
+template <int DT, int CODES, int DD, bool PART, bool SINKS>
 __global__ void __launch_bounds__(kThreads, groups_per_cu(DD, CODES != PSQ_CODES_NONE))
 paged_attention_kernel(AttnArgs a)
 {
@@ -296,14 +298,19 @@ paged_attention_kernel(AttnArgs a)
     const int D = PART ? a.D : DD, per_page = a.page / kTile, units = a.Hkv * a.tiles;   // (units of a sequence)
 
     // ---- the workgroup's run of rounds
-    auto span = [&](int b, int &len, int &lo, bool &past) {   // tokens of sequence b; its rounds
+    // With sinks tokens are counted without those between them and the window (whole groups: skip of them, from
+    // sink_end on); len and lo, the end of what the window hides, are such counts.
+    const int sink_end = (a.sinks + kTile - 1) & ~(kTile - 1);
+    auto span = [&](int b, int &len, int &lo, int &skip, bool &past) {   // tokens of sequence b; its rounds
         len = max(a.lengths[b], 0);
         past = len > a.cap;
         len = min(len, a.cap);
         lo = a.window ? max(len - a.window, 0) : 0;
-        return past ? 1 : max((len - (lo & ~(kTile - 1)) + kGrain - 1) / kGrain, 1);
+        skip = SINKS ? max((lo & ~(kTile - 1)) - sink_end, 0) : 0;
+        len -= skip, lo -= skip;
+        return past ? 1 : max((len - (SINKS ? 0 : lo & ~(kTile - 1)) + kGrain - 1) / kGrain, 1);
     };
-    int len, lo, rounds;
+    int len, lo, skip, rounds;
     bool past;
     // Each wave scans the lengths for itself where it holds them (64 sequences), else the workgroup does.
     const bool narrow = a.B <= 64;
@@ -311,7 +318,7 @@ paged_attention_kernel(AttnArgs a)
     const int mine_at = narrow ? lane : tid * each;
     uint32_t own = 0;
     for (int i = 0; i < each; i++)
-        if (mine_at + i < a.B) own += span(mine_at + i, len, lo, past);
+        if (mine_at + i < a.B) own += span(mine_at + i, len, lo, skip, past);
     uint32_t before = own;                                  // rounds up to and with this thread's
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -338,7 +345,7 @@ paged_attention_kernel(AttnArgs a)
     int b, unit, r = 0;
     if (a.alone) {
         b = w / (uint32_t)units, unit = w - b * units;
-        end = rounds = span(b, len, lo, past);
+        end = rounds = span(b, len, lo, skip, past);
     } else {
         if (w >= runs) return;
         x = first_of(w), end = first_of(w + 1);
@@ -352,7 +359,7 @@ paged_attention_kernel(AttnArgs a)
             if (here) {
                 int i = mine_at;
                 for (;; i++) {
-                    const int n = span(i, len, lo, past);
+                    const int n = span(i, len, lo, skip, past);
                     if (y < before + n) break;
                     before += n;
                 }
@@ -363,13 +370,13 @@ paged_attention_kernel(AttnArgs a)
             b = __builtin_amdgcn_readfirstlane(start_b);
             at = (uint32_t)__builtin_amdgcn_readfirstlane(start_r);
         }
-        rounds = span(b, len, lo, past);
+        rounds = span(b, len, lo, skip, past);
         const uint64_t in = x - (uint64_t)at * units;
         unit = (int)divide(in, rounds), r = (int)(in - (uint64_t)unit * rounds);
     }
     Cut cut[2] = {};       // what the run has part of: a unit that it goes on with, and one that it leaves
 
-    // ---- the segment of the run at hand: n rounds of one unit, tokens c0 .. hi - 1
+    // ---- the segment of the run at hand: n rounds of one unit, tokens c0 .. hi - 1 (so counted)
     int n, hk, ht, heads, c0, hi, steps;
     int64_t head0;
     v4i qf[NC];
@@ -381,7 +388,7 @@ paged_attention_kernel(AttnArgs a)
         bool out = false;
         grp = 0;
         if (t < hi) {
-            const uint32_t i = (uint32_t)t / kTile, col = i / (uint32_t)per_page;
+            const uint32_t i = (uint32_t)(!SINKS || t < sink_end ? t : t + skip) / kTile, col = i / (uint32_t)per_page;
             const int pg = a.table[b * a.table_stride + col];
             out = pg < 0 || pg >= a.num_pages;
             grp = out ? 0 : ((uint32_t)pg * a.Hkv + hk) * per_page + (i - col * per_page);
@@ -408,7 +415,7 @@ paged_attention_kernel(AttnArgs a)
         n = (int)min(end - x, (uint64_t)(rounds - r));
         hk = unit / a.tiles, ht = unit - hk * a.tiles, heads = min(a.G - ht * kTile, kTile);
         head0 = b * (int64_t)a.Hq + hk * a.G + ht * kTile;
-        c0 = (lo & ~(kTile - 1)) + r * kGrain, hi = past ? c0 : min(c0 + n * kGrain, len);
+        c0 = (SINKS ? 0 : lo & ~(kTile - 1)) + r * kGrain, hi = past ? c0 : min(c0 + n * kGrain, len);
         steps = c0 + kStep * wave < hi ? (hi - c0 - kStep * wave + kGrain - 1) / kGrain : 0;
         const uint16_t *q = a.q + b * a.q_batch + (int64_t)(hk * a.G + ht * kTile + m) * a.q_head;
 #pragma unroll
@@ -475,7 +482,7 @@ paged_attention_kernel(AttnArgs a)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int tok = t0 + kTile * t + 4 * g + i;
-                    if (tok < lo || tok >= hi) {
+                    if ((tok < lo && (!SINKS || tok >= a.sinks)) || tok >= hi) {
                         sc[t][i] = -INFINITY;
                         if constexpr (ES == 1) st.vs[t][i] = 0.0f;
                         if constexpr (CODES != PSQ_CODES_I8) {
@@ -604,7 +611,7 @@ paged_attention_kernel(AttnArgs a)
         r = 0;
         if (++unit == units) {
             unit = 0;
-            rounds = span(++b, len, lo, past);
+            rounds = span(++b, len, lo, skip, past);
         }
         open();
     }
@@ -706,12 +713,14 @@ Plan plan(int codes, int64_t B, int Hq, int Hkv, int D, int64_t max_len)
     return p;
 }
 
-template <int DT, int CODES, int DD, bool PART>
+template <int DT, int CODES, int DD, bool PART, bool SINKS = false>
 int launch(const AttnArgs &a, int64_t groups, hipStream_t st)
 {
+    if constexpr (!SINKS)
+        if (a.sinks) return launch<DT, CODES, DD, PART, true>(a, groups, st);
     // the waves' outputs, then (joining) 256 quads with their maxima and sums
     const int lds = std::max(kWaves * std::min(a.G, kTile) * (DD + 4), 6 * kThreads) * 4;
-    auto *kernel = paged_attention_kernel<DT, CODES, DD, PART>;
+    auto *kernel = paged_attention_kernel<DT, CODES, DD, PART, SINKS>;
     if (lds > 48 * 1024) {
         static bool raised[64] = {};
         int dev = 0;
@@ -755,16 +764,17 @@ int psq_paged_attention_own_workspace(int codes, int64_t B, int Hq, int Hkv, int
     return psq::plan(codes, B, Hq, Hkv, D, std::min<int64_t>(max_len, 0x7fffffffLL)).apart;
 }
 
-int psq_paged_attention(int codes, const void *q, int dtype, int64_t q_batch, int64_t q_head, const void *k_cache,
-                        const void *v_cache, const float *k_scale, const float *v_scale, int64_t num_pages, int page_size,
-                        const int32_t *block_table, int64_t table_stride, int64_t table_cols, const int32_t *lengths, int64_t B,
-                        int Hq, int Hkv, int D, float scale, int64_t window, int64_t max_len, void *out, float *lse,
-                        void *workspace, int64_t workspace_bytes, void *stream)
+int psq_paged_attention_sinks(int codes, const void *q, int dtype, int64_t q_batch, int64_t q_head, const void *k_cache,
+                              const void *v_cache, const float *k_scale, const float *v_scale, int64_t num_pages, int page_size,
+                              const int32_t *block_table, int64_t table_stride, int64_t table_cols, const int32_t *lengths, int64_t B,
+                              int Hq, int Hkv, int D, float scale, int64_t window, int64_t sinks, int64_t max_len, void *out,
+                              float *lse, void *workspace, int64_t workspace_bytes, void *stream)
 {
     using namespace psq;
     const char *name = "paged_attention";
-    if (B < 0 || Hq < 0 || table_cols < 0 || window < 0 || max_len < 0 || workspace_bytes < 0)
+    if (B < 0 || Hq < 0 || table_cols < 0 || window < 0 || sinks < 0 || max_len < 0 || workspace_bytes < 0)
         return set_error(PSQ_E_ARG, "%s: negative size", name);
+    if (sinks && !window) return set_error(PSQ_E_ARG, "%s: sinks are of a window", name);
     if (dtype != PSQ_BF16 && dtype != PSQ_F16) return set_error(PSQ_E_ARG, "%s: queries must be bf16 or f16 (dtype %d)", name, dtype);
     if (int e = check_kv_cache(name, codes, k_cache, v_cache, k_scale, v_scale, num_pages, page_size, Hkv, D)) return e;
     if (B == 0 || Hq == 0) return PSQ_OK;
@@ -788,7 +798,7 @@ int psq_paged_attention(int codes, const void *q, int dtype, int64_t q_batch, in
                      (uint32_t *)workspace, (Cut *)((uint8_t *)workspace + p.cuts_at), (float *)((uint8_t *)workspace + p.parts_at),
                      p.part_floats, (int)num_pages, (int)cap, (int)B, page_size, Hq, Hkv, D, Hq / Hkv, p.tiles,
                      (int)std::min<int64_t>(window, cap), alone, !alone && p.apart, scale * kLog2e,
-                     codes == PSQ_CODES_NONE && dtype == PSQ_F16 ? 1.0f / kF16Unit : 1.0f};
+                     codes == PSQ_CODES_NONE && dtype == PSQ_F16 ? 1.0f / kF16Unit : 1.0f, (int)std::min<int64_t>(sinks, cap)};
     hipStream_t st = (hipStream_t)stream;
     auto go = [&](auto dtc) {
         constexpr int DT = decltype(dtc)::value;
@@ -797,6 +807,17 @@ int psq_paged_attention(int codes, const void *q, int dtype, int64_t q_batch, in
         return launch_dim<DT, PSQ_CODES_NONE>(a, groups, st);
     };
     return dtype == PSQ_BF16 ? go(std::integral_constant<int, PSQ_BF16>{}) : go(std::integral_constant<int, PSQ_F16>{});
+}
+
+int psq_paged_attention(int codes, const void *q, int dtype, int64_t q_batch, int64_t q_head, const void *k_cache,
+                        const void *v_cache, const float *k_scale, const float *v_scale, int64_t num_pages, int page_size,
+                        const int32_t *block_table, int64_t table_stride, int64_t table_cols, const int32_t *lengths, int64_t B,
+                        int Hq, int Hkv, int D, float scale, int64_t window, int64_t max_len, void *out, float *lse,
+                        void *workspace, int64_t workspace_bytes, void *stream)
+{
+    return psq_paged_attention_sinks(codes, q, dtype, q_batch, q_head, k_cache, v_cache, k_scale, v_scale, num_pages, page_size, block_table,
+                                     table_stride, table_cols, lengths, B, Hq, Hkv, D, scale, window, 0, max_len, out, lse, workspace,
+                                     workspace_bytes, stream);
 }
 
 }  // extern "C"

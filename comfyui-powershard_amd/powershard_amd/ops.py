@@ -750,13 +750,14 @@ def kv_read(slots, k_cache, v_cache, k_scale=None, v_scale=None, out_dtype=None)
 
 
 def paged_attention(q, k_cache, v_cache, block_table, lengths, k_scale=None, v_scale=None, scale=None, window=0,
-                    max_len=None, return_lse=False):
+                    max_len=None, return_lse=False, sinks=0):
     """Attention of one new token per sequence over a paged cache: [batch, heads, head dim] of q's dtype.
 
     q: [batch, heads, head dim] bf16/f16, heads a multiple of the cache's kv heads; a 16-bit cache has q's
     dtype.  block_table: [batch, columns] int32, the page of token t in column t // page_size; lengths:
     [batch] int32, each sequence's tokens, the new one included (0: zeros).  scale: of the scores (default
-    head_dim ** -0.5); window: the last tokens that are attended to (0: all).  max_len: about the longest
+    head_dim ** -0.5); window: the last tokens that are attended to (0: all); sinks: the first tokens of a
+    sequence that a window does not hide.  max_len: about the longest
     length, for the number of workgroups (default: what the table can hold; any value gives right results).
     return_lse: also the natural log of the softmax's denominator, [batch, heads] fp32.
     A sequence that needs a page outside the pool, or more tokens than its table has, gets NaN.
@@ -765,7 +766,7 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, k_scale=None, v_s
     if index >= 0 and _timer is None and (direct := _native.direct()):
         raw = _raw(index)
         done = direct.paged_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, scale, window, max_len, return_lse,
-                                      _workspaces.get((index, raw or None)), raw)
+                                      _workspaces.get((index, raw or None)), raw, sinks)
         if done is not None:
             return done
     code, (pages, Hk, page, D), ks, vs = _pools("paged_attention", index, k_cache, v_cache, k_scale, v_scale)
@@ -784,6 +785,8 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, k_scale=None, v_s
         raise ValueError(f"paged_attention: lengths must be int32 [{B}]")
     if window is None or window < 0:
         raise ValueError("paged_attention: window must be 0 or more")
+    if sinks is None or sinks < 0 or (sinks and not window):
+        raise ValueError("paged_attention: sinks must be 0 or more, with a window")
     cols = block_table.shape[1]
     if not block_table.is_contiguous() and cols > 1 and block_table.stride(1) != 1:
         block_table = block_table.contiguous()
@@ -791,8 +794,8 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, k_scale=None, v_s
         lengths = lengths.contiguous()
     q, q_batch, q_head = _heads(q)
     max_len = cols * page if max_len is None or max_len < 0 else min(int(max_len), cols * page)
-    if window and window < max_len:
-        max_len = int(window)
+    if window and window + sinks < max_len:
+        max_len = int(window + sinks)
     lib, raw, device = _native.lib(), _raw(index), q.device
     out = torch.empty((B, H, D), dtype=dtype, device=device)
     lse = torch.empty((B, H), dtype=torch.float32, device=device) if return_lse else None
@@ -801,9 +804,9 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, k_scale=None, v_s
         ws = torch.empty(nb, dtype=torch.uint8, device=device)   # two launches: the call's own
     else:
         ws, nb = _workspace(device, raw or None, nb)
-    _call("paged_attention", lib.psq_paged_attention, code, q.data_ptr(), dt, q_batch, q_head, k_cache.data_ptr(),
+    _call("paged_attention", lib.psq_paged_attention_sinks, code, q.data_ptr(), dt, q_batch, q_head, k_cache.data_ptr(),
           v_cache.data_ptr(), ks, vs, pages, page, block_table.data_ptr(), block_table.stride(0), cols, lengths.data_ptr(), B, H,
-          Hk, D, D ** -0.5 if scale is None else scale, window, max_len, out.data_ptr(), lse.data_ptr() if return_lse else None,
+          Hk, D, D ** -0.5 if scale is None else scale, window, sinks, max_len, out.data_ptr(), lse.data_ptr() if return_lse else None,
           None if ws is None else ws.data_ptr(), nb, raw)
     return (out, lse) if return_lse else out
 
@@ -832,6 +835,12 @@ def _rows_on_cache(name, q, rows, k_cache, v_cache, block_table, lengths, k_scal
     return index, code, dt, (pages, Hk, page, D), ks, vs, block_table, lengths if lengths.is_contiguous() else lengths.contiguous()
 
 
+def _parts(rows, B, N, H, Hk, D, window, sinks, max_len, device):
+    """(memory of the call's own for the parts of split sequences, its bytes)."""
+    nb = _native.lib().psq_paged_block_workspace_bytes(rows, B, N, H, Hk, D, window, sinks, max_len)
+    return (torch.empty(nb, dtype=torch.uint8, device=device) if nb else None), nb
+
+
 def paged_prompt_attention(q, k_cache, v_cache, block_table, starts, lengths, k_scale=None, v_scale=None, scale=None, window=0, sinks=0,
                            max_len=None, return_lse=False):
     """Attention of a batch of prompts, or of parts of them, over the paged cache that holds them: [tokens, heads, dim].
@@ -855,10 +864,11 @@ def paged_prompt_attention(q, k_cache, v_cache, block_table, starts, lengths, k_
     max_len = cols * page if max_len is None or max_len < 0 else min(int(max_len), cols * page)
     out = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
     lse = torch.empty((T, H), dtype=torch.float32, device=q.device) if return_lse else None
+    ws, nb = _parts(T, B, 0, H, Hk, D, window, sinks, max_len, q.device)
     _call(name, _native.lib().psq_paged_prompt_attention, code, q.data_ptr(), dt, q_token, q_head, k_cache.data_ptr(), v_cache.data_ptr(),
           ks, vs, pages, page, block_table.data_ptr(), block_table.stride(0), cols, starts.data_ptr(), lengths.data_ptr(), B, T, H, Hk, D,
-          D ** -0.5 if scale is None else scale, window, sinks, max_len, out.data_ptr(), lse.data_ptr() if return_lse else None, None, 0,
-          _raw(index))
+          D ** -0.5 if scale is None else scale, window, sinks, max_len, out.data_ptr(), lse.data_ptr() if return_lse else None,
+          None if ws is None else ws.data_ptr(), nb, _raw(index))
     return (out, lse) if return_lse else out
 
 
@@ -891,10 +901,12 @@ def paged_tree_attention(q, k_cache, v_cache, block_table, lengths, parents, k_s
     max_len = cols * page if max_len is None or max_len < 0 else min(int(max_len), cols * page)
     out = torch.empty((B, N, H, D), dtype=q.dtype, device=q.device)
     lse = torch.empty((B, N, H), dtype=torch.float32, device=q.device) if return_lse else None
+    ws, nb = _parts(B * N, B, N, H, Hk, D, window, sinks, max_len, q.device)
     _call(name, _native.lib().psq_paged_tree_attention, code, q.data_ptr(), dt, q_token, q_head, k_cache.data_ptr(), v_cache.data_ptr(),
           ks, vs, pages, page, block_table.data_ptr(), block_table.stride(0), cols, lengths.data_ptr(), parents.data_ptr(),
           None if drafts is None else drafts.data_ptr(), B, N, H, Hk, D, D ** -0.5 if scale is None else scale, window, sinks, max_len,
-          out.data_ptr(), lse.data_ptr() if return_lse else None, None, 0, _raw(index))
+          out.data_ptr(), lse.data_ptr() if return_lse else None,
+          None if ws is None else ws.data_ptr(), nb, _raw(index))
     return (out, lse) if return_lse else out
 
 

@@ -389,6 +389,15 @@ PSQ_API int psq_paged_attention(int codes, const void *q, int dtype, int64_t q_b
                         int64_t max_len, void *out, float *lse, void *workspace, int64_t workspace_bytes,
                         void *stream);
 
+/* psq_paged_attention with sinks: of a window (it is not 0), the first `sinks` tokens of a sequence stay visible beside the
+ * last `window`.  The two queries take the most tokens that a head sees, at most window + sinks, as max_len. */
+PSQ_API int psq_paged_attention_sinks(int codes, const void *q, int dtype, int64_t q_batch, int64_t q_head, const void *k_cache,
+                              const void *v_cache, const float *k_scale, const float *v_scale, int64_t num_pages,
+                              int page_size, const int32_t *block_table, int64_t table_stride, int64_t table_cols,
+                              const int32_t *lengths, int64_t B, int Hq, int Hkv, int D, float scale, int64_t window,
+                              int64_t sinks, int64_t max_len, void *out, float *lse, void *workspace,
+                              int64_t workspace_bytes, void *stream);
+
 /* Attention of new tokens of a batch of sequences, prompts or parts of them, over the cache that holds them:
  *   rows starts[b] .. starts[b + 1] - 1 of q are the newest tokens of sequence b, its last ones; the token at position
  *   p sees the tokens t <= p, with a window those with t > p - window or t < sinks
@@ -401,7 +410,11 @@ PSQ_API int psq_paged_attention(int codes, const void *q, int dtype, int64_t q_b
  * A row that sees a token whose page is outside the pool, or past its table, gets NaN.  A value that is not finite
  * reaches only the rows that see it.
  * max_len: about the longest length, for the number of workgroups (any value gives right results).
- * workspace: NULL. */
+ * workspace: NULL (no sequence is split over its length), or memory of the call's own (any contents; the call makes two
+ * launches then, and nothing else may write to it in between) of psq_paged_block_workspace_bytes() bytes, 256-byte
+ * aligned; 0 bytes: no use for one.  N: 0 here; T: B N for trees. */
+PSQ_API int64_t psq_paged_block_workspace_bytes(int64_t T, int64_t B, int N, int Hq, int Hkv, int D, int64_t window,
+                                        int64_t sinks, int64_t max_len);
 PSQ_API int psq_paged_prompt_attention(int codes, const void *q, int dtype, int64_t q_token, int64_t q_head,
                                const void *k_cache, const void *v_cache, const float *k_scale, const float *v_scale,
                                int64_t num_pages, int page_size, const int32_t *block_table, int64_t table_stride,
