@@ -77,11 +77,33 @@ __device__ __forceinline__ v16f mfma(const v4i &a, const v4i &b, const v16f &c)
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
+// 16 bytes per lane from descriptor base + off into LDS at dst + 16 lane.  The compiler would wait for a load that
+// it knows of before the next transposed LDS read, whatever place that reads; the tile loop has its own waits.
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, lds_ptr dst, uint32_t off)
+{
+    const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)dst);
+    uint32_t m0;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0) : "s"(to), "v"(off), "s"(rs) : "memory");
+}
+
+// Order of N steps of READS LDS reads and MFMAS matrix instructions each: the reads of DEPTH steps go ahead.
+template <int N, int READS, int DEPTH, int MFMAS = 1>
+__device__ __forceinline__ void ahead()
+{
+    __builtin_amdgcn_sched_group_barrier(0x100, READS * DEPTH, 0);
+    static_for<N - DEPTH>([](auto) {
+        __builtin_amdgcn_sched_group_barrier(0x8, MFMAS, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    });
+    __builtin_amdgcn_sched_group_barrier(0x8, MFMAS * DEPTH, 0);
+}
+
 // over the two halves of the wave
 __device__ __forceinline__ float half_max(float x)
 {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    return __builtin_elementwise_maximum(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 __device__ __forceinline__ float half_sum(float x)
 {
@@ -216,8 +238,6 @@ __device__ __forceinline__ Runs runs_of(const Args &a, int count)
     r.runs = min((uint32_t)a.runs, max(r.all / (uint32_t)a.least, 1u));
     return r;
 }
-
-enum { WHOLE, EDGE, CAREFUL };
 
 template <int DT, int CODES, int DD, bool PART>
 __global__ void __launch_bounds__(kThreads, DD > 128 ? 1 : 2)
@@ -377,8 +397,8 @@ block_attention_kernel(Args a)
             uint8_t *k = buf + wave * kGroup * L::PITCH, *v = k + L::TILE;
 #pragma unroll
             for (int j = 0; j < kGroup * L::PITCH / 1024; j++) {
-                buffer_load_lds16(rk, (lds_ptr)(k + 1024 * j), koff[j], 0);
-                buffer_load_lds16(rv, (lds_ptr)(v + 1024 * j), voff[j], 0);
+                dma16(rk, (lds_ptr)(k + 1024 * j), koff[j]);
+                dma16(rv, (lds_ptr)(v + 1024 * j), voff[j]);
             }
         } else {
             // places behind the sequence hold zeros
@@ -396,6 +416,14 @@ block_attention_kernel(Args a)
             sreg = 0.0f;
             if (lane < 32 && n % kGroup < left) sreg = (lane < kGroup ? a.ks : a.vs)[g * kGroup + n % kGroup];
         }
+    };
+    // values of 16 bits where no tokens are (behind the sequence, on pages that are not there): zeros, by the wave that
+    // brings the others of the group
+    auto clear = [&](int t0, uint32_t astray, uint8_t *buf) {
+        const int left = astray >> wave & 1 ? 0 : s.len - t0 - kGroup * wave;
+        uint8_t *v = buf + L::TILE + wave * kGroup * L::PITCH;
+        for (int at = lane; at < kGroup * CH; at += 64)
+            if (at / CH >= left) *(v4i *)(v + at * 16) = v4i{0, 0, 0, 0};
     };
     auto deliver = [&](uint8_t *buf) {            // codes from registers to LDS
         if constexpr (ES == 1) {
@@ -421,8 +449,8 @@ block_attention_kernel(Args a)
     float run_m, run_l;    // the maximum that scores are taken off (in their own units); the lane's part of the sum
     const uint32_t klane = n * L::PITCH + ((h ^ L::kx(n)) << 4);
     const uint32_t vlane = (4 * h + (n & 15) / 4) * L::PITCH + ((((n >> 4) << 1 | (n & 3) >> 1) ^ L::vx((n & 15) / 4)) << 4) + (n & 1) * 8;
-    auto compute = [&](auto modec, int t0, uint32_t astray, const uint8_t *buf) {
-        constexpr int MODE = decltype(modec)::value;
+    auto compute = [&](auto carefulc, int tile0, bool edge, uint32_t astray, const uint8_t *buf) {
+        constexpr bool CAREFUL = decltype(carefulc)::value;
         v16f sc[2];
 #pragma unroll
         for (int t = 0; t < 2; t++) {
@@ -432,6 +460,7 @@ block_attention_kernel(Args a)
             for (int c = 0; c < NC; c++)
                 if (!PART || 16 * c < D) sc[t] = mfma<DT>(*(const v4i *)(buf + 32 * t * L::PITCH + (klane ^ (c << 5))), qf[c], sc[t]);
         }
+        if constexpr (!PART) ahead<2 * NC, 1, 4>();
         const float *scales = (const float *)(buf + 2 * L::TILE);
         if constexpr (ES == 1) {
 #pragma unroll
@@ -444,29 +473,37 @@ block_attention_kernel(Args a)
                 }
         }
         uint32_t seen = 0;
-        if constexpr (MODE != WHOLE) {
+        int t0 = tile0;
+        if (CAREFUL || edge) {
+            asm volatile("" : "+v"(t0));   // (a branch, not selects that all tiles pay for)
+            // key 32 t + 8 (i >> 2) + (i & 3) of the lane's against these
+            const int at = t0 + 4 * h, to = min(pos, s.text - 1) - at, from = low - at, sinks = a.sinks - at, text = s.text - at;
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const int tok = t0 + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3);
-                    const uint32_t draft = (uint32_t)(tok - s.text);
-                    const bool see = tok < s.text ? tok <= pos && (tok >= low || tok < a.sinks) : draft < 64 && (way >> (draft & 63) & 1);
+                    const int k = 32 * t + 8 * (i >> 2) + (i & 3);
+                    bool see = (k <= to) & ((k >= from) | (k < sinks));
+                    if (a.N) {
+                        const uint32_t draft = (uint32_t)(k - text);
+                        see |= (draft < 64) & ((uint32_t)(way >> (draft & 63)) & 1);
+                    }
                     if (astray >> (2 * t + (i >> 3)) & 1) sc[t][i] = NAN;    // its page is not there
                     if (!see) sc[t][i] = -INFINITY;
-                    seen |= (uint32_t)see << (16 * t + i);
+                    if (CAREFUL) seen |= (uint32_t)see << (16 * t + i);
                 }
         }
-        float top = fmaxf(sc[0][0], sc[1][0]);
+        // (NaN wins; it raises nothing, and the row's sum will be NaN)
+        float top = __builtin_elementwise_maximum(sc[0][0], sc[1][0]);
 #pragma unroll
-        for (int i = 1; i < 16; i++) top = fmaxf(top, fmaxf(sc[0][i], sc[1][i]));
+        for (int i = 1; i < 16; i++) top = __builtin_elementwise_maximum(top, __builtin_elementwise_maximum(sc[0][i], sc[1][i]));
         top = half_max(top);
         // (a maximum that comes first, or is raised from -inf, is any growth)
         const bool raise = top * a.scale > run_m * a.scale + kGrowth;
         if (__any(raise)) {
             const float next = raise ? top : run_m;    // (each row by itself: its result does not depend on the others')
             float keep = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((run_m - next) * a.scale);
-            if (MODE == CAREFUL) keep = fmaxf(keep, 0x1p-126f);   // (an infinite sum stays one)
+            if (CAREFUL) keep = fmaxf(keep, 0x1p-126f);   // (an infinite sum stays one)
             run_m = next;
             run_l *= keep;
 #pragma unroll
@@ -490,7 +527,7 @@ block_attention_kernel(Args a)
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         sc[t][i + j] *= x[j];
-                        if (MODE != WHOLE && !(seen >> (16 * t + i + j) & 1)) sc[t][i + j] = 0.0f;   // (its scale may be infinite)
+                        if (CAREFUL && !(seen >> (16 * t + i + j) & 1)) sc[t][i + j] = 0.0f;   // (its scale may be infinite)
                     }
                 }
             }
@@ -507,15 +544,6 @@ block_attention_kernel(Args a)
         const uint8_t *vb = buf + L::TILE;
 #pragma unroll
         for (int u = 0; u < 4; u++) {
-            v4i keep;      // of 16-bit values: behind the sequence lie no tokens
-            if constexpr (MODE == EDGE && ES == 2) {
-                const int left = s.len - t0 - 16 * u - 4 * h;
-#pragma unroll
-                for (int d = 0; d < 4; d++) {
-                    const int k = 8 * (d >> 1) + 2 * (d & 1);
-                    keep[d] = (k < left ? 0xffff : 0) | (k + 1 < left ? (int)0xffff0000 : 0);
-                }
-            }
 #pragma unroll
             for (int d = 0; d < ND; d++) {
                 if (PART && 32 * d >= D) break;
@@ -524,8 +552,7 @@ block_attention_kernel(Args a)
                 const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(src + 8 * L::PITCH));
                 const v2i xi = __builtin_bit_cast(v2i, x), yi = __builtin_bit_cast(v2i, y);
                 v4i vf{xi[0], xi[1], yi[0], yi[1]};
-                if constexpr (MODE == EDGE && ES == 2) vf &= keep;
-                if constexpr (MODE == CAREFUL) {
+                if constexpr (CAREFUL) {
                     constexpr uint32_t EXP = PVT == PSQ_BF16 ? 0x7f80 : 0x7c00, ONE = PVT == PSQ_BF16 ? 0x3f80 : 0x3c00;
                     v4i up, down, look;     // ones where a value is +inf, is -inf (NaN: both); where a key is seen
                     bool any = false;
@@ -535,11 +562,11 @@ block_attention_kernel(Args a)
 #pragma unroll
                         for (int k = 0; k < 2; k++) {
                             const uint32_t w = (uint32_t)vf[e] >> (16 * k) & 0xffff;
-                            const bool odd = (w & EXP) == EXP, nan = odd && (w & (EXP ^ 0x7fff));
+                            const bool odd = (w & EXP) == EXP, nan = odd & ((w & (EXP ^ 0x7fff)) != 0);
                             any |= odd;
                             c |= (odd ? 0 : w) << (16 * k);
-                            pu |= (odd && (nan || !(w & 0x8000)) ? ONE : 0) << (16 * k);
-                            pd |= (odd && (nan || (w & 0x8000)) ? ONE : 0) << (16 * k);
+                            pu |= (odd & (nan | !(w & 0x8000)) ? ONE : 0) << (16 * k);
+                            pd |= (odd & (nan | ((w & 0x8000) != 0)) ? ONE : 0) << (16 * k);
                             ps |= (seen >> (8 * u + 2 * e + k) & 1 ? ONE : 0) << (16 * k);
                         }
                         vf[e] = (int)c, up[e] = (int)pu, down[e] = (int)pd, look[e] = (int)ps;
@@ -558,55 +585,52 @@ block_attention_kernel(Args a)
                 if constexpr (PAIR) o[d] = mfma<PVT>(vf, pl[u], o[d]);
             }
         }
+        if constexpr (!PART && !CAREFUL) ahead<4 * ND, 2, 4, PAIR ? 2 : 1>();
     };
 
-    bool careful = false;
-    for (;;) {
+    // All of the workgroup's key tiles of the unit.
+    auto pass = [&](auto carefulc) {
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
             for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
         run_m = -INFINITY, run_l = 0.0f;
-        uint8_t *buf = smem, *other = smem + L::BUFFER;
+        uint32_t here = 0, next = L::BUFFER;   // offsets of the buffers
         uint32_t astray = 0;
         __syncthreads();                       // LDS is free
         int i = next_of(first);
         if (i < last) {
             look(i);
-            stage(i, buf);
+            stage(i, smem);
             astray = (uint32_t)wild & 15;
-            deliver(buf);
+            deliver(smem);
         }
         while (i < last) {
-            const int j = next_of(i + 1);
+            const int j = next_of(i + 1), t0 = keys.tile(i) * kKeys, t1 = t0 + kKeys - 1;
             wait_vmcnt<0>();
+            if (ES == 2 && (t1 >= s.len || astray)) clear(t0, astray, smem + here);
             stage_barrier();                   // the tile is here, and the one before it is done with
-            uint32_t next = 0;
+            uint32_t gone = 0;
             if (j < last) {
                 if (j - base >= kLook) look(j);
-                stage(j, other);
-                next = (uint32_t)(wild >> (4 * (j - base))) & 15;
+                stage(j, smem + next);
+                gone = (uint32_t)(wild >> (4 * (j - base))) & 15;
             }
-            const int t0 = keys.tile(i) * kKeys, t1 = t0 + kKeys - 1;
-            if (mine > 0 && t0 <= any_hi && (t1 >= any_lo || t0 < a.sinks)) {
-                if (careful) compute(std::integral_constant<int, CAREFUL>{}, t0, astray, buf);
-                else if (t1 <= full_hi && (t0 >= full_lo || t1 < a.sinks) && !astray) compute(std::integral_constant<int, WHOLE>{}, t0, 0, buf);
-                else compute(std::integral_constant<int, EDGE>{}, t0, astray, buf);
-            }
-            if (j < last) deliver(other);
-            astray = next, i = j;
-            std::swap(buf, other);
+            if (mine > 0 && t0 <= any_hi && (t1 >= any_lo || t0 < a.sinks))
+                compute(carefulc, t0, !(t1 <= full_hi && (t0 >= full_lo || t1 < a.sinks) && !astray), astray, smem + here);
+            if (j < last) deliver(smem + next);
+            astray = gone, i = j;
+            std::swap(here, next);
         }
-        if (careful) break;
-        float any = 0.0f;
+    };
+    pass(std::false_type{});
+    float any = 0.0f;
 #pragma unroll
-        for (int d = 0; d < ND; d++)
-            if (!PART || 32 * d < D)
+    for (int d = 0; d < ND; d++)
+        if (!PART || 32 * d < D)
 #pragma unroll
-                for (int i = 0; i < 16; i++) any = __builtin_fmaf(o[d][i], 0.0f, any);
-        if (!__syncthreads_or(any != any)) break;
-        careful = true;
-    }
+            for (int i = 0; i < 16; i++) any = __builtin_fmaf(o[d][i], 0.0f, any);
+    if (__syncthreads_or(any != any)) pass(std::true_type{});
 
     // ---- the rows' outputs, or the part of them
     run_l = half_sum(run_l);
