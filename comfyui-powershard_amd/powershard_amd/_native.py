@@ -66,7 +66,7 @@ SIGNATURES = {
                                  _I64, _I64, _P, _P, _P, _I64, _P]),
     "psq_paged_attention_sinks": (_I, [_I, _P, _I, _I64, _I64, _P, _P, _P, _P, _I64, _I, _P, _I64, _I64, _P, _I64, _I, _I, _I, _F,
                                        _I64, _I64, _I64, _P, _P, _P, _I64, _P]),
-    "psq_paged_block_workspace_bytes": (_I64, [_I64, _I64, _I, _I, _I, _I, _I64, _I64, _I64]),
+    "psq_paged_block_workspace_bytes": (_I64, [_I, _I64, _I64, _I, _I, _I, _I, _I64, _I64, _I64]),
     "psq_paged_prompt_attention": (_I, [_I, _P, _I, _I64, _I64, _P, _P, _P, _P, _I64, _I, _P, _I64, _I64, _P, _P, _I64, _I64, _I, _I, _I,
                                         _F, _I64, _I64, _I64, _P, _P, _P, _I64, _P]),
     "psq_paged_tree_attention": (_I, [_I, _P, _I, _I64, _I64, _P, _P, _P, _P, _I64, _I, _P, _I64, _I64, _P, _P, _P, _I64, _I, _I, _I, _I,

@@ -42,25 +42,26 @@ int check(const char *name, Args &a, int codes, const void *q, int dtype, int64_
     return 1;
 }
 
-// Units (sequence, kv head, tile of rows) that there are at most, and the runs that their key tiles are cut into (0: they
-// stay whole).
-struct Plan { int64_t units, runs, bytes; };
+// Rows of a workgroup's tile; units (sequence, kv head, tile of rows) that there are at most, and the runs that their key
+// tiles are cut into (0: they stay whole).
+struct Plan { int rows; int64_t units, runs, bytes; };
 
-Plan plan(int64_t T, int64_t B, int N, int Hq, int Hkv, int D, int64_t window, int64_t sinks, int64_t max_len)
+Plan plan(int codes, int64_t T, int64_t B, int N, int Hq, int Hkv, int D, int64_t window, int64_t sinks, int64_t max_len)
 {
     Plan p{};
-    const int64_t G = Hq / Hkv;
-    p.units = Hkv * (N ? B * ((N * G + kRows - 1) / kRows) : T * G / kRows + B + 1);
+    const int64_t G = Hq / Hkv, each = (N ? N : T / std::max<int64_t>(B, 1)) * G;     // rows of a sequence and kv head
+    p.rows = D <= 128 && (codes != PSQ_CODES_NONE || each >= 512) ? 256 : 128;
+    p.units = Hkv * (N ? B * ((N * G + p.rows - 1) / p.rows) : T * G / p.rows + B + 1);
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess) dev = 0;
-    const int64_t slots = (int64_t)cu_count(dev) * (D > 128 ? 1 : 2);
+    const int64_t slots = (int64_t)cu_count(dev) * (D > 128 || p.rows == 256 ? 1 : 2);
     // of a unit, at most: with a window those of its first row's to its last row's
     int64_t tiles = (max_len + kKeys - 1) / kKeys;
-    if (window) tiles = std::min(tiles, (window + std::min<int64_t>(sinks, max_len) + kRows / G) / kKeys + 3);
-    if (tiles <= 1 || p.units >= (tiles <= 16 ? slots / 2 : 2 * slots) || p.units * tiles > 0x7fffffffLL) return p;
+    if (window) tiles = std::min(tiles, (window + std::min<int64_t>(sinks, max_len) + p.rows / G) / kKeys + 3);
+    if (tiles <= 2 || p.units >= (tiles <= 16 ? slots / 2 : 2 * slots) || p.units * tiles > 0x7fffffffLL) return p;
     p.runs = slots;
     const int DD = D <= 64 ? 64 : D <= 128 ? 128 : 256;
-    p.bytes = 2 * p.runs * kRows * (DD + 2) * 4;
+    p.bytes = 2 * p.runs * part_floats(p.rows, DD) * 4;
     return p;
 }
 
@@ -68,6 +69,7 @@ int run(int codes, int dtype, Args &a, const Plan &p, void *workspace, int64_t w
 {
     if (int e = require_device()) return e;
     const unsigned g = (unsigned)p.units;
+    a.rows = p.rows;
     if (p.runs && workspace && workspace_bytes >= p.bytes) a.runs = (int)p.runs, a.least = 2, a.part = (float *)workspace;
     if (codes == PSQ_CODES_I8) return dtype == PSQ_BF16 ? launch_bf16_i8(a, g, st) : launch_f16_i8(a, g, st);
     if (codes == PSQ_CODES_E4M3) return dtype == PSQ_BF16 ? launch_bf16_fp8(a, g, st) : launch_f16_fp8(a, g, st);
@@ -80,12 +82,12 @@ int run(int codes, int dtype, Args &a, const Plan &p, void *workspace, int64_t w
 
 extern "C" {
 
-int64_t psq_paged_block_workspace_bytes(int64_t T, int64_t B, int N, int Hq, int Hkv, int D, int64_t window, int64_t sinks, int64_t max_len)
+int64_t psq_paged_block_workspace_bytes(int codes, int64_t T, int64_t B, int N, int Hq, int Hkv, int D, int64_t window, int64_t sinks, int64_t max_len)
 {
     if (T <= 0 || B <= 0 || N < 0 || N > 64 || Hq <= 0 || Hkv <= 0 || D <= 0 || D > 256 || window < 0 || sinks < 0 || max_len <= 0 || Hq % Hkv ||
         B > 65535 || T > 0x3fffffffLL / Hq)
         return 0;
-    return psq::block::plan(T, B, N, Hq, Hkv, D, window, sinks, std::min<int64_t>(max_len, 0x3fffffffLL)).bytes;
+    return psq::block::plan(codes, T, B, N, Hq, Hkv, D, window, sinks, std::min<int64_t>(max_len, 0x3fffffffLL)).bytes;
 }
 
 int psq_paged_prompt_attention(int codes, const void *q, int dtype, int64_t q_token, int64_t q_head, const void *k_cache,
@@ -104,7 +106,7 @@ int psq_paged_prompt_attention(int codes, const void *q, int dtype, int64_t q_to
     if (!starts) return set_error(PSQ_E_ARG, "%s: null pointer", name);
     if ((uintptr_t)starts & 3) return set_error(PSQ_E_SHAPE, "%s: misaligned starts", name);
     a.starts = starts;
-    return run(codes, dtype, a, plan(T, B, 0, Hq, Hkv, D, window, sinks, std::min(max_len, table_cols * page_size)), workspace, workspace_bytes, (hipStream_t)stream);
+    return run(codes, dtype, a, plan(codes, T, B, 0, Hq, Hkv, D, window, sinks, std::min(max_len, table_cols * page_size)), workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 int psq_paged_tree_attention(int codes, const void *q, int dtype, int64_t q_token, int64_t q_head, const void *k_cache,
@@ -127,7 +129,7 @@ int psq_paged_tree_attention(int codes, const void *q, int dtype, int64_t q_toke
     if (!parents) return set_error(PSQ_E_ARG, "%s: null pointer", name);
     if (((uintptr_t)parents | (uintptr_t)drafts) & 3) return set_error(PSQ_E_SHAPE, "%s: misaligned parents or drafts", name);
     a.N = N, a.parents = parents, a.drafts = drafts;
-    return run(codes, dtype, a, plan(0, B, N, Hq, Hkv, D, window, sinks, std::min(max_len, table_cols * page_size)), workspace, workspace_bytes, (hipStream_t)stream);
+    return run(codes, dtype, a, plan(codes, 0, B, N, Hq, Hkv, D, window, sinks, std::min(max_len, table_cols * page_size)), workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 }  // extern "C"

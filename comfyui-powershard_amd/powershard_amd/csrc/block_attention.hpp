@@ -33,17 +33,19 @@
 #include <algorithm>
 #include <math.h>
 
+#define PSQ_INLINE __attribute__((always_inline))   // lambdas over register arrays: a call would put these in memory
+
 namespace psq {
 namespace block {
 
-constexpr int kWaves = 4, kThreads = 64 * kWaves;
-constexpr int kRows = 32 * kWaves;      // of a workgroup's tile
+constexpr int kThreads = 256;           // of the joining kernel
 constexpr int kKeys = 64;               // of a key tile
 constexpr int kGroup = 16;              // tokens of a group (one page holds it)
 constexpr int kLook = 64 / (kKeys / kGroup);   // key tiles whose pages are looked up at once
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kGrowth = 8.0f;         // log2 of what a row's maximum may grow before it is raised
 constexpr int kF16Unit = 7;             // log2 of the unit of f16 probabilities
+constexpr uint32_t kPast = 0x40000000;  // an offset past every group of a pool
 
 struct Args {
     const uint16_t *q;
@@ -57,6 +59,7 @@ struct Args {
     float *lse;
     float *part;           // two per run: of the unit that it goes on with, of the one that it leaves
     int runs;              // 0: units stay whole
+    int rows;              // of a workgroup's tile, 32 a wave
     int least;             // key tiles of a run, at least
     int num_pages, cols, B, T, N, page, Hq, Hkv, D, G;   // T: tokens of q; N: drafts per sequence (0: prompts)
     int window, sinks;
@@ -66,7 +69,12 @@ struct Args {
 };
 
 typedef short v4s __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) v4s *lds_v4s;
+// T at an LDS address
+template <class T>
+__device__ __forceinline__ __attribute__((address_space(3))) T *at_lds(uint32_t at)
+{
+    return (__attribute__((address_space(3))) T *)(uintptr_t)at;
+}
 
 template <int DT>
 __device__ __forceinline__ v16f mfma(const v4i &a, const v4i &b, const v16f &c)
@@ -79,24 +87,29 @@ __device__ __forceinline__ v16f mfma(const v4i &a, const v4i &b, const v16f &c)
 
 // 16 bytes per lane from descriptor base + off into LDS at dst + 16 lane.  The compiler would wait for a load that
 // it knows of before the next transposed LDS read, whatever place that reads; the tile loop has its own waits.
-__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, lds_ptr dst, uint32_t off)
+__device__ __forceinline__ void dma16(const v4i &rs, uint32_t dst, uint32_t off)
 {
-    const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)dst);
+    const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)dst);
     uint32_t m0;
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
                  : "=&s"(m0) : "s"(to), "v"(off), "s"(rs) : "memory");
 }
 
-// Order of N steps of READS LDS reads and MFMAS matrix instructions each: the reads of DEPTH steps go ahead.
-template <int N, int READS, int DEPTH, int MFMAS = 1>
-__device__ __forceinline__ void ahead()
+// 4 bytes per lane
+__device__ __forceinline__ void dma4(const v4i &rs, uint32_t dst, uint32_t off)
 {
-    __builtin_amdgcn_sched_group_barrier(0x100, READS * DEPTH, 0);
-    static_for<N - DEPTH>([](auto) {
-        __builtin_amdgcn_sched_group_barrier(0x8, MFMAS, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
-    });
-    __builtin_amdgcn_sched_group_barrier(0x8, MFMAS * DEPTH, 0);
+    const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)dst);
+    uint32_t m0;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dword %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0) : "s"(to), "v"(off), "s"(rs) : "memory");
+}
+
+// x, in a way that what follows from it is worked out here again and not kept in registers, which are short.
+template <class T>
+__device__ __forceinline__ T again(T x)
+{
+    asm volatile("" : "+v"(x));
+    return x;
 }
 
 // over the two halves of the wave
@@ -131,7 +144,7 @@ __device__ __forceinline__ Seq sequence(const Args &a, int b)
     return s;
 }
 
-__device__ __forceinline__ int row_tiles(const Args &a, const Seq &s) { return (s.n * a.G + kRows - 1) / kRows; }
+__device__ __forceinline__ int row_tiles(const Args &a, const Seq &s) { return (s.n * a.G + a.rows - 1) / a.rows; }
 
 // The key tiles that rows r0 .. r1 of a sequence need, in a list: those of the sinks, then lo .. hi - 1.
 struct Keys {
@@ -197,11 +210,24 @@ __device__ __forceinline__ void widen(const v4i &c, v4i (&w)[2])
     }
 }
 
-// DD: head dims that tiles are laid out for; PART: D < DD, the rest of a row is not there.
-template <int DD>
+// DD: head dims that tiles are laid out for; W: waves of a workgroup; ES: bytes of a cached element.
+// Keys and values have rings of RK and RV buffers.  While a tile's weights meet its values, the next one's keys are read, and
+// loaded are the keys of the tile DK behind it and the values of that DV behind it.  A barrier comes every STEPS tiles
+// (two where the LDS holds eight buffers, for as many workgroups as the registers allow).
+// Codes (RAW) are loaded as they are, tiles up to RR behind, each by the wave that widens it later; wide heads' go
+// through registers.
+template <int DD, int W, int ES>
 struct Layout {
-    static constexpr int PITCH = 2 * DD, TILE = kKeys * PITCH;      // bytes of a row, a tile
-    static constexpr int BUFFER = 2 * TILE + 2 * kKeys * 4;         // keys, values, their scales
+    static constexpr bool RAW = ES == 1 && DD <= 128;
+    static constexpr int PITCH = 2 * DD, TILE = kKeys * PITCH;          // bytes of a row, a tile
+    static constexpr int BUFFER = TILE + (ES == 2 ? 0 : PITCH > 256 ? PITCH : 256);   // and its scales; whole rows
+    static constexpr int STEPS = ES == 2 && (DD == 64 || W == 8) ? 2 : 1;
+    static constexpr int DK = STEPS + 1, DV = STEPS == 2 ? 2 : DD == 256 || ES == 1 ? 1 : 2;
+    static constexpr int RK = STEPS == 2 ? 4 : 2, RV = STEPS == 2 ? 4 : DV + 1;
+    static constexpr int RW = kKeys / W;                                // rows of a tile that a wave brings
+    static constexpr int RR = RAW ? 5 : 0, RAW_TILE = kKeys * (2 * DD + 8);   // keys, values, their scales
+    static constexpr int RAW_AT = (RK + RV) * BUFFER, BYTES = RAW_AT + RR * RAW_TILE;
+    static constexpr int AHEAD = RAW ? RR : DK;                         // tiles that are known ahead
     // 16-byte chunk c of row r is stored at chunk c ^ kx(r) (keys), c ^ vx(r) (values): the lanes that the
     // LDS serves together then hit all banks
     static __device__ __forceinline__ int kx(int r) { return DD == 64 ? (r >> 1) & 7 : r & 15; }
@@ -209,8 +235,7 @@ struct Layout {
 };
 
 // A part: sums of 4 dims of a row, [dims / 4][rows], then the rows' maxima (log2) and sums of weights (-1: sees nothing).
-template <int DD>
-constexpr int part_floats() { return kRows * (DD + 2); }
+constexpr int64_t part_floats(int rows, int DD) { return rows * (DD + 2); }
 
 // Runs: the key tiles of all units laid end to end, a sequence's units (kv head, tile of rows) with as many each.
 struct Runs {
@@ -239,68 +264,34 @@ __device__ __forceinline__ Runs runs_of(const Args &a, int count)
     return r;
 }
 
-template <int DT, int CODES, int DD, bool PART>
-__global__ void __launch_bounds__(kThreads, DD > 128 ? 1 : 2)
-block_attention_kernel(Args a)
+// A part of a unit, or all of it: the key tiles first .. first + tiles - 1 of the sequence's list (runs), or the rows' own
+// list, for rows r0 .. of sequence b and kv head hk.  lds: the tiles' address in LDS.  True: some sum is NaN, and if not CAREFUL that may be for what masks
+// hide.
+template <int DT, int CODES, int DD, bool PART, int W, bool CAREFUL>
+__device__ __forceinline__ bool block_unit(const Args &a, uint32_t lds, int b, uint32_t hk, int r0, int first, int tiles, bool whole)
 {
-    using L = Layout<DD>;
     constexpr int ES = CODES == PSQ_CODES_NONE ? 2 : 1;
+    using L = Layout<DD, W, ES>;
     constexpr int PVT = CODES == PSQ_CODES_NONE ? DT : PSQ_BF16;   // of the second product
     constexpr bool PAIR = CODES != PSQ_CODES_NONE && DT == PSQ_F16;
     constexpr int NC = DD / 16, ND = DD / 32;
     constexpr int CH = DD / 8;                        // 16-byte chunks of a row of 16-bit elements
-    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // (the careful form works everything out for itself: what both share would stay in registers all along)
+    const int tid = CAREFUL ? again(threadIdx.x) : threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
     const int D = PART ? a.D : DD, per_page = a.page / kGroup;
 
-    // ---- the workgroup's units
-    const int count = a.N ? a.B : a.B + 1;
-    int b, r0, first = 0, tiles = 0;       // key tiles first .. of the unit's list are the workgroup's
-    uint32_t hk, x = 0, end = 0;
-    Runs runs{};
-    if (!a.runs) {
-        auto tiles_of = [&](int b) { return (uint32_t)row_tiles(a, sequence(a, b)); };
-        const uint32_t all = sum_of(count, tiles_of), units = all * a.Hkv;
-        if (blockIdx.x >= units) return;
-        // Workgroups of an XCD share a kv head's keys and values in its L2; the rows that see most go first.
-        const uint32_t rank = (uint32_t)xcd_rank(blockIdx.x, units);
-        hk = rank / all;
-        uint32_t before;
-        const uint32_t place = all - 1 - (rank - hk * all);
-        b = __builtin_amdgcn_readfirstlane(find(count, place, before, tiles_of));
-        r0 = (int)(place - before) * kRows;
-    } else {
-        runs = runs_of(a, count);
-        const uint32_t w = (uint32_t)xcd_rank(blockIdx.x, a.runs);
-        if (w >= runs.runs) return;
-        x = runs.first(w), end = runs.first(w + 1);
-    }
-
-    do {
-    bool whole = true;
-    if (a.runs) {
-        uint32_t before;
-        b = __builtin_amdgcn_readfirstlane(find(count, x, before, [&](int b) { return weight_of(a, b); }));
-        const Seq s = sequence(a, b);
-        const uint32_t each = (uint32_t)key_tiles(a, s), per = (uint32_t)row_tiles(a, s), unit = (x - before) / each;
-        hk = unit / per, r0 = (int)(unit - hk * per) * kRows;
-        first = (int)(x - before - unit * each);
-        tiles = (int)min(each - first, end - x);
-        whole = tiles == (int)each;
-        x += tiles;
-    }
     const Seq s = sequence(a, b);
-    const int rows = min(s.n * a.G - r0, kRows);
+    const int rows = min(s.n * a.G - r0, a.rows);
     const Keys keys = a.runs ? keys_of(a, s, 0, s.n * a.G - 1) : keys_of(a, s, r0, r0 + rows - 1);
     const Keys own = keys_of(a, s, r0, r0 + rows - 1);
     const int last = min(first + (a.runs ? tiles : keys.count()), keys.count());
     // the next tile of the list from i on that these rows need
-    auto next_of = [&](int i) {
-        const int t = i < last ? keys.tile(i) : own.hi;
-        if (t >= own.hi) return last;
-        return t >= own.lo || t * kKeys < a.sinks ? i : min(i + own.lo - t, last);
+    auto next_of = [&](int i) PSQ_INLINE {
+        const int t = keys.tile(i);
+        const int to = t >= own.hi ? last : t >= own.lo || t * kKeys < a.sinks ? i : i + own.lo - t;
+        return min(to, last);
     };
 
     // ---- the lane's row
@@ -339,10 +330,9 @@ block_attention_kernel(Args a)
         pos = s.len - s.n + token;
     }
     const int low = a.window ? pos - a.window + 1 : 0;
-    // of the wave: keys up to full_hi, from full_lo or among the sinks, are seen by all rows; keys past any_hi, or before
-    // any_lo and past the sinks, by none
+    // of the wave: keys up to full_hi, from full_lo or among the sinks, are seen by all rows
     const int w0 = a.N ? s.text : s.len - s.n + wrow / a.G, w1 = a.N ? s.len - 1 : s.len - s.n + (wrow + max(mine, 1) - 1) / a.G;
-    const int full_hi = a.N ? s.text - 1 : w0, full_lo = a.window ? w1 - a.window + 1 : 0, any_hi = w1, any_lo = a.window ? w0 - a.window + 1 : 0;
+    const int full_hi = a.N ? s.text - 1 : w0, full_lo = a.window ? w1 - a.window + 1 : 0;
 
     v4i qf[NC];
     {
@@ -356,12 +346,12 @@ block_attention_kernel(Args a)
         }
     }
 
-    // ---- bringing key tiles to LDS: wave w has group w of a tile's four
+    // ---- bringing key tiles to LDS
     const int row_bytes = D * ES;
     uint32_t grp;          // lane 4 i + g: pool group of tile base + i's group g
     uint64_t there, wild;  // tokens that are there; whose page is not
     int base = 0;
-    auto look = [&](int i) {
+    auto look = [&](int i) PSQ_INLINE {
         base = i;
         const int j = i + (lane >> 2), t = j < last ? keys.tile(j) * kKeys + kGroup * (lane & 3) : s.len;
         bool in = t < s.len, out = false;
@@ -375,186 +365,237 @@ block_attention_kernel(Args a)
         there = __ballot(in && !out);
         wild = __ballot(out);
     };
-    constexpr int CP = DD / 16 * kGroup / 64;     // 16-byte pieces of codes that a lane has of its wave's group
-    v4i kreg[ES == 1 ? CP : 1], vreg[ES == 1 ? CP : 1];
-    float sreg = 0.0f;
-    uint32_t koff[ES == 2 ? kGroup * L::PITCH / 1024 : 1], voff[ES == 2 ? kGroup * L::PITCH / 1024 : 1];
-    if constexpr (ES == 2) {
+    // A tile on its way: its number (-1: none), which of its groups have no page; the wave's rows of it: their group and how
+    // many hold tokens.
+    struct Tile { int number, astray, group, left; };
+    const int first_row = wave * L::RW;               // in a tile
+    int at_tile;           // the newest tile's place in the list
+    auto tile_at = [&](int i) PSQ_INLINE {
+        at_tile = i;
+        if (i - base >= kLook) look(i);
+        const int bit = 4 * (i - base) + first_row / kGroup, number = keys.tile(i);
+        const int left = min(max(s.len - (number * kKeys + first_row), 0), L::RW);
+        return Tile{i < last ? number : -1, (int)(wild >> (4 * (i - base))) & 15, __builtin_amdgcn_readlane((int)grp, bit),
+                    there >> bit & 1 ? left : 0};   // (past the last tile nothing is there)
+    };
+    auto row_of = [&](const Tile &t) PSQ_INLINE { return (int64_t)(uint32_t)t.group * kGroup + first_row % kGroup; };
+    // 16-bit elements go to LDS by themselves: descriptors of rows, past whose tokens loads give zeros, ...
+    constexpr int NL = ES == 2 ? L::RW * L::PITCH / 1024 : 0;
+    auto descriptor = [&](const uint8_t *pool, const Tile &t) PSQ_INLINE {
+        const uint64_t from = (uint64_t)(pool + row_of(t) * row_bytes);
+        return v4i{__builtin_amdgcn_readfirstlane((int)from), __builtin_amdgcn_readfirstlane((int)(from >> 32) & 0xffff),
+                   __builtin_amdgcn_readfirstlane(t.left * row_bytes), 0x00020000};
+    };
+    // ... and load j: row lane / CH + 64 j / CH of the wave's, the chunk whose place is lane % CH (dims that are not there:
+    // past every end).  Its offset for j = 0, without the row's, in bytes; x: the placement's exclusive or.
+    const uint32_t row_off = (uint32_t)(lane / CH * row_bytes);
+    const uint32_t key_off = (uint32_t)(lane % CH ^ L::kx(lane / CH) ^ L::kx(first_row)) * 16, value_off = (uint32_t)(lane % CH ^ L::vx(lane / CH) ^ L::vx(first_row)) * 16;
+    auto bring = [&](const v4i &rs, uint32_t buffer, int j, uint32_t off, int x) PSQ_INLINE {
+        const uint32_t at = off ^ (x * 16), from = at + row_off + j * (64 / CH) * row_bytes;
+        dma16(rs, lds + buffer + first_row * L::PITCH + 1024 * j, PART && (int)at >= 2 * D ? kPast : from);
+    };
+    auto bring_keys = [&](const v4i &rs, uint32_t buffer, int j) PSQ_INLINE { bring(rs, buffer, j, key_off, L::kx(j * (64 / CH))); };
+    auto bring_values = [&](const v4i &rs, uint32_t buffer, int j) PSQ_INLINE { bring(rs, buffer, j, value_off, L::vx(j * (64 / CH))); };
+    // Codes go through registers: loaded (zeros where no tokens are), then widened into LDS.
+    constexpr int CP = ES == 1 ? (DD / 16 * L::RW + 63) / 64 : 1;     // 16-byte pieces of a lane
+    struct Codes { v4i piece[CP]; float scale; };
+    auto fetch = [&](Codes &c, const uint8_t *pool, const float *scales, const Tile &t) PSQ_INLINE {
+        const uint8_t *src = pool + row_of(t) * row_bytes;
 #pragma unroll
-        for (int i = 0; i < kGroup * L::PITCH / 1024; i++) {
-            const int at = i * 64 + lane, r = at / CH, c = at % CH, ck = c ^ L::kx(r), cv = c ^ L::vx(r);
-            koff[i] = (uint32_t)(r * row_bytes + (PART && ck * 8 >= D ? 0 : ck * 16));
-            voff[i] = (uint32_t)(r * row_bytes + (PART && cv * 8 >= D ? 0 : cv * 16));
+        for (int j = 0; j < CP; j++) {
+            const int at = 64 * j + lane, r = at / (DD / 16), p = at % (DD / 16);
+            c.piece[j] = v4i{0, 0, 0, 0};
+            if (r < t.left && (!PART || p * 16 < D)) c.piece[j] = *(const v4i *)(src + r * row_bytes + p * 16);
         }
-    }
-    auto stage = [&](int i, uint8_t *buf) {       // tile i's loads (codes: into registers)
-        const int bit = 4 * (i - base) + wave;
-        const bool here = there >> bit & 1;
-        const int64_t g = (uint32_t)__builtin_amdgcn_readlane((int)grp, bit);
+        c.scale = 0.0f;
+        if (lane < t.left) c.scale = scales[row_of(t) + lane];
+    };
+    auto deliver = [&](auto typec, const Codes &codes, uint32_t buffer, auto place) PSQ_INLINE {
+        const uint32_t to = lds + buffer + first_row * L::PITCH;
+#pragma unroll
+        for (int j = 0; j < CP; j++) {
+            const int at = 64 * j + lane, r = at / (DD / 16), c = 2 * (at % (DD / 16)), x = place(r) ^ place(first_row);
+            v4i w[2];
+            widen<decltype(typec)::value, CODES>(codes.piece[j], w);
+            if (64 * CP * 16 == L::RW * DD || r < L::RW) {
+                *at_lds<v4i>(to + r * L::PITCH + (c ^ x) * 16) = w[0];
+                *at_lds<v4i>(to + r * L::PITCH + ((c + 1) ^ x) * 16) = w[1];
+            }
+        }
+        if (lane < L::RW) *at_lds<float>(lds + buffer + L::TILE + 4 * (first_row + lane)) = codes.scale;
+    };
+    auto deliver_keys = [&](const Codes &c, uint32_t buffer) PSQ_INLINE { deliver(std::integral_constant<int, DT>{}, c, buffer, [](int r) { return L::kx(r); }); };
+    auto deliver_values = [&](const Codes &c, uint32_t buffer) PSQ_INLINE { deliver(std::integral_constant<int, PVT>{}, c, buffer, [](int r) { return L::vx(r); }); };
+    // or as they are: the wave's rows of a tile's keys and values, and their scales, to a raw buffer ...
+    constexpr int PIECES = L::RW * DD / 16;           // lanes that have 16 bytes of them
+    auto load_raw = [&](const Tile &t, uint32_t raw) PSQ_INLINE {
+        const int64_t row = row_of(t);
+        auto rows = [&](const void *pool, int bytes) PSQ_INLINE {
+            const uint64_t from = (uint64_t)pool + row * bytes;
+            return v4i{__builtin_amdgcn_readfirstlane((int)from), __builtin_amdgcn_readfirstlane((int)(from >> 32) & 0xffff),
+                       __builtin_amdgcn_readfirstlane(t.left * bytes), 0x00020000};
+        };
+        const int p = lane % (DD / 16);
+        const uint32_t off = PART && p * 16 >= D ? kPast : (uint32_t)(lane / (DD / 16) * row_bytes + p * 16);
+        const uint32_t at = lds + raw + first_row * DD, sc = lds + raw + kKeys * 2 * DD + first_row * 4;
+        const v4i rk = rows(a.kc, row_bytes), rv = rows(a.vc, row_bytes), sk = rows(a.ks, 4), sv = rows(a.vs, 4);
+        if (PIECES >= 64 || lane < PIECES) {
+            dma16(rk, at, off);
+            dma16(rv, at + kKeys * DD, off);
+        }
+        if (lane < L::RW) {
+            dma4(sk, sc, (uint32_t)lane * 4);
+            dma4(sv, sc + kKeys * 4, (uint32_t)lane * 4);
+        }
+    };
+    // ... and, once they are there, widened into the tile's place
+    auto raw_piece = [&](uint32_t raw, int values) PSQ_INLINE {
+        Codes c;
+        c.piece[0] = *at_lds<const v4i>(lds + raw + values * kKeys * DD + first_row * DD + lane % PIECES * 16);
+        c.scale = *at_lds<const float>(lds + raw + kKeys * 2 * DD + values * kKeys * 4 + 4 * (first_row + lane % L::RW));
+        return c;
+    };
+    // a tile at once
+    auto take_keys = [&](const Tile &t, uint32_t buffer) PSQ_INLINE {
         if constexpr (ES == 2) {
-            if (!here) return;
-            const __amdgpu_buffer_rsrc_t rk = raw_rsrc(a.kc + g * (kGroup * row_bytes)), rv = raw_rsrc(a.vc + g * (kGroup * row_bytes));
-            uint8_t *k = buf + wave * kGroup * L::PITCH, *v = k + L::TILE;
+            const v4i rs = descriptor(a.kc, t);
 #pragma unroll
-            for (int j = 0; j < kGroup * L::PITCH / 1024; j++) {
-                dma16(rk, (lds_ptr)(k + 1024 * j), koff[j]);
-                dma16(rv, (lds_ptr)(v + 1024 * j), voff[j]);
-            }
+            for (int j = 0; j < NL; j++) bring_keys(rs, buffer, j);
         } else {
-            // places behind the sequence hold zeros
-            const int left = here ? s.len - (keys.tile(i) * kKeys + kGroup * wave) : 0;
-            const uint8_t *k = a.kc + g * (kGroup * row_bytes), *v = a.vc + g * (kGroup * row_bytes);
-#pragma unroll
-            for (int j = 0; j < CP; j++) {
-                const int at = 64 * j + lane, r = at / (DD / 16), c = at % (DD / 16);
-                kreg[j] = vreg[j] = v4i{0, 0, 0, 0};
-                if (r < left && (!PART || c * 16 < D)) {
-                    kreg[j] = *(const v4i *)(k + r * row_bytes + c * 16);
-                    vreg[j] = *(const v4i *)(v + r * row_bytes + c * 16);
-                }
-            }
-            sreg = 0.0f;
-            if (lane < 32 && n % kGroup < left) sreg = (lane < kGroup ? a.ks : a.vs)[g * kGroup + n % kGroup];
+            Codes c;
+            fetch(c, a.kc, a.ks, t);
+            deliver_keys(c, buffer);
         }
     };
-    // values of 16 bits where no tokens are (behind the sequence, on pages that are not there): zeros, by the wave that
-    // brings the others of the group
-    auto clear = [&](int t0, uint32_t astray, uint8_t *buf) {
-        const int left = astray >> wave & 1 ? 0 : s.len - t0 - kGroup * wave;
-        uint8_t *v = buf + L::TILE + wave * kGroup * L::PITCH;
-        for (int at = lane; at < kGroup * CH; at += 64)
-            if (at / CH >= left) *(v4i *)(v + at * 16) = v4i{0, 0, 0, 0};
-    };
-    auto deliver = [&](uint8_t *buf) {            // codes from registers to LDS
-        if constexpr (ES == 1) {
-            uint8_t *k = buf + wave * kGroup * L::PITCH, *v = k + L::TILE;
+    auto take_values = [&](const Tile &t, uint32_t buffer) PSQ_INLINE {
+        if constexpr (ES == 2) {
+            const v4i rs = descriptor(a.vc, t);
 #pragma unroll
-            for (int j = 0; j < CP; j++) {
-                const int at = 64 * j + lane, r = at / (DD / 16), c = 2 * (at % (DD / 16));
-                v4i w[2];
-                widen<DT, CODES>(kreg[j], w);
-                *(v4i *)(k + r * L::PITCH + (c ^ L::kx(r)) * 16) = w[0];
-                *(v4i *)(k + r * L::PITCH + ((c + 1) ^ L::kx(r)) * 16) = w[1];
-                widen<PVT, CODES>(vreg[j], w);
-                *(v4i *)(v + r * L::PITCH + (c ^ L::vx(r)) * 16) = w[0];
-                *(v4i *)(v + r * L::PITCH + ((c + 1) ^ L::vx(r)) * 16) = w[1];
-            }
-            float *sc = (float *)(buf + 2 * L::TILE);
-            if (lane < 32) sc[(lane < kGroup ? 0 : kKeys) + wave * kGroup + n % kGroup] = sreg;
+            for (int j = 0; j < NL; j++) bring_values(rs, buffer, j);
+        } else {
+            Codes c;
+            fetch(c, a.vc, a.vs, t);
+            deliver_values(c, buffer);
         }
     };
 
     // ---- a key tile of the wave's rows
     v16f o[ND];
     float run_m, run_l;    // the maximum that scores are taken off (in their own units); the lane's part of the sum
-    const uint32_t klane = n * L::PITCH + ((h ^ L::kx(n)) << 4);
-    const uint32_t vlane = (4 * h + (n & 15) / 4) * L::PITCH + ((((n >> 4) << 1 | (n & 3) >> 1) ^ L::vx((n & 15) / 4)) << 4) + (n & 1) * 8;
-    auto compute = [&](auto carefulc, int tile0, bool edge, uint32_t astray, const uint8_t *buf) {
-        constexpr bool CAREFUL = decltype(carefulc)::value;
-        v16f sc[2];
+    uint32_t seen;         // (carefully) scores that count
+    bool raise;            // of the tile's maximum over run_m
+    float top;             // of the tile: the lane's, then the row's
+    // LDS addresses of the lane's reads in the first buffers.  Chunks are picked by exclusive or of a row's low bits, which
+    // the buffers' offsets leave alone.
+    const uint32_t klane = lds + n * L::PITCH + ((h ^ L::kx(n)) << 4);
+    const uint32_t vlane = lds + (4 * h + (n & 15) / 4) * L::PITCH + ((((n >> 4) << 1 | (n & 3) >> 1) ^ L::vx((n & 15) / 4)) << 4) + (n & 1) * 8;
+    auto key = [&](uint32_t at, int t, int c) PSQ_INLINE { return *at_lds<const v4i>((at ^ (c << 5)) + 32 * t * L::PITCH); };
+    auto value = [&](uint32_t at, int u, int d) PSQ_INLINE {
+        const uint32_t src = (at ^ (d << 6)) + 16 * u * L::PITCH;
+        const v2i x = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16(at_lds<v4s>(src)));
+        const v2i y = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16(at_lds<v4s>(src + 8 * L::PITCH)));
+        return v4i{x[0], x[1], y[0], y[1]};
+    };
+    // scores of a tile from its products: scales, masks, their maximum (turn has done the first, and the last where there are
+    // no masks)
+    auto scale_keys = [&](v16f (&sc)[2], int q, const v4f &x) PSQ_INLINE {
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-#pragma unroll
-            for (int i = 0; i < 16; i++) sc[t][i] = 0.0f;
-#pragma unroll
-            for (int c = 0; c < NC; c++)
-                if (!PART || 16 * c < D) sc[t] = mfma<DT>(*(const v4i *)(buf + 32 * t * L::PITCH + (klane ^ (c << 5))), qf[c], sc[t]);
-        }
-        if constexpr (!PART) ahead<2 * NC, 1, 4>();
-        const float *scales = (const float *)(buf + 2 * L::TILE);
-        if constexpr (ES == 1) {
-#pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    const v4f x = *(const v4f *)(scales + 32 * t + 2 * i + 4 * h);
-#pragma unroll
-                    for (int j = 0; j < 4; j++) sc[t][i + j] *= x[j];
-                }
-        }
-        uint32_t seen = 0;
-        int t0 = tile0;
-        if (CAREFUL || edge) {
-            asm volatile("" : "+v"(t0));   // (a branch, not selects that all tiles pay for)
-            // key 32 t + 8 (i >> 2) + (i & 3) of the lane's against these
-            const int at = t0 + 4 * h, to = min(pos, s.text - 1) - at, from = low - at, sinks = a.sinks - at, text = s.text - at;
-#pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int k = 32 * t + 8 * (i >> 2) + (i & 3);
-                    bool see = (k <= to) & ((k >= from) | (k < sinks));
-                    if (a.N) {
-                        const uint32_t draft = (uint32_t)(k - text);
-                        see |= (draft < 64) & ((uint32_t)(way >> (draft & 63)) & 1);
-                    }
-                    if (astray >> (2 * t + (i >> 3)) & 1) sc[t][i] = NAN;    // its page is not there
-                    if (!see) sc[t][i] = -INFINITY;
-                    if (CAREFUL) seen |= (uint32_t)see << (16 * t + i);
-                }
-        }
-        // (NaN wins; it raises nothing, and the row's sum will be NaN)
-        float top = __builtin_elementwise_maximum(sc[0][0], sc[1][0]);
+        for (int j = 0; j < 4; j++) sc[q / 4][4 * (q & 3) + j] *= x[j];
+    };
+    auto scale_of = [&](uint32_t buffer, int q) PSQ_INLINE { return *at_lds<const v4f>(lds + buffer + L::TILE + 4 * (32 * (q / 4) + 8 * (q & 3) + 4 * h)); };
+    auto lane_top = [&](const v16f (&sc)[2]) PSQ_INLINE {
+        top = __builtin_elementwise_maximum(sc[0][0], sc[1][0]);
 #pragma unroll
         for (int i = 1; i < 16; i++) top = __builtin_elementwise_maximum(top, __builtin_elementwise_maximum(sc[0][i], sc[1][i]));
+    };
+    auto row_top = [&]() PSQ_INLINE {
+        // (NaN wins; it raises nothing, and the row's sum will be NaN)
         top = half_max(top);
         // (a maximum that comes first, or is raised from -inf, is any growth)
-        const bool raise = top * a.scale > run_m * a.scale + kGrowth;
-        if (__any(raise)) {
-            const float next = raise ? top : run_m;    // (each row by itself: its result does not depend on the others')
-            float keep = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((run_m - next) * a.scale);
-            if (CAREFUL) keep = fmaxf(keep, 0x1p-126f);   // (an infinite sum stays one)
-            run_m = next;
-            run_l *= keep;
+        raise = top * a.scale > run_m * a.scale + kGrowth;
+    };
+    auto scores = [&](v16f (&sc)[2], int tile0, bool edge, uint32_t astray) PSQ_INLINE {
+        if (CAREFUL) seen = 0;
+        if (CAREFUL || edge) {
+            int t0 = tile0;
+            asm volatile("" : "+v"(t0));   // (a branch, not selects that all tiles pay for)
+            if (astray)                    // pages that are not there: NaN
 #pragma unroll
-            for (int d = 0; d < ND; d++)
+                for (int t = 0; t < 2; t++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) o[d][i] *= keep;
+                    for (int i = 0; i < 16; i++)
+                        if (astray >> (2 * t + (i >> 3)) & 1) sc[t][i] = NAN;
+            // Bits c of a word: key 32 t + c of the lane's half, c = 8 (i >> 2) + (i & 3).  below(x): those with c < x.
+            auto below = [](int x) { return x <= 0 ? 0u : x >= 32 ? ~0u : (1u << x) - 1; };
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const int at = t0 + 32 * t + 4 * h, text = s.text - at;
+                uint32_t see = below(min(pos + 1, s.text) - at) & (~below(low - at) | below(a.sinks - at));
+                if (a.N) see |= text >= 0 ? (text < 32 ? (uint32_t)way << text : 0) : text > -64 ? (uint32_t)(way >> -text) : 0;
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int on = (int)(see << (31 - (8 * (i >> 2) + (i & 3)))) >> 31;
+                    sc[t][i] = __int_as_float((__float_as_int(sc[t][i]) & on) | (~on & (int)0xff800000));
+                }
+                if (CAREFUL) seen |= ((see & 15) | (see >> 4 & 0xf0) | (see >> 8 & 0xf00) | (see >> 12 & 0xf000)) << (16 * t);
+            }
+            lane_top(sc);
+            row_top();
         }
+    };
+    auto grow = [&]() PSQ_INLINE {
+        if (!__any(raise)) return;
+        const float to = raise ? top : run_m;    // (each row by itself: its result does not depend on the others')
+        float keep = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((run_m - to) * a.scale);
+        if (CAREFUL) keep = fmaxf(keep, 0x1p-126f);   // (an infinite sum stays one)
+        run_m = to;
+        run_l *= keep;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[d][i] *= keep;
+    };
+    // Scores in sc, the tile's values in vb, the next tile's keys in kb: its products into sc, the tile's weights and
+    // values into o.
+    auto turn = [&](const v16f (&sc)[2], v16f (&next)[2], uint32_t kb, uint32_t vb, auto aside) PSQ_INLINE {
+        const uint32_t kat = again(klane + kb), vat = again(vlane + vb);
         const float ref = (PVT == PSQ_F16 ? kF16Unit : 0) - (run_m == -INFINITY ? 0.0f : run_m * a.scale);
         v4i ph[4], pl[PAIR ? 4 : 1];
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                sc[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i], a.scale, ref));
-                run_l += sc[t][i];
-            }
+        v4f vs, ks;        // scales at hand
+        // two scores to weights: pair q of the tile's 16
+        auto weigh = [&](auto qc) PSQ_INLINE {
+            constexpr int Q = decltype(qc)::value, T = Q / 8, I = 2 * (Q & 7);
+            float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[T][I], a.scale, ref)), y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[T][I + 1], a.scale, ref));
+            run_l += x;
+            run_l += y;
             if constexpr (ES == 1) {
-#pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    const v4f x = *(const v4f *)(scales + kKeys + 32 * t + 2 * i + 4 * h);
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        sc[t][i + j] *= x[j];
-                        if (CAREFUL && !(seen >> (16 * t + i + j) & 1)) sc[t][i + j] = 0.0f;   // (its scale may be infinite)
-                    }
+                if constexpr (Q % 2 == 0) {
+                    vs = scale_of(vb, Q / 2);
                 }
+                x *= vs[I & 2], y *= vs[(I & 2) + 1];
+                if (CAREFUL && !(seen >> (16 * T + I) & 1)) x = 0.0f;        // (its scale may be infinite)
+                if (CAREFUL && !(seen >> (16 * T + I + 1) & 1)) y = 0.0f;
             }
+            const uint32_t p = pack_half2<PVT>(x, y);
+            ph[Q / 4][Q & 3] = (int)p;
+            if constexpr (PAIR) pl[Q / 4][Q & 3] = (int)pack_half2<PVT>(x - half_to_f32<PVT>(p), y - half_to_f32<PVT>(p >> 16));
+        };
+        // A slot is a matrix instruction, the LDS read of the one AHEAD slots later, and what vector work it covers:
+        // vector and matrix units work at the same time only where the instructions of both take turns (two
+        // waves of a SIMD fall into step).  First the next tile's scores, then the values with the weights, of which
+        // those of a step of 16 keys are ready when it begins; beside these the maximum of the next tile's.
+        constexpr int AHEAD = ES == 1 ? 2 : 4, QK = 2 * NC, ALL = QK + 4 * ND, COVER = QK + 3 * ND;
+        if constexpr (CAREFUL) {
+            static_for<16>([&](auto q) PSQ_INLINE {
+                weigh(q);
+                __builtin_amdgcn_sched_barrier(0);   // (here and below: it is not to need more registers than the other)
+            });
 #pragma unroll
-            for (int u = 0; u < 2; u++)
+            for (int u = 0; u < 4; u++)
 #pragma unroll
-                for (int d = 0; d < 4; d++) {
-                    const float x = sc[t][8 * u + 2 * d], y = sc[t][8 * u + 2 * d + 1];
-                    const uint32_t p = pack_half2<PVT>(x, y);
-                    ph[2 * t + u][d] = (int)p;
-                    if constexpr (PAIR) pl[2 * t + u][d] = (int)pack_half2<PVT>(x - half_to_f32<PVT>(p), y - half_to_f32<PVT>(p >> 16));
-                }
-        }
-        const uint8_t *vb = buf + L::TILE;
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-#pragma unroll
-            for (int d = 0; d < ND; d++) {
-                if (PART && 32 * d >= D) break;
-                const uint8_t *src = vb + 16 * u * L::PITCH + (vlane ^ (d << 6));
-                const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)src);
-                const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(src + 8 * L::PITCH));
-                const v2i xi = __builtin_bit_cast(v2i, x), yi = __builtin_bit_cast(v2i, y);
-                v4i vf{xi[0], xi[1], yi[0], yi[1]};
-                if constexpr (CAREFUL) {
+                for (int d = 0; d < ND; d++) {
                     constexpr uint32_t EXP = PVT == PSQ_BF16 ? 0x7f80 : 0x7c00, ONE = PVT == PSQ_BF16 ? 0x3f80 : 0x3c00;
-                    v4i up, down, look;     // ones where a value is +inf, is -inf (NaN: both); where a key is seen
+                    v4i vf = value(vat, u, d), up, down, is;     // ones where a value is +inf, is -inf (NaN: both); where a key is seen
                     bool any = false;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
@@ -569,72 +610,226 @@ block_attention_kernel(Args a)
                             pd |= (odd & (nan | ((w & 0x8000) != 0)) ? ONE : 0) << (16 * k);
                             ps |= (seen >> (8 * u + 2 * e + k) & 1 ? ONE : 0) << (16 * k);
                         }
-                        vf[e] = (int)c, up[e] = (int)pu, down[e] = (int)pd, look[e] = (int)ps;
+                        vf[e] = (int)c, up[e] = (int)pu, down[e] = (int)pd, is[e] = (int)ps;
                     }
                     if (__any(any)) {
                         v16f zero = {};
-                        const v16f more = mfma<PVT>(up, look, zero), less = mfma<PVT>(down, look, zero);
+                        const v16f more = mfma<PVT>(up, is, zero), less = mfma<PVT>(down, is, zero);
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
                             if (more[i] > 0.0f) o[d][i] += INFINITY;
                             if (less[i] > 0.0f) o[d][i] -= INFINITY;
                         }
                     }
+                    o[d] = mfma<PVT>(vf, ph[u], o[d]);
+                    if constexpr (PAIR) o[d] = mfma<PVT>(vf, pl[u], o[d]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                o[d] = mfma<PVT>(vf, ph[u], o[d]);
-                if constexpr (PAIR) o[d] = mfma<PVT>(vf, pl[u], o[d]);
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                next[t] = v16f{};
+#pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    next[t] = mfma<DT>(key(kat, t, c), qf[c], next[t]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
+            if constexpr (ES == 1)
+#pragma unroll
+                for (int q = 0; q < 8; q++) scale_keys(next, q, scale_of(kb, q));
+            lane_top(next);
+            row_top();
+            static_for<ALL>([&](auto i) PSQ_INLINE { aside(i); });
+        } else {
+            v4i f[AHEAD];
+            auto read = [&](auto ic) PSQ_INLINE {
+                constexpr int I = decltype(ic)::value;
+                if constexpr (I < QK) f[I % AHEAD] = key(kat, I / NC, I % NC);
+                else if constexpr (I < ALL) f[I % AHEAD] = value(vat, (I - QK) / ND, (I - QK) % ND);
+            };
+            static_for<AHEAD>([&](auto i) PSQ_INLINE { read(i); });
+            static_for<ALL>([&](auto ic) PSQ_INLINE {
+                constexpr int I = decltype(ic)::value;
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (I < QK) {
+                    if constexpr (I % NC == 0) next[I / NC] = mfma<DT>(f[I % AHEAD], qf[0], v16f{});
+                    else next[I / NC] = mfma<DT>(f[I % AHEAD], qf[I % NC], next[I / NC]);
+                } else {
+                    constexpr int U = (I - QK) / ND, V = (I - QK) % ND;
+                    o[V] = mfma<PVT>(f[I % AHEAD], ph[U], o[V]);
+                    if constexpr (PAIR) o[V] = mfma<PVT>(f[I % AHEAD], pl[U], o[V]);
+                }
+                read(std::integral_constant<int, I + AHEAD>{});
+                aside(ic);
+                // some of the next scores, four at a time: scaled, and their maximum, the row's in the end
+                if constexpr (I >= QK) {
+                    constexpr int TOP = 4 * ND - 3, P = (I - QK) * 32 / TOP / 4 * 4, E = (I - QK + 1) * 32 / TOP / 4 * 4;
+                    static_for<32>([&](auto kc) PSQ_INLINE {
+                        constexpr int K = decltype(kc)::value;
+                        if constexpr (K >= P && K < E && I - QK < TOP) {
+                            if constexpr (ES == 1) {
+                                if constexpr (K % 4 == 0) ks = scale_of(kb, K / 4);
+                                next[K / 16][K % 16] *= ks[K & 3];
+                            }
+                            if constexpr (K == 1) top = __builtin_elementwise_maximum(next[0][0], next[0][1]);
+                            else if constexpr (K % 2) top = __builtin_elementwise_maximum(top, __builtin_elementwise_maximum(next[K / 16][K % 16 - 1], next[K / 16][K % 16]));
+                        }
+                    });
+                    if constexpr (I - QK == TOP) row_top();
+                }
+                // pairs q of COVER slots' share
+                constexpr int A = I * 16 / COVER, B = (I + 1) * 16 / COVER;
+                static_for<16>([&](auto q) PSQ_INLINE {
+                    if constexpr (I < COVER && decltype(q)::value >= A && decltype(q)::value < B) weigh(q);
+                });
+            });
+            asm volatile("" : "+v"(run_l));    // (its sums belong to the slots)
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if constexpr (!PART && !CAREFUL) ahead<4 * ND, 2, 4, PAIR ? 2 : 1>();
     };
 
     // All of the workgroup's key tiles of the unit.
-    auto pass = [&](auto carefulc) {
+    auto pass = [&]() PSQ_INLINE {
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
             for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
         run_m = -INFINITY, run_l = 0.0f;
-        uint32_t here = 0, next = L::BUFFER;   // offsets of the buffers
-        uint32_t astray = 0;
         __syncthreads();                       // LDS is free
         int i = next_of(first);
-        if (i < last) {
-            look(i);
-            stage(i, smem);
-            astray = (uint32_t)wild & 15;
-            deliver(smem);
-        }
-        while (i < last) {
-            const int j = next_of(i + 1), t0 = keys.tile(i) * kKeys, t1 = t0 + kKeys - 1;
-            wait_vmcnt<0>();
-            if (ES == 2 && (t1 >= s.len || astray)) clear(t0, astray, smem + here);
-            stage_barrier();                   // the tile is here, and the one before it is done with
-            uint32_t gone = 0;
-            if (j < last) {
-                if (j - base >= kLook) look(j);
-                stage(j, smem + next);
-                gone = (uint32_t)(wild >> (4 * (j - base))) & 15;
+        if (i >= last) return;
+        // whether a tile's masks hide some of it from some row of the wave
+        auto edge = [&](const Tile &t) {
+            const int tile0 = t.number * kKeys, tile1 = tile0 + kKeys - 1;
+            return !(tile1 <= full_hi && (tile0 >= full_lo || tile1 < a.sinks) && !t.astray);
+        };
+        constexpr int DK = L::DK, DV = L::DV;
+        constexpr uint32_t VALUES = L::RK * L::BUFFER, VALUES_END = L::RAW_AT;
+        Tile q[L::AHEAD + 1];                        // the tile at hand and those behind it
+        look(i);
+#pragma unroll
+        for (int d = 0; d < L::AHEAD; d++) {
+            q[d] = tile_at(d ? next_of(at_tile + 1) : i);
+            if constexpr (L::RAW) {
+                load_raw(q[d], L::RAW_AT + d * L::RAW_TILE);
+            } else {
+                take_keys(q[d], d * L::BUFFER);
+                if (d < DV) take_values(q[d], VALUES + d * L::BUFFER);
             }
-            if (mine > 0 && t0 <= any_hi && (t1 >= any_lo || t0 < a.sinks))
-                compute(carefulc, t0, !(t1 <= full_hi && (t0 >= full_lo || t1 < a.sinks) && !astray), astray, smem + here);
-            if (j < last) deliver(smem + next);
-            astray = gone, i = j;
-            std::swap(here, next);
         }
+        wait_vmcnt<0>();
+        asm volatile("" ::: "memory");
+        if constexpr (L::RAW) {
+            deliver_keys(raw_piece(L::RAW_AT, 0), 0);
+            deliver_keys(raw_piece(L::RAW_AT + L::RAW_TILE, 0), L::BUFFER);
+            deliver_values(raw_piece(L::RAW_AT, 1), VALUES);
+        }
+        stage_barrier();
+        uint32_t raw = L::RAW_AT;              // the raw buffer of the tile at hand, whose codes are done with
+        // buffers: of the keys read (the next tile's) and loaded, the values read and loaded
+        uint32_t kr = L::BUFFER, kl = DK % L::RK * L::BUFFER, vr = VALUES, vl = VALUES + DV * L::BUFFER;
+        auto advance = [](uint32_t &at, uint32_t from, uint32_t end) PSQ_INLINE {
+            at += L::BUFFER;
+            if (at == end) at = from;
+        };
+        // q[0]'s scores are in sc, its values and q[1]'s keys here once the loads up to them are; q[0]'s keys are done with.
+        // False: q[0] was the last (the products of what lies in place of the next one's keys are not used).
+        auto step = [&](auto workc, auto meetc, v16f (&sc)[2], v16f (&to)[2]) PSQ_INLINE {
+            constexpr bool WORK = decltype(workc)::value;
+            if constexpr (decltype(meetc)::value) {
+                if constexpr (!L::RAW) wait_vmcnt<0>();     // (raw tiles are waited for where they are widened)
+                stage_barrier();
+            }
+            q[L::AHEAD] = tile_at(next_of(at_tile + 1));
+            if constexpr (L::RAW) {
+                auto behind = [&](int tiles) PSQ_INLINE {
+                    const uint32_t at = raw + tiles * L::RAW_TILE;
+                    return at >= (uint32_t)L::BYTES ? at - L::RR * L::RAW_TILE : at;
+                };
+                // the wave's own loads of the tile two behind, and those before, are here when as many are on their way as came after
+                Codes ck, cv;
+                auto convert = [&](auto ic) PSQ_INLINE {
+                    constexpr int I = decltype(ic)::value;
+                    if constexpr (I == 1) load_raw(q[L::RR], raw);
+                    if constexpr (I == 3) {
+                        wait_vmcnt<(L::RR - 2) * 4>();
+                        asm volatile("" ::: "memory");
+                        cv = raw_piece(behind(1), 1);
+                    }
+                    if constexpr (I == 6) deliver_values(cv, vl);
+                    if constexpr (I == 8) ck = raw_piece(behind(2), 0);
+                    if constexpr (I == 11) deliver_keys(ck, kl);
+                };
+                if constexpr (WORK) {
+                    grow();
+                    turn(sc, to, kr, vr, convert);
+                } else {
+                    static_for<12>([&](auto ic) PSQ_INLINE { convert(ic); });
+                }
+                raw = behind(1);
+            } else if constexpr (ES == 2) {
+                const v4i rv = descriptor(a.vc, q[DV]), rk = descriptor(a.kc, q[DK]);
+                auto load = [&](auto ic) PSQ_INLINE {      // one in two slots
+                    constexpr int I = decltype(ic)::value;
+                    if constexpr (I % 2 == 1 && I / 2 < NL) bring_values(rv, vl, I / 2);
+                    else if constexpr (I % 2 == 1 && I / 2 < 2 * NL) bring_keys(rk, kl, I / 2 - NL);
+                };
+                if constexpr (WORK) {
+                    grow();
+                    turn(sc, to, kr, vr, load);
+                } else {
+                    static_for<4 * NL>([&](auto ic) PSQ_INLINE { load(ic); });
+                }
+            } else {
+                Codes ck, cv;
+                fetch(cv, a.vc, a.vs, q[DV]);
+                fetch(ck, a.kc, a.ks, q[DK]);
+                if constexpr (WORK) {
+                    grow();
+                    turn(sc, to, kr, vr, [](auto) {});
+                }
+                deliver_values(cv, vl);
+                deliver_keys(ck, kl);
+            }
+            if (q[1].number < 0) return false;
+            if constexpr (WORK) scores(to, q[1].number * kKeys, edge(q[1]), (uint32_t)q[1].astray);
+#pragma unroll
+            for (int d = 0; d < L::AHEAD; d++) q[d] = q[d + 1];
+            advance(kr, 0, VALUES), advance(kl, 0, VALUES), advance(vr, VALUES, VALUES_END), advance(vl, VALUES, VALUES_END);
+            return true;
+        };
+        v16f sa[2] = {}, sb[2] = {};
+        using Meet = std::true_type;
+        using Other = std::bool_constant<L::STEPS == 1>;
+        if (mine == 0) {                       // (waves without rows bring their groups)
+            while (step(std::false_type{}, Meet{}, sa, sb) && step(std::false_type{}, Other{}, sa, sb)) {}
+            return;
+        }
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int c = 0; c < NC; c++) sa[t] = mfma<DT>(key(klane, t, c), qf[c], sa[t]);
+        if constexpr (ES == 1)
+#pragma unroll
+            for (int q = 0; q < 8; q++) scale_keys(sa, q, scale_of(0, q));
+        lane_top(sa);
+        row_top();
+        scores(sa, q[0].number * kKeys, edge(q[0]), (uint32_t)q[0].astray);
+        using Work = std::true_type;
+        while (step(Work{}, Meet{}, sa, sb) && step(Work{}, Other{}, sb, sa)) {}
     };
-    pass(std::false_type{});
+    pass();
+    wait_vmcnt<0>();       // (loads into the LDS end before it may be another's)
     float any = 0.0f;
 #pragma unroll
     for (int d = 0; d < ND; d++)
         if (!PART || 32 * d < D)
 #pragma unroll
             for (int i = 0; i < 16; i++) any = __builtin_fmaf(o[d][i], 0.0f, any);
-    if (__syncthreads_or(any != any)) pass(std::true_type{});
 
     // ---- the rows' outputs, or the part of them
     run_l = half_sum(run_l);
-    const float top = run_m * a.scale - (PVT == PSQ_F16 ? kF16Unit : 0);     // (in log2, the weights' unit taken off)
+    const float level = run_m * a.scale - (PVT == PSQ_F16 ? kF16Unit : 0);     // (in log2, the weights' unit taken off)
     const int64_t at = (int64_t)(s.first + token) * a.Hq + head;
     if (valid && whole) {
         const float r = pos < 0 ? 0.0f : 1.0f / run_l;    // (sees nothing: zeros)
@@ -646,16 +841,79 @@ block_attention_kernel(Args a)
                 if (!PART || dim < D)
                     *(v2i *)(a.out + at * D + dim) = v2i{(int)pack_half2<DT>(o[d][i] * r, o[d][i + 1] * r), (int)pack_half2<DT>(o[d][i + 2] * r, o[d][i + 3] * r)};
             }
-        if (a.lse && h == 0) a.lse[at] = pos < 0 ? -INFINITY : top * kLn2 + logf(run_l);
+        if (a.lse && h == 0) a.lse[at] = pos < 0 ? -INFINITY : level * kLn2 + logf(run_l);
     } else if (valid) {
-        float *part = a.part + (2 * (int64_t)xcd_rank(blockIdx.x, a.runs) + (first == 0)) * part_floats<DD>();
+        float *part = a.part + (2 * (int64_t)xcd_rank(blockIdx.x, a.runs) + (first == 0)) * part_floats(a.rows, DD);
         const int r = 32 * wave + n;
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
-                ((v4f *)part)[(8 * d + i / 2 + h) * kRows + r] = v4f{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
-        if (h == 0) part[kRows * DD + r] = top, part[kRows * (DD + 1) + r] = pos < 0 ? -1.0f : run_l;
+                ((v4f *)part)[(8 * d + i / 2 + h) * a.rows + r] = v4f{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
+        if (h == 0) part[a.rows * DD + r] = level, part[a.rows * (DD + 1) + r] = pos < 0 ? -1.0f : run_l;
+    }
+    return any != any;
+}
+
+template <int DT, int CODES, int DD, bool PART, int W>
+__global__ void __launch_bounds__(64 * W, DD > 128 ? 1 : 2)
+block_attention_kernel(Args a)
+{
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+    const uint32_t lds = (uint32_t)(uintptr_t)(lds_ptr)smem;
+
+    // ---- the workgroup's units
+    const int count = a.N ? a.B : a.B + 1;
+    int b, r0, first = 0, tiles = 0;       // key tiles first .. of the unit's list are the workgroup's
+    uint32_t hk, x = 0, end = 0;
+    Runs runs{};
+    if (!a.runs) {
+        auto tiles_of = [&](int b) { return (uint32_t)row_tiles(a, sequence(a, b)); };
+        const uint32_t all = sum_of(count, tiles_of), units = all * a.Hkv;
+        if (blockIdx.x >= units) return;
+        // Workgroups of an XCD share a kv head's keys and values in its L2; the rows that see most go first.
+        const uint32_t rank = (uint32_t)xcd_rank(blockIdx.x, units);
+        hk = rank / all;
+        uint32_t before;
+        const uint32_t place = all - 1 - (rank - hk * all);
+        b = __builtin_amdgcn_readfirstlane(find(count, place, before, tiles_of));
+        r0 = (int)(place - before) * a.rows;
+    } else {
+        runs = runs_of(a, count);
+        const uint32_t w = (uint32_t)xcd_rank(blockIdx.x, a.runs);
+        if (w >= runs.runs) return;
+        x = runs.first(w), end = runs.first(w + 1);
+    }
+
+    do {
+    bool whole = true;
+    if (a.runs) {
+        uint32_t before;
+        b = __builtin_amdgcn_readfirstlane(find(count, x, before, [&](int b) { return weight_of(a, b); }));
+        const Seq s = sequence(a, b);
+        const uint32_t each = (uint32_t)key_tiles(a, s), per = (uint32_t)row_tiles(a, s), unit = (x - before) / each;
+        hk = unit / per, r0 = (int)(unit - hk * per) * a.rows;
+        first = (int)(x - before - unit * each);
+        tiles = (int)min(each - first, end - x);
+        whole = tiles == (int)each;
+        x += tiles;
+    }
+    const bool odd = block_unit<DT, CODES, DD, PART, W, false>(a, lds, b, hk, r0, first, tiles, whole);
+    // (whether any wave's is; the LDS has no room beside the tiles)
+    const bool some = __any(odd);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) *at_lds<int>(lds + 4 * (threadIdx.x / 64)) = some;
+    __syncthreads();
+    int odds = 0;
+#pragma unroll
+    for (int w = 0; w < W; w++) odds |= *at_lds<int>(lds + 4 * w);
+    if (__builtin_amdgcn_readfirstlane(odds)) {
+        auto *args = (const __attribute__((address_space(4))) uint32_t *)__builtin_amdgcn_kernarg_segment_ptr();
+        asm volatile("" : "+s"(args));
+        uint32_t words[sizeof(Args) / 4];
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(Args) / 4); i++) words[i] = args[i];
+        block_unit<DT, CODES, DD, PART, W, true>(__builtin_bit_cast(Args, words), lds, b, hk, r0, first, tiles, whole);
     }
     } while (x < end);
 }
@@ -673,7 +931,7 @@ join_kernel(Args a)
     const int b = __builtin_amdgcn_readfirstlane(find(count, blockIdx.x, before, units_of));
     const Seq s = sequence(a, b);
     const uint32_t unit = blockIdx.x - before, each = (uint32_t)key_tiles(a, s), per = (uint32_t)row_tiles(a, s), hk = unit / per;
-    const int r0 = (int)(unit - hk * per) * kRows, r = (int)blockIdx.y * kJoin + (threadIdx.x & (kJoin - 1)), quad = threadIdx.x / kJoin;
+    const int r0 = (int)(unit - hk * per) * a.rows, r = (int)blockIdx.y * kJoin + (threadIdx.x & (kJoin - 1)), quad = threadIdx.x / kJoin;
     const Runs runs = runs_of(a, count);
     const uint32_t x = sum_of(b, [&](int b) { return weight_of(a, b); }) + unit * each;
     const uint32_t w0 = runs.owner(x), parts = runs.owner(x + each - 1) - w0 + 1;
@@ -689,9 +947,9 @@ join_kernel(Args a)
             const uint32_t p = p0 + u;
             y[u] = v4f{0, 0, 0, 0}, m[u] = -INFINITY, l[u] = 0.0f;
             if (p < parts) {
-                const float *part = a.part + (2 * (int64_t)(w0 + p) + (p == 0)) * part_floats<DD>();
-                y[u] = ((const v4f *)part)[quad * kRows + r];
-                m[u] = part[kRows * DD + r], l[u] = part[kRows * (DD + 1) + r];
+                const float *part = a.part + (2 * (int64_t)(w0 + p) + (p == 0)) * part_floats(a.rows, DD);
+                y[u] = ((const v4f *)part)[quad * a.rows + r];
+                m[u] = part[a.rows * DD + r], l[u] = part[a.rows * (DD + 1) + r];
             }
         }
         float to = M;
@@ -719,11 +977,12 @@ join_kernel(Args a)
     if (a.lse && quad == 0) a.lse[at] = none ? -INFINITY : M * kLn2 + logf(L);
 }
 
-template <int DT, int CODES, int DD, bool PART>
+template <int DT, int CODES, int DD, bool PART, int W>
 int launch(const Args &a, unsigned groups, hipStream_t st)
 {
-    auto *kernel = block_attention_kernel<DT, CODES, DD, PART>;
-    const int lds = 2 * Layout<DD>::BUFFER;
+    auto *kernel = block_attention_kernel<DT, CODES, DD, PART, W>;
+    constexpr int lds = Layout<DD, W, CODES == PSQ_CODES_NONE ? 2 : 1>::BYTES;
+    static_assert(lds <= 160 * 1024 / (W == 4 && DD <= 128 ? 2 : 1), "tiles fit the LDS");
     static bool raised[64] = {};
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return set_error(PSQ_E_DEVICE, "no current HIP device");
@@ -732,20 +991,28 @@ int launch(const Args &a, unsigned groups, hipStream_t st)
             return set_error(PSQ_E_DEVICE, "block attention: cannot raise the LDS size");
         raised[dev] = true;
     }
-    kernel<<<a.runs ? a.runs : groups, kThreads, lds, st>>>(a);
-    if (a.runs) join_kernel<DT, DD><<<dim3(groups, kRows / (1024 / DD)), kThreads, 0, st>>>(a);
+    kernel<<<a.runs ? a.runs : groups, 64 * W, lds, st>>>(a);
+    if (a.runs) join_kernel<DT, DD><<<dim3(groups, a.rows / (1024 / DD)), kThreads, 0, st>>>(a);
     return check_launch("block attention");
 }
 
 template <int DT, int CODES>
 int launch_dim(const Args &a, unsigned groups, hipStream_t st)
 {
-    if (a.D == 64) return launch<DT, CODES, 64, false>(a, groups, st);
-    if (a.D == 128) return launch<DT, CODES, 128, false>(a, groups, st);
-    if (a.D == 256) return launch<DT, CODES, 256, false>(a, groups, st);
-    if (a.D < 64) return launch<DT, CODES, 64, true>(a, groups, st);
-    if (a.D < 128) return launch<DT, CODES, 128, true>(a, groups, st);
-    return launch<DT, CODES, 256, true>(a, groups, st);
+    if (a.rows == 256) {
+        if (a.D == 64) return launch<DT, CODES, 64, false, 8>(a, groups, st);
+        if (a.D == 128) return launch<DT, CODES, 128, false, 8>(a, groups, st);
+        if (a.D < 64) return launch<DT, CODES, 64, true, 8>(a, groups, st);
+        return launch<DT, CODES, 128, true, 8>(a, groups, st);
+    }
+    if (a.D == 256) return launch<DT, CODES, 256, false, 4>(a, groups, st);
+    if constexpr (CODES == PSQ_CODES_NONE) {
+        if (a.D == 64) return launch<DT, CODES, 64, false, 4>(a, groups, st);
+        if (a.D == 128) return launch<DT, CODES, 128, false, 4>(a, groups, st);
+        if (a.D < 64) return launch<DT, CODES, 64, true, 4>(a, groups, st);
+        if (a.D < 128) return launch<DT, CODES, 128, true, 4>(a, groups, st);
+    }
+    return launch<DT, CODES, 256, true, 4>(a, groups, st);
 }
 
 // by element type of the queries and kind of cache, each compiled in a file of its own

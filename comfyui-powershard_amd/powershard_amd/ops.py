@@ -835,9 +835,9 @@ def _rows_on_cache(name, q, rows, k_cache, v_cache, block_table, lengths, k_scal
     return index, code, dt, (pages, Hk, page, D), ks, vs, block_table, lengths if lengths.is_contiguous() else lengths.contiguous()
 
 
-def _parts(rows, B, N, H, Hk, D, window, sinks, max_len, device):
+def _parts(code, rows, B, N, H, Hk, D, window, sinks, max_len, device):
     """(memory of the call's own for the parts of split sequences, its bytes)."""
-    nb = _native.lib().psq_paged_block_workspace_bytes(rows, B, N, H, Hk, D, window, sinks, max_len)
+    nb = _native.lib().psq_paged_block_workspace_bytes(code, rows, B, N, H, Hk, D, window, sinks, max_len)
     return (torch.empty(nb, dtype=torch.uint8, device=device) if nb else None), nb
 
 
@@ -864,7 +864,7 @@ def paged_prompt_attention(q, k_cache, v_cache, block_table, starts, lengths, k_
     max_len = cols * page if max_len is None or max_len < 0 else min(int(max_len), cols * page)
     out = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
     lse = torch.empty((T, H), dtype=torch.float32, device=q.device) if return_lse else None
-    ws, nb = _parts(T, B, 0, H, Hk, D, window, sinks, max_len, q.device)
+    ws, nb = _parts(code, T, B, 0, H, Hk, D, window, sinks, max_len, q.device)
     _call(name, _native.lib().psq_paged_prompt_attention, code, q.data_ptr(), dt, q_token, q_head, k_cache.data_ptr(), v_cache.data_ptr(),
           ks, vs, pages, page, block_table.data_ptr(), block_table.stride(0), cols, starts.data_ptr(), lengths.data_ptr(), B, T, H, Hk, D,
           D ** -0.5 if scale is None else scale, window, sinks, max_len, out.data_ptr(), lse.data_ptr() if return_lse else None,
@@ -901,7 +901,7 @@ def paged_tree_attention(q, k_cache, v_cache, block_table, lengths, parents, k_s
     max_len = cols * page if max_len is None or max_len < 0 else min(int(max_len), cols * page)
     out = torch.empty((B, N, H, D), dtype=q.dtype, device=q.device)
     lse = torch.empty((B, N, H), dtype=torch.float32, device=q.device) if return_lse else None
-    ws, nb = _parts(B * N, B, N, H, Hk, D, window, sinks, max_len, q.device)
+    ws, nb = _parts(code, B * N, B, N, H, Hk, D, window, sinks, max_len, q.device)
     _call(name, _native.lib().psq_paged_tree_attention, code, q.data_ptr(), dt, q_token, q_head, k_cache.data_ptr(), v_cache.data_ptr(),
           ks, vs, pages, page, block_table.data_ptr(), block_table.stride(0), cols, lengths.data_ptr(), parents.data_ptr(),
           None if drafts is None else drafts.data_ptr(), B, N, H, Hk, D, D ** -0.5 if scale is None else scale, window, sinks, max_len,

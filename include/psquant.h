@@ -413,7 +413,7 @@ PSQ_API int psq_paged_attention_sinks(int codes, const void *q, int dtype, int64
  * workspace: NULL (no sequence is split over its length), or memory of the call's own (any contents; the call makes two
  * launches then, and nothing else may write to it in between) of psq_paged_block_workspace_bytes() bytes, 256-byte
  * aligned; 0 bytes: no use for one.  N: 0 here; T: B N for trees. */
-PSQ_API int64_t psq_paged_block_workspace_bytes(int64_t T, int64_t B, int N, int Hq, int Hkv, int D, int64_t window,
+PSQ_API int64_t psq_paged_block_workspace_bytes(int codes, int64_t T, int64_t B, int N, int Hq, int Hkv, int D, int64_t window,
                                         int64_t sinks, int64_t max_len);
 PSQ_API int psq_paged_prompt_attention(int codes, const void *q, int dtype, int64_t q_token, int64_t q_head,
                                const void *k_cache, const void *v_cache, const float *k_scale, const float *v_scale,
