@@ -131,14 +131,17 @@ struct Seq { int first, n, len, text, drafts; };
 __device__ __forceinline__ Seq sequence(const Args &a, int b)
 {
     Seq s{};
+    // (of a length far past the table no row sees less than one token there: a shorter one that does the same bounds
+    // the work, and sums of positions)
+    auto length = [&](int n) { return min(max(a.lengths[b], 0), a.cols * a.page + n + kKeys); };
     if (a.N) {
-        s.first = b * a.N, s.n = a.N, s.len = max(a.lengths[b], 0);
+        s.first = b * a.N, s.n = a.N, s.len = length(a.N);
         s.drafts = min(a.drafts ? min(max(a.drafts[b], 0), a.N) : a.N, s.len);
         s.text = s.len - s.drafts;
     } else {
         s.first = min(max(a.starts[b], 0), a.T);
         s.n = b == a.B ? a.T - s.first : min(max(a.starts[b + 1], s.first), a.T) - s.first;
-        s.len = b == a.B ? 0 : max(a.lengths[b], 0);
+        s.len = b == a.B ? 0 : length(s.n);
         s.text = s.len;
     }
     return s;
@@ -256,12 +259,20 @@ __device__ __forceinline__ uint32_t weight_of(const Args &a, int b)
     return s.n ? (uint32_t)row_tiles(a, s) * a.Hkv * key_tiles(a, s) : 0;
 }
 
-__device__ __forceinline__ Runs runs_of(const Args &a, int count)
+__device__ __forceinline__ Runs runs_of(const Args &a, uint32_t all)
 {
     Runs r;
-    r.all = sum_of(count, [&](int b) { return weight_of(a, b); });
+    r.all = all;
     r.runs = min((uint32_t)a.runs, max(r.all / (uint32_t)a.least, 1u));
     return r;
+}
+
+// weight(lane), the first 64 sequences'; where a batch has no more, its scans load nothing further
+template <class F>
+__device__ __forceinline__ uint32_t first_weights(int count, F weight)
+{
+    const int lane = threadIdx.x & 63;
+    return lane < count ? weight(lane) : 0;
 }
 
 // A part of a unit, or all of it: the key tiles first .. first + tiles - 1 of the sequence's list (runs), or the rows' own
@@ -865,21 +876,25 @@ block_attention_kernel(Args a)
     // ---- the workgroup's units
     const int count = a.N ? a.B : a.B + 1;
     int b, r0, first = 0, tiles = 0;       // key tiles first .. of the unit's list are the workgroup's
-    uint32_t hk, x = 0, end = 0;
-    Runs runs{};
+    uint32_t hk, x = 0, end = 0, kept = 0;
+    auto weight = [&](int b) { return weight_of(a, b); };
     if (!a.runs) {
         auto tiles_of = [&](int b) { return (uint32_t)row_tiles(a, sequence(a, b)); };
-        const uint32_t all = sum_of(count, tiles_of), units = all * a.Hkv;
+        const uint32_t kept = first_weights(count, tiles_of);
+        auto kept_of = [&](int b) { return b < 64 ? kept : tiles_of(b); };
+        const uint32_t all = sum_of(count, kept_of), units = all * a.Hkv;
         if (blockIdx.x >= units) return;
         // Workgroups of an XCD share a kv head's keys and values in its L2; the rows that see most go first.
         const uint32_t rank = (uint32_t)xcd_rank(blockIdx.x, units);
         hk = rank / all;
         uint32_t before;
         const uint32_t place = all - 1 - (rank - hk * all);
-        b = __builtin_amdgcn_readfirstlane(find(count, place, before, tiles_of));
+        b = __builtin_amdgcn_readfirstlane(find(count, place, before, kept_of));
+        if (b >= count) return;            // (only of starts that a caller may not give, as below)
         r0 = (int)(place - before) * a.rows;
     } else {
-        runs = runs_of(a, count);
+        kept = first_weights(count, weight);
+        const Runs runs = runs_of(a, sum_of(count, [&](int b) { return b < 64 ? kept : weight(b); }));
         const uint32_t w = (uint32_t)xcd_rank(blockIdx.x, a.runs);
         if (w >= runs.runs) return;
         x = runs.first(w), end = runs.first(w + 1);
@@ -889,10 +904,13 @@ block_attention_kernel(Args a)
     bool whole = true;
     if (a.runs) {
         uint32_t before;
-        b = __builtin_amdgcn_readfirstlane(find(count, x, before, [&](int b) { return weight_of(a, b); }));
+        b = __builtin_amdgcn_readfirstlane(find(count, x, before, [&](int b) { return b < 64 ? kept : weight(b); }));
+        if (b >= count) return;            // (this and the next too)
         const Seq s = sequence(a, b);
         const uint32_t each = (uint32_t)key_tiles(a, s), per = (uint32_t)row_tiles(a, s), unit = (x - before) / each;
-        hk = unit / per, r0 = (int)(unit - hk * per) * a.rows;
+        hk = unit / per;
+        if (hk >= (uint32_t)a.Hkv) return;
+        r0 = (int)(unit - hk * per) * a.rows;
         first = (int)(x - before - unit * each);
         tiles = (int)min(each - first, end - x);
         whole = tiles == (int)each;
@@ -915,6 +933,7 @@ block_attention_kernel(Args a)
         for (int i = 0; i < (int)(sizeof(Args) / 4); i++) words[i] = args[i];
         block_unit<DT, CODES, DD, PART, W, true>(__builtin_bit_cast(Args, words), lds, b, hk, r0, first, tiles, whole);
     }
+    if (x < end) kept = first_weights(count, weight);   // (not kept in a register through the unit)
     } while (x < end);
 }
 
@@ -926,16 +945,29 @@ join_kernel(Args a)
     constexpr int kJoin = 1024 / DD, U = 8;
     const int count = a.N ? a.B : a.B + 1;
     auto units_of = [&](int b) { return (uint32_t)row_tiles(a, sequence(a, b)) * a.Hkv; };
-    if (blockIdx.x >= sum_of(count, units_of)) return;
     uint32_t before;
-    const int b = __builtin_amdgcn_readfirstlane(find(count, blockIdx.x, before, units_of));
+    int b;
+    if (a.N) {                             // (as many units each, and a grid with no more)
+        const uint32_t units = (uint32_t)((a.N * a.G + a.rows - 1) / a.rows) * a.Hkv;
+        b = blockIdx.x / units, before = b * units;
+    } else {
+        if (blockIdx.x >= sum_of(count, units_of)) return;
+        b = __builtin_amdgcn_readfirstlane(find(count, blockIdx.x, before, units_of));
+    }
     const Seq s = sequence(a, b);
     const uint32_t unit = blockIdx.x - before, each = (uint32_t)key_tiles(a, s), per = (uint32_t)row_tiles(a, s), hk = unit / per;
     const int r0 = (int)(unit - hk * per) * a.rows, r = (int)blockIdx.y * kJoin + (threadIdx.x & (kJoin - 1)), quad = threadIdx.x / kJoin;
-    const Runs runs = runs_of(a, count);
-    const uint32_t x = sum_of(b, [&](int b) { return weight_of(a, b); }) + unit * each;
+    uint32_t front = 0;                    // key tiles of the sequences in front
+    const Runs runs = runs_of(a, sum_of(count, [&](int i) {
+        const uint32_t w = weight_of(a, i);
+        front += i < b ? w : 0;
+        return w;
+    }));
+#pragma unroll
+    for (int o = 32; o; o >>= 1) front += __shfl_xor(front, o, 64);
+    const uint32_t x = (uint32_t)__builtin_amdgcn_readfirstlane((int)front) + unit * each;
     const uint32_t w0 = runs.owner(x), parts = runs.owner(x + each - 1) - w0 + 1;
-    if (parts == 1 || r0 + r >= s.n * a.G || 4 * quad >= a.D) return;
+    if (parts == 1 || w0 + parts > (uint32_t)a.runs || r0 + r >= s.n * a.G || 4 * quad >= a.D) return;
     float M = -INFINITY, L = 0.0f;
     v4f acc = {0, 0, 0, 0};
     bool none = false;
@@ -992,7 +1024,8 @@ int launch(const Args &a, unsigned groups, hipStream_t st)
         raised[dev] = true;
     }
     kernel<<<a.runs ? a.runs : groups, 64 * W, lds, st>>>(a);
-    if (a.runs) join_kernel<DT, DD><<<dim3(groups, a.rows / (1024 / DD)), kThreads, 0, st>>>(a);
+    const int rows = a.N ? min(a.N * a.G, a.rows) : a.rows, join = 1024 / DD;
+    if (a.runs) join_kernel<DT, DD><<<dim3(groups, (rows + join - 1) / join), kThreads, 0, st>>>(a);
     return check_launch("block attention");
 }
 
