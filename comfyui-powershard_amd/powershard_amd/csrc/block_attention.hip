@@ -50,15 +50,32 @@ Plan plan(int codes, int64_t T, int64_t B, int N, int Hq, int Hkv, int D, int64_
 {
     Plan p{};
     const int64_t G = Hq / Hkv, each = (N ? N : T / std::max<int64_t>(B, 1)) * G;     // rows of a sequence and kv head
-    p.rows = D <= 128 && (codes != PSQ_CODES_NONE || each >= 512) ? 256 : 128;
+    // Codes are widened once per tile of keys, for twice as many rows (512 tokens on 64977, int8: 1257 us with 128, 1133 with
+    // 256).  16 bits, 40 heads on 8, bf16, 128 | 256 rows, us: 1024 tokens 41 | 47, 8192 684 | 698; of dims of 64, 16 heads:
+    // 1024 23 | 37, 8192 202 | 187 (256 never in front by more than 10%, so these have one form).
+    p.rows = D <= 128 && codes != PSQ_CODES_NONE ? 256 : 128;
     p.units = Hkv * (N ? B * ((N * G + p.rows - 1) / p.rows) : T * G / p.rows + B + 1);
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess) dev = 0;
-    const int64_t slots = (int64_t)cu_count(dev) * (D > 128 || p.rows == 256 ? 1 : 2);
-    // of a unit, at most: with a window those of its first row's to its last row's
-    int64_t tiles = (max_len + kKeys - 1) / kKeys;
-    if (window) tiles = std::min(tiles, (window + std::min<int64_t>(sinks, max_len) + p.rows / G) / kKeys + 3);
-    if (tiles <= 2 || p.units >= (tiles <= 16 ? slots / 2 : 2 * slots) || p.units * tiles > 0x7fffffffLL) return p;
+    const int64_t cus = cu_count(dev), slots = cus * (D > 128 || p.rows == 256 ? 1 : 2);
+    // Key tiles of a unit, at most, on average and at least, and of a sequence's list, which runs are cut from: a causal
+    // unit ends at its own last row, and a run's share counts tiles that its rows do not see.
+    const double tokens = (double)each / G, most_len = (double)max_len, rows_tokens = std::max((double)p.rows / G, 1.0);
+    const double list = window ? std::min(most_len, (double)window + sinks + tokens) / kKeys + 1 : most_len / kKeys;
+    const double most = window ? std::min(most_len, (double)window + sinks + rows_tokens) / kKeys + 1 : list;
+    const double cut = window || N ? 0 : std::min(tokens, most_len) / kKeys;
+    // Times in tile steps.  kBegin: to begin a unit (its queries, pages and first tiles), and as much again to write parts
+    // and join them.  Whole units: their share of a slot, the last round not full; no less than the longest.  Alone on a
+    // CU a workgroup takes 0.6 of the time that each of two takes.
+    // us, whole | runs (40 heads on 8, dims of 128, bf16): 512 tokens 29 | 57, 2048 82 | 143, 4096 231 | 364, 512 on 8192
+    // 223 | 131, trees of 16 on 300 17 | 27, 32 of them on 1000 43 | 53; int8: 2048 on 16384 1214 | 885, 8 x 256 on 4096
+    // 360 | 290, 128 on 1024 58 | 41, trees of 64 on 60000 2370 | 183.
+    constexpr double kBegin = 5;
+    const double units = (double)std::max<int64_t>(B, 1) * ((each + p.rows - 1) / p.rows) * Hkv, share = units / slots;
+    double whole = kBegin + most;
+    if (share > 1) whole = std::max(whole, share * (kBegin + most - cut / 2) + (std::ceil(share) - share) * (kBegin + most - cut));
+    else if (slots > cus && units <= cus) whole *= 0.6;
+    if (whole <= kBegin * (2 + share) + share * list || p.units * (list + 2) > 2147483647.0) return p;
     p.runs = slots;
     const int DD = D <= 64 ? 64 : D <= 128 ? 128 : 256;
     p.bytes = 2 * p.runs * part_floats(p.rows, DD) * 4;

@@ -3,10 +3,10 @@
 //
 //   s = scale (q . k_t) ks_t over the tokens t that the row sees,  p = softmax(s),  out = sum_t p_t vs_t v_t
 //
-// Rows are (token, head of a kv head's group): a tile of 128 rows of one sequence and kv head meets tiles of 64
-// keys, which a workgroup of 4 waves brings to LDS once for all of them, as 16-bit elements (codes are converted
-// on the way; they are exact in 16 bits).  A wave has 32 rows, one per lane in both halves (32x32x16 matrix
-// instructions, fp32 accumulation).  Lane l, n = l & 31, h = l >> 5:
+// Rows are (token, head of a kv head's group): a tile of 32 W rows of one sequence and kv head meets tiles of 64
+// keys, which the workgroup of W waves brings to LDS once for all of them, as 16-bit elements.  W is 4; 8 for codes of
+// at most 128 dims, which are loaded as they are and widened there (they are exact in 16 bits).  A wave has 32 rows, one
+// per lane in both halves (32x32x16 matrix instructions, fp32 accumulation).  Lane l, n = l & 31, h = l >> 5:
 //   S^T = K Q^T: the lane holds row n's scores of keys 8 (i >> 2) + 4 h + (i & 3), i < 16, of each 32 keys;
 //   O^T = V^T P^T: those probabilities are, as they are, the lane's part of P^T if contraction index 8 h + j of
 //     keys 16 u .. stands for key 16 u + 8 (j >> 2) + 4 h + (j & 3); the transposed LDS reads deliver V^T to match.
@@ -20,7 +20,16 @@
 // Many tiles of rows: a workgroup each, those with most keys first.  Few: the key tiles of all units (sequence, kv
 // head, tile of rows), in their order, are cut into equal runs, one per workgroup, as many as the chip holds: the
 // host needs no lengths.  A workgroup leaves its parts of cut units (two at most) in the workspace, and a second
-// kernel adds them up in their order.
+// kernel adds them up in their order.  plan() chooses, and has times of both.
+//
+// Tiles come by loads that go to LDS past the registers, some tiles ahead, in rings; the loop waits for them by count.
+// The scores of the next tile are worked out while the weights of this one are: matrix and vector instructions
+// alternate, each in the other's shadow, with one barrier a tile.  Bound by instruction issue, not by memory: the two
+// kinds fill 90% of a wave's cycles (per 32 rows x 64 keys x 128 dims 32 products of about 35 cycles and some 250
+// vector instructions).  Measured: 8191 tokens, 40 heads on 8 of 128, bf16, causal: 700 us, 980 TFLOP/s (a library
+// product of 16384^3: 1567); 512 tokens on 64977, int8: 1131 us, 605; 7 prompts with a window of 1024, f16: 514 us; trees
+// of 24 on 61 sequences of up to 4096, int8: 288 us.  Tried without gain: half the barriers, deeper rings, loads by one
+// wave, wave priorities, chains of products interleaved.
 //
 // Tiles that all rows of a wave see whole take no masks.  In the others a masked score is -inf whatever its key
 // holds.  A masked value would still poison a row if it were infinite or NaN (0 * inf): sums that come out NaN are
@@ -216,7 +225,7 @@ __device__ __forceinline__ void widen(const v4i &c, v4i (&w)[2])
 // DD: head dims that tiles are laid out for; W: waves of a workgroup; ES: bytes of a cached element.
 // Keys and values have rings of RK and RV buffers.  While a tile's weights meet its values, the next one's keys are read, and
 // loaded are the keys of the tile DK behind it and the values of that DV behind it.  A barrier comes every STEPS tiles
-// (two where the LDS holds eight buffers, for as many workgroups as the registers allow).
+// (two where the LDS holds eight buffers for two workgroups).
 // Codes (RAW) are loaded as they are, tiles up to RR behind, each by the wave that widens it later; wide heads' go
 // through registers.
 template <int DD, int W, int ES>
@@ -224,7 +233,7 @@ struct Layout {
     static constexpr bool RAW = ES == 1 && DD <= 128;
     static constexpr int PITCH = 2 * DD, TILE = kKeys * PITCH;          // bytes of a row, a tile
     static constexpr int BUFFER = TILE + (ES == 2 ? 0 : PITCH > 256 ? PITCH : 256);   // and its scales; whole rows
-    static constexpr int STEPS = ES == 2 && (DD == 64 || W == 8) ? 2 : 1;
+    static constexpr int STEPS = ES == 2 && DD == 64 ? 2 : 1;
     static constexpr int DK = STEPS + 1, DV = STEPS == 2 ? 2 : DD == 256 || ES == 1 ? 1 : 2;
     static constexpr int RK = STEPS == 2 ? 4 : 2, RV = STEPS == 2 ? 4 : DV + 1;
     static constexpr int RW = kKeys / W;                                // rows of a tile that a wave brings
@@ -1032,19 +1041,12 @@ int launch(const Args &a, unsigned groups, hipStream_t st)
 template <int DT, int CODES>
 int launch_dim(const Args &a, unsigned groups, hipStream_t st)
 {
-    if (a.rows == 256) {
-        if (a.D == 64) return launch<DT, CODES, 64, false, 8>(a, groups, st);
-        if (a.D == 128) return launch<DT, CODES, 128, false, 8>(a, groups, st);
-        if (a.D < 64) return launch<DT, CODES, 64, true, 8>(a, groups, st);
-        return launch<DT, CODES, 128, true, 8>(a, groups, st);
-    }
+    constexpr int W = CODES == PSQ_CODES_NONE ? 4 : 8;   // (as a.rows)
+    if (a.D == 64) return launch<DT, CODES, 64, false, W>(a, groups, st);
+    if (a.D == 128) return launch<DT, CODES, 128, false, W>(a, groups, st);
     if (a.D == 256) return launch<DT, CODES, 256, false, 4>(a, groups, st);
-    if constexpr (CODES == PSQ_CODES_NONE) {
-        if (a.D == 64) return launch<DT, CODES, 64, false, 4>(a, groups, st);
-        if (a.D == 128) return launch<DT, CODES, 128, false, 4>(a, groups, st);
-        if (a.D < 64) return launch<DT, CODES, 64, true, 4>(a, groups, st);
-        if (a.D < 128) return launch<DT, CODES, 128, true, 4>(a, groups, st);
-    }
+    if (a.D < 64) return launch<DT, CODES, 64, true, W>(a, groups, st);
+    if (a.D < 128) return launch<DT, CODES, 128, true, W>(a, groups, st);
     return launch<DT, CODES, 256, true, 4>(a, groups, st);
 }
 
