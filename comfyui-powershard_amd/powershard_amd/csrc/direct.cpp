@@ -27,6 +27,10 @@ decltype(&psq_kv_read) f_read;
 decltype(&psq_paged_attention_workspace_bytes) f_attend_bytes;
 decltype(&psq_paged_attention_own_workspace) f_attend_own;
 decltype(&psq_paged_attention_sinks) f_attend;
+decltype(&psq_rope_kv_write) f_rope;
+decltype(&psq_paged_block_workspace_bytes) f_block_bytes;
+decltype(&psq_paged_prompt_attention) f_prompt;
+decltype(&psq_paged_tree_attention) f_tree;
 
 // Other threads run while memory is allocated and the kernel is launched (a full queue makes the launch wait).
 struct Unlocked {
@@ -276,6 +280,122 @@ PyObject *attend(PyObject *, PyObject *const *o, Py_ssize_t n)
     });
 }
 
+// rope_kv_write(q, k, v, positions, inv_freq, slots, k_cache, v_cache, k_scale, v_scale, axes, interleaved, stream) -> q turned
+PyObject *rope(PyObject *, PyObject *const *o, Py_ssize_t n)
+{
+    return guarded([&]() -> PyObject * {
+        Arg q, k, v, positions, freq, slots, axes;
+        Pools p;
+        if (n != 13 || !f_rope || !take(o[0], -1, q) || !q.t) return none();
+        const int64_t index = q.t->get_device();
+        if (!take(o[1], index, k) || !k.t || !take(o[2], index, v) || !v.t || !take(o[3], index, positions) || !positions.t ||
+            !take(o[4], index, freq) || !freq.t || !take(o[5], index, slots) || !slots_of(slots) || !p.take_from(o + 6, index) || !take(o[10], index, axes))
+            return none();
+        const int paired = PyObject_IsTrue(o[11]);
+        void *stream = PyLong_AsVoidPtr(o[12]);
+        if (PyErr_Occurred()) {
+            PyErr_Clear();
+            return none();
+        }
+        const auto type = q.t->scalar_type(), count = positions.t->scalar_type();
+        const int dt = half_type(type);
+        if (dt < 0 || k.t->scalar_type() != type || v.t->scalar_type() != type || (!p.codes && p.k.t->scalar_type() != type) || !rows_of_heads(*q.t) ||
+            !rows_of_heads(*k.t) || !rows_of_heads(*v.t) || v.t->sizes() != k.t->sizes() || k.t->size(1) != p.heads || k.t->size(2) != p.dim)
+            return none();
+        const int64_t T = k.t->size(0), H = q.t->size(1);
+        if (q.t->size(0) != T || q.t->size(2) != p.dim || H > 0x7fffffff || slots.t->size(0) != T || freq.t->scalar_type() != at::kDouble ||
+            freq.t->dim() != 1 || !freq.t->is_contiguous())
+            return none();
+        const int64_t pairs = freq.t->size(0), dims = axes.t ? 2 : 1;
+        if (pairs <= 0 || 2 * pairs > p.dim || pairs % 8 || (count != at::kInt && count != at::kLong) || positions.t->dim() != dims ||
+            positions.t->size(dims - 1) != T || positions.t->stride(dims - 1) != 1)
+            return none();
+        if (axes.t && (axes.t->scalar_type() != at::kInt || axes.t->dim() != 1 || axes.t->size(0) != pairs || !axes.t->is_contiguous() ||
+                       positions.t->size(0) < 1 || positions.t->size(0) > 0x7fffffff))
+            return none();
+        at::Tensor out;
+        int status;
+        {
+            Unlocked unlocked;
+            out = at::empty({T, H, p.dim}, at::TensorOptions().device(q.t->device()).dtype(type));
+            status = f_rope(p.codes, q.t->data_ptr(), k.t->data_ptr(), v.t->data_ptr(), dt, q.t->stride(0), q.t->stride(1), k.t->stride(0),
+                            k.t->stride(1), v.t->stride(0), v.t->stride(1), positions.t->data_ptr(), count == at::kLong ? 64 : 32,
+                            axes.t ? (int)positions.t->size(0) : 1, axes.t ? positions.t->stride(0) : 0,
+                            axes.t ? (const int32_t *)axes.t->data_ptr() : nullptr, (const double *)freq.t->data_ptr(), (int)(2 * pairs), paired,
+                            (const int64_t *)slots.t->data_ptr(), T, (int)H, p.heads, p.dim, p.k.t->data_ptr(), p.v.t->data_ptr(), p.scale(p.ks),
+                            p.scale(p.vs), p.pages, (int)p.page, out.data_ptr(), stream);
+        }
+        return status ? none() : THPVariable_Wrap(out);
+    });
+}
+
+bool int32_of(const Arg &a, at::IntArrayRef sizes)
+{
+    return a.t && a.t->scalar_type() == at::kInt && a.t->sizes() == sizes && a.t->is_contiguous();
+}
+
+// paged_prompt_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, starts, None, scale, window, sinks,
+//                        max_len (None: the table's), return_lse, stream) -> out or (out, lse)
+// paged_tree_attention(q, ..., lengths, parents, drafts, scale, ...)
+template <bool TREE>
+PyObject *block(PyObject *, PyObject *const *o, Py_ssize_t n)
+{
+    return guarded([&]() -> PyObject * {
+        Arg q, table, lengths, rows, drafts;
+        Pools p;
+        if (n != 15 || !f_block_bytes || !f_prompt || !f_tree || !take(o[0], -1, q) || !q.t) return none();
+        const int64_t index = q.t->get_device();
+        if (!p.take_from(o + 1, index) || !take(o[5], index, table) || !table.t || !take(o[6], index, lengths) || !lengths.t ||
+            !take(o[7], index, rows) || !take(o[8], index, drafts))
+            return none();
+        const double scale = o[9] == Py_None ? 1 / std::sqrt((double)p.dim) : PyFloat_AsDouble(o[9]);
+        const long long window = PyLong_AsLongLong(o[10]), sinks = PyLong_AsLongLong(o[11]);
+        long long max_len = o[12] == Py_None ? -1 : PyLong_AsLongLong(o[12]);
+        const int want = PyObject_IsTrue(o[13]);
+        void *stream = PyLong_AsVoidPtr(o[14]);
+        if (PyErr_Occurred()) {
+            PyErr_Clear();
+            return none();
+        }
+        const auto type = q.t->scalar_type();
+        const int dt = half_type(type);
+        constexpr int at_heads = TREE ? 2 : 1;
+        if (dt < 0 || (!p.codes && p.k.t->scalar_type() != type) || q.t->dim() != at_heads + 2 || lengths.t->dim() != 1 || p.heads <= 0 || !aligned(*q.t))
+            return none();
+        const int64_t B = lengths.t->size(0), H = q.t->size(at_heads), N = TREE ? q.t->size(1) : 0, T = TREE ? B * N : q.t->size(0);
+        const int64_t token = q.t->stride(at_heads - 1), head = q.t->stride(at_heads);
+        if (q.t->size(at_heads + 1) != p.dim || q.t->stride(at_heads + 1) != 1 || ((token | head) & 7) || H > 0x7fffffff || H % p.heads || N > 64 ||
+            (TREE && (q.t->size(0) != B || (B > 1 && q.t->stride(0) != N * token))) || !int32_of(lengths, {B}) || table.t->scalar_type() != at::kInt ||
+            table.t->dim() != 2 || table.t->size(0) != B || (table.t->size(1) > 1 && table.t->stride(1) != 1) || window < 0 || sinks < 0 ||
+            (sinks && !window) || (TREE ? !int32_of(rows, {B, N}) : !int32_of(rows, {B + 1})) || (drafts.t && (!TREE || !int32_of(drafts, {B}))))
+            return none();
+        const int64_t cols = table.t->size(1);
+        if (max_len < 0 || max_len > cols * p.page) max_len = cols * p.page;
+        const int64_t need = f_block_bytes(p.codes, T, B, (int)N, (int)H, p.heads, p.dim, window, sinks, max_len);
+        const auto opt = at::TensorOptions().device(q.t->device());
+        at::Tensor out, lse, parts;
+        int status;
+        {
+            Unlocked unlocked;
+            if (need > 0) parts = at::empty({need}, opt.dtype(at::kByte));
+            out = at::empty(q.t->sizes(), opt.dtype(type));
+            if (want) lse = at::empty(q.t->sizes().slice(0, at_heads + 1), opt.dtype(at::kFloat));
+            void *ws = need > 0 ? parts.data_ptr() : nullptr;
+            float *sums = want ? (float *)lse.data_ptr() : nullptr;
+            const auto *pages = (const int32_t *)table.t->data_ptr(), *n = (const int32_t *)lengths.t->data_ptr(), *more = (const int32_t *)rows.t->data_ptr();
+            if constexpr (TREE)
+                status = f_tree(p.codes, q.t->data_ptr(), dt, token, head, p.k.t->data_ptr(), p.v.t->data_ptr(), p.scale(p.ks), p.scale(p.vs), p.pages,
+                                (int)p.page, pages, table.t->stride(0), cols, n, more, drafts.t ? (const int32_t *)drafts.t->data_ptr() : nullptr, B,
+                                (int)N, (int)H, p.heads, p.dim, (float)scale, window, sinks, max_len, out.data_ptr(), sums, ws, need, stream);
+            else
+                status = f_prompt(p.codes, q.t->data_ptr(), dt, token, head, p.k.t->data_ptr(), p.v.t->data_ptr(), p.scale(p.ks), p.scale(p.vs),
+                                  p.pages, (int)p.page, pages, table.t->stride(0), cols, more, n, B, T, (int)H, p.heads, p.dim, (float)scale, window,
+                                  sinks, max_len, out.data_ptr(), sums, ws, need, stream);
+        }
+        return status ? none() : want ? tuple(out, lse) : THPVariable_Wrap(out);
+    });
+}
+
 // bind({name: address})
 PyObject *bind(PyObject *, PyObject *d)
 {
@@ -289,6 +409,10 @@ PyObject *bind(PyObject *, PyObject *d)
     f_attend_bytes = (decltype(f_attend_bytes))at("psq_paged_attention_workspace_bytes");
     f_attend_own = (decltype(f_attend_own))at("psq_paged_attention_own_workspace");
     f_attend = (decltype(f_attend))at("psq_paged_attention_sinks");
+    f_rope = (decltype(f_rope))at("psq_rope_kv_write");
+    f_block_bytes = (decltype(f_block_bytes))at("psq_paged_block_workspace_bytes");
+    f_prompt = (decltype(f_prompt))at("psq_paged_prompt_attention");
+    f_tree = (decltype(f_tree))at("psq_paged_tree_attention");
     if (PyErr_Occurred()) return nullptr;
     Py_RETURN_NONE;
 }
@@ -299,6 +423,9 @@ PyMethodDef methods[] = {
     {"kv_write", (PyCFunction)(void (*)(void))kv_write, METH_FASTCALL, nullptr},
     {"kv_read", (PyCFunction)(void (*)(void))kv_read, METH_FASTCALL, nullptr},
     {"paged_attention", (PyCFunction)(void (*)(void))attend, METH_FASTCALL, nullptr},
+    {"rope_kv_write", (PyCFunction)(void (*)(void))rope, METH_FASTCALL, nullptr},
+    {"paged_prompt_attention", (PyCFunction)(void (*)(void))block<false>, METH_FASTCALL, nullptr},
+    {"paged_tree_attention", (PyCFunction)(void (*)(void))block<true>, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

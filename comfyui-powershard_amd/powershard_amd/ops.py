@@ -686,6 +686,10 @@ def rope_kv_write(q, k, v, positions, inv_freq, slots, k_cache, v_cache, k_scale
     fp64; keys are turned in fp32 and quantized from there.
     """
     index = q.get_device()
+    if index >= 0 and _timer is None and (direct := _native.direct()):
+        done = direct.rope_kv_write(q, k, v, positions, inv_freq, slots, k_cache, v_cache, k_scale, v_scale, axes, interleaved, _raw(index))
+        if done is not None:
+            return done
     code, (pages, H, page, D), ks, vs = _pools("rope_kv_write", index, k_cache, v_cache, k_scale, v_scale)
     for t in (k, v, positions, inv_freq) + (() if axes is None else (axes,)):
         if t.get_device() != index:
@@ -852,6 +856,11 @@ def paged_prompt_attention(q, k_cache, v_cache, block_table, starts, lengths, k_
     in paged_attention.
     A row that sees a token whose page is outside the pool, or past the table, gets NaN.
     """
+    if (index := q.get_device()) >= 0 and _timer is None and (direct := _native.direct()):
+        done = direct.paged_prompt_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, starts, None, scale, window, sinks,
+                                          max_len, return_lse, _raw(index))
+        if done is not None:
+            return done
     name = "paged_prompt_attention"
     index, code, dt, (pages, Hk, page, D), ks, vs, block_table, lengths = _rows_on_cache(
         name, q, 1, k_cache, v_cache, block_table, lengths, k_scale, v_scale, window, sinks, starts)
@@ -883,6 +892,11 @@ def paged_tree_attention(q, k_cache, v_cache, block_table, lengths, parents, k_s
     way from there and itself.  Its position is the text's length plus the number of drafts in front of it on its way;
     window and sinks count positions.  The rest as in paged_prompt_attention (lse [batch, n, heads]).
     """
+    if (index := q.get_device()) >= 0 and _timer is None and (direct := _native.direct()):
+        done = direct.paged_tree_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, parents, drafts, scale, window, sinks,
+                                         max_len, return_lse, _raw(index))
+        if done is not None:
+            return done
     name = "paged_tree_attention"
     index, code, dt, (pages, Hk, page, D), ks, vs, block_table, lengths = _rows_on_cache(
         name, q, 2, k_cache, v_cache, block_table, lengths, k_scale, v_scale, window, sinks, parents, *(() if drafts is None else (drafts,)))
