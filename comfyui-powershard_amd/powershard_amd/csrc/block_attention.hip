@@ -46,6 +46,8 @@ int check(const char *name, Args &a, int codes, const void *q, int dtype, int64_
 // tiles are cut into (0: they stay whole).
 struct Plan { int rows; int64_t units, runs, bytes; };
 
+constexpr int kLeast = 2;    // key tiles of a run (twice as many: a tree of 24 on 8 x 1000, int8, 39 us with either, 8: 46)
+
 Plan plan(int codes, int64_t T, int64_t B, int N, int Hq, int Hkv, int D, int64_t window, int64_t sinks, int64_t max_len)
 {
     Plan p{};
@@ -76,7 +78,11 @@ Plan plan(int codes, int64_t T, int64_t B, int N, int Hq, int Hkv, int D, int64_
     if (share > 1) whole = std::max(whole, share * (kBegin + most - cut / 2) + (std::ceil(share) - share) * (kBegin + most - cut));
     else if (slots > cus && units <= cus) whole *= 0.6;
     if (whole <= kBegin * (2 + share) + share * list || p.units * (list + 2) > 2147483647.0) return p;
-    p.runs = slots;
+    // A run that goes on with a second unit begins anew.  Where units of that length cut into equal parts make no longer runs
+    // than that costs, there are as many runs as parts, and with equal lengths each is of one unit (40 heads on 8, bf16: a
+    // tree of 16 on 4000 43.7 -> 27.5 us, of 16 on 1000 30 -> 20, 256 tokens on 3000 64 -> 49, 512 on 8192 131 -> 122).
+    const double parts = std::floor(std::min(1 / share, list / kLeast));
+    p.runs = parts >= 1 && list / parts <= share * list + kBegin ? (int64_t)(units * parts) : slots;
     const int DD = D <= 64 ? 64 : D <= 128 ? 128 : 256;
     p.bytes = 2 * p.runs * part_floats(p.rows, DD) * 4;
     return p;
@@ -87,7 +93,7 @@ int run(int codes, int dtype, Args &a, const Plan &p, void *workspace, int64_t w
     if (int e = require_device()) return e;
     const unsigned g = (unsigned)p.units;
     a.rows = p.rows;
-    if (p.runs && workspace && workspace_bytes >= p.bytes) a.runs = (int)p.runs, a.least = 2, a.part = (float *)workspace;
+    if (p.runs && workspace && workspace_bytes >= p.bytes) a.runs = (int)p.runs, a.least = kLeast, a.part = (float *)workspace;
     if (codes == PSQ_CODES_I8) return dtype == PSQ_BF16 ? launch_bf16_i8(a, g, st) : launch_f16_i8(a, g, st);
     if (codes == PSQ_CODES_E4M3) return dtype == PSQ_BF16 ? launch_bf16_fp8(a, g, st) : launch_f16_fp8(a, g, st);
     return dtype == PSQ_BF16 ? launch_bf16(a, g, st) : launch_f16(a, g, st);
