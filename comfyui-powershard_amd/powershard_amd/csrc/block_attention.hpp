@@ -26,10 +26,10 @@
 // The scores of the next tile are worked out while the weights of this one are: matrix and vector instructions
 // alternate, each in the other's shadow, with one barrier a tile.  Bound by instruction issue, not by memory: the two
 // kinds fill 90% of a wave's cycles (per 32 rows x 64 keys x 128 dims 32 products of about 35 cycles and some 250
-// vector instructions).  Measured: 8191 tokens, 40 heads on 8 of 128, bf16, causal: 700 us, 980 TFLOP/s (a library
-// product of 16384^3: 1567); 512 tokens on 64977, int8: 1131 us, 605; 7 prompts with a window of 1024, f16: 514 us; trees
-// of 24 on 61 sequences of up to 4096, int8: 288 us.  Tried without gain: half the barriers, deeper rings, loads by one
-// wave, wave priorities, chains of products interleaved.
+// vector instructions).  Measured: 8191 tokens, 40 heads on 8 of 128, bf16, causal: 690 to 735 us on several cards,
+// 930 to 1000 TFLOP/s (a library product of 16384^3: 1567); 512 tokens on 64977, int8: 1133 us, 605; 7 prompts with a
+// window of 1024, f16, dims of 64: 514 us, 515; trees of 24 on 61 sequences of up to 4096, int8: 288 us; a tree of 16 on 4000: 28.
+// Tried without gain: half the barriers, deeper rings, loads by one wave, wave priorities, chains of products interleaved.
 //
 // Tiles that all rows of a wave see whole take no masks.  In the others a masked score is -inf whatever its key
 // holds.  A masked value would still poison a row if it were infinite or NaN (0 * inf): sums that come out NaN are

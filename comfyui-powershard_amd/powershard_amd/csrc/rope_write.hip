@@ -4,6 +4,8 @@
 //   t = position[axis(i)] f_i;  a' = a cos t - b sin t,  b' = b cos t + a sin t  for pair i = (a, b)
 //   q: rounded to its type; k, v: codes and scales as in kv_cache.hip, k's from the turned values in fp32
 // Bound by memory: queries 2 bytes in and 2 out per element, keys and values 2 in and 1 or 2 out.
+// 8191 tokens, 40 heads on 8 of 128, e4m3, with the read-back: 60.8 us, 4.4 TB/s (a large copy: 4.75); 4095 tokens, 64 heads on 16
+// of 64, three axes, f16, likewise: 30.2 us, 4.45 TB/s; one token: 11.5 us for both calls, the host's part.
 // A lane has 16 elements of a row: its 8 pairs, where it turns (the two pieces of 8 elements that are half
 // the rotary dims apart, or 16 neighbours where pairs are neighbours), else 16 neighbours.  A row is the
 // D / 16 lanes next to each other.  The angles of a workgroup's tokens are worked out once, into LDS, and all heads'
