@@ -75,8 +75,8 @@ SIGNATURES = {
 }
 
 DIRECT_CALLS = ("psq_add_rms_norm", "psq_kv_write", "psq_kv_read", "psq_paged_attention_workspace_bytes",
-                "psq_paged_attention_own_workspace", "psq_paged_attention_sinks", "psq_rope_kv_write", "psq_paged_block_workspace_bytes",
-                "psq_paged_prompt_attention", "psq_paged_tree_attention")
+                "psq_paged_attention_own_workspace", "psq_paged_attention", "psq_paged_attention_sinks",
+                "psq_rope_kv_write", "psq_paged_block_workspace_bytes", "psq_paged_prompt_attention", "psq_paged_tree_attention")
 
 
 class NativeLibraryError(ImportError):

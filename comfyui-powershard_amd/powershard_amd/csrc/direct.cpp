@@ -28,7 +28,8 @@ decltype(&psq_kv_write) f_write;
 decltype(&psq_kv_read) f_read;
 decltype(&psq_paged_attention_workspace_bytes) f_attend_bytes;
 decltype(&psq_paged_attention_own_workspace) f_attend_own;
-decltype(&psq_paged_attention_sinks) f_attend;
+decltype(&psq_paged_attention) f_attend;
+decltype(&psq_paged_attention_sinks) f_attend_sinks;
 decltype(&psq_rope_kv_write) f_rope;
 decltype(&psq_paged_block_workspace_bytes) f_block_bytes;
 decltype(&psq_paged_prompt_attention) f_prompt;
@@ -237,7 +238,7 @@ PyObject *attend(PyObject *, PyObject *const *o, Py_ssize_t n)
     return guarded([&]() -> PyObject * {
         Arg q, table, lengths, ws;
         Pools p;
-        if ((n != 13 && n != 14) || !f_attend || !f_attend_bytes || !f_attend_own || !take(o[0], -1, q) || !q.t) return none();
+        if ((n != 13 && n != 14) || !f_attend || !f_attend_sinks || !f_attend_bytes || !f_attend_own || !take(o[0], -1, q) || !q.t) return none();
         const int64_t index = q.t->get_device();
         if (!p.take_from(o + 1, index) || !take(o[5], index, table) || !table.t || !take(o[6], index, lengths) || !lengths.t || !take(o[11], index, ws))
             return none();
@@ -272,11 +273,18 @@ PyObject *attend(PyObject *, PyObject *const *o, Py_ssize_t n)
             const at::Tensor *work = own ? &parts : ws.t;
             out = at::empty({B, H, p.dim}, opt.dtype(q.t->scalar_type()));
             if (want) lse = at::empty({B, H}, opt.dtype(at::kFloat));
-            status = f_attend(p.codes, q.t->data_ptr(), dt, q.t->stride(0), q.t->stride(1), p.k.t->data_ptr(), p.v.t->data_ptr(), p.scale(p.ks),
-                              p.scale(p.vs), p.pages, (int)p.page, (const int32_t *)table.t->data_ptr(), table.t->stride(0), cols,
-                              (const int32_t *)lengths.t->data_ptr(), B, (int)H, p.heads, p.dim, (float)scale, window, sinks, max_len, out.data_ptr(),
-                              want ? (float *)lse.data_ptr() : nullptr, need > 0 ? work->data_ptr() : nullptr, need > 0 ? work->numel() : 0,
-                              stream);
+            auto *sums = want ? (float *)lse.data_ptr() : nullptr;
+            auto *memory = need > 0 ? work->data_ptr() : nullptr;
+            const int64_t bytes = need > 0 ? work->numel() : 0;
+            const auto *pages = (const int32_t *)table.t->data_ptr(), *tokens = (const int32_t *)lengths.t->data_ptr();
+            if (sinks)
+                status = f_attend_sinks(p.codes, q.t->data_ptr(), dt, q.t->stride(0), q.t->stride(1), p.k.t->data_ptr(), p.v.t->data_ptr(),
+                                        p.scale(p.ks), p.scale(p.vs), p.pages, (int)p.page, pages, table.t->stride(0), cols, tokens, B, (int)H,
+                                        p.heads, p.dim, (float)scale, window, sinks, max_len, out.data_ptr(), sums, memory, bytes, stream);
+            else
+                status = f_attend(p.codes, q.t->data_ptr(), dt, q.t->stride(0), q.t->stride(1), p.k.t->data_ptr(), p.v.t->data_ptr(),
+                                  p.scale(p.ks), p.scale(p.vs), p.pages, (int)p.page, pages, table.t->stride(0), cols, tokens, B, (int)H, p.heads,
+                                  p.dim, (float)scale, window, max_len, out.data_ptr(), sums, memory, bytes, stream);
         }
         return status ? none() : want ? tuple(out, lse) : THPVariable_Wrap(out);
     });
@@ -410,7 +418,8 @@ PyObject *bind(PyObject *, PyObject *d)
     f_read = (decltype(f_read))at("psq_kv_read");
     f_attend_bytes = (decltype(f_attend_bytes))at("psq_paged_attention_workspace_bytes");
     f_attend_own = (decltype(f_attend_own))at("psq_paged_attention_own_workspace");
-    f_attend = (decltype(f_attend))at("psq_paged_attention_sinks");
+    f_attend = (decltype(f_attend))at("psq_paged_attention");
+    f_attend_sinks = (decltype(f_attend_sinks))at("psq_paged_attention_sinks");
     f_rope = (decltype(f_rope))at("psq_rope_kv_write");
     f_block_bytes = (decltype(f_block_bytes))at("psq_paged_block_workspace_bytes");
     f_prompt = (decltype(f_prompt))at("psq_paged_prompt_attention");

@@ -808,10 +808,10 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, k_scale=None, v_s
         ws = torch.empty(nb, dtype=torch.uint8, device=device)   # two launches: the call's own
     else:
         ws, nb = _workspace(device, raw or None, nb)
-    _call("paged_attention", lib.psq_paged_attention_sinks, code, q.data_ptr(), dt, q_batch, q_head, k_cache.data_ptr(),
-          v_cache.data_ptr(), ks, vs, pages, page, block_table.data_ptr(), block_table.stride(0), cols, lengths.data_ptr(), B, H,
-          Hk, D, D ** -0.5 if scale is None else scale, window, sinks, max_len, out.data_ptr(), lse.data_ptr() if return_lse else None,
-          None if ws is None else ws.data_ptr(), nb, raw)
+    _call("paged_attention", lib.psq_paged_attention_sinks if sinks else lib.psq_paged_attention, code, q.data_ptr(), dt, q_batch,
+          q_head, k_cache.data_ptr(), v_cache.data_ptr(), ks, vs, pages, page, block_table.data_ptr(), block_table.stride(0), cols,
+          lengths.data_ptr(), B, H, Hk, D, D ** -0.5 if scale is None else scale, window, *((sinks,) if sinks else ()), max_len, out.data_ptr(),
+          lse.data_ptr() if return_lse else None, None if ws is None else ws.data_ptr(), nb, raw)
     return (out, lse) if return_lse else out
 
 
