@@ -330,3 +330,31 @@ def test_lengths_past_the_table(gpu, codes, dtype, far, new):
     lengths[0] = 325                       # the last five tokens past the table, the twenty in front of them NaN in the cache
     got = ops.paged_prompt_attention(q, k, v, table, starts, lengths, ks, vs)
     assert got[max(new - 25, 0):new].isnan().all() and not got[:max(new - 25, 0)].isnan().any()
+
+
+@pytest.mark.parametrize("codes", [torch.bfloat16, torch.int8])
+def test_pools_past_4_gib(gpu, codes):
+    """Pages whose bytes lie past 2^32: the bits of the same pages at the pool's start."""
+    from powershard_amd import ops
+    H, Hk, D, page, n = 8, 8, 128, 64, 9
+    pages = 2 ** 33 // (Hk * page * D * codes.itemsize) // 2 * 9 // 8        # 4.5 GiB
+    g = torch.Generator(device=gpu).manual_seed(3)
+    small = [torch.zeros(n, Hk, page, D, dtype=codes, device=gpu) for _ in range(2)]
+    small += [None, None] if codes is torch.bfloat16 else [torch.ones(n, Hk, page, device=gpu) for _ in range(2)]
+    large = [t if t is None else torch.empty((pages,) + t.shape[1:], dtype=t.dtype, device=gpu) for t in small]
+    q, k, v = (torch.randn(n * page, h, D, generator=g, device=gpu).bfloat16() for h in (H, Hk, Hk))
+    at, freq = torch.arange(n * page, dtype=torch.int32, device=gpu), 100.0 ** (-torch.arange(64, device=gpu).double() / 64)
+    table = torch.randperm(n, generator=g, device=gpu)[None].int()
+    slots = table[0].long().repeat_interleave(page) * page + torch.arange(page, device=gpu).repeat(n)
+    lengths, starts = (torch.tensor(x, dtype=torch.int32, device=gpu) for x in ([n * page], [0, 100]))
+    parents = torch.arange(-1, 15, dtype=torch.int32, device=gpu)[None]
+    got = []
+    for pools, first in ((small, 0), (large, pages - n)):
+        turned = ops.rope_kv_write(q, k, v, at, freq, slots + first * page, *pools)
+        where = table + first
+        got.append([turned, *ops.kv_read(slots + first * page, *pools),
+                    ops.paged_prompt_attention(turned[-100:], *pools[:2], where, starts, lengths, *pools[2:]),
+                    ops.paged_tree_attention(turned[-16:][None], *pools[:2], where, lengths, parents, *pools[2:]),
+                    ops.paged_attention(turned[-1:], *pools[:2], where, lengths, *pools[2:], window=100, sinks=70)])
+    for a, b in zip(*got):
+        assert torch.equal(a, b) and not a.isnan().any()
