@@ -51,7 +51,9 @@ constexpr int kLeast = 2;    // key tiles of a run (twice as many: a tree of 24 
 Plan plan(int codes, int64_t T, int64_t B, int N, int Hq, int Hkv, int D, int64_t window, int64_t sinks, int64_t max_len)
 {
     Plan p{};
-    const int64_t G = Hq / Hkv, each = (N ? N : T / std::max<int64_t>(B, 1)) * G;     // rows of a sequence and kv head
+    // Sequences that have rows: of fewer rows than sequences some have none.  Rows of one and a kv head, on average and rounded
+    // up: with rows there is a unit.
+    const int64_t G = Hq / Hkv, some = std::max<int64_t>(N ? B : std::min(B, T), 1), each = (N ? N : (T + some - 1) / some) * G;
     // Codes are widened once per tile of keys, for twice as many rows (512 tokens on 64977, int8: 1257 us with 128, 1133 with
     // 256).  16 bits, 40 heads on 8, bf16, 128 | 256 rows, us: 1024 tokens 41 | 47, 8192 684 | 698; of dims of 64, 16 heads:
     // 1024 23 | 37, 8192 202 | 187 (256 never in front by more than 10%, so these have one form).
@@ -73,7 +75,7 @@ Plan plan(int codes, int64_t T, int64_t B, int N, int Hq, int Hkv, int D, int64_
     // 223 | 131, trees of 16 on 300 17 | 27, 32 of them on 1000 43 | 53; int8: 2048 on 16384 1214 | 885, 8 x 256 on 4096
     // 360 | 290, 128 on 1024 58 | 41, trees of 64 on 60000 2370 | 183.
     constexpr double kBegin = 5;
-    const double units = (double)std::max<int64_t>(B, 1) * ((each + p.rows - 1) / p.rows) * Hkv, share = units / slots;
+    const double units = (double)some * ((each + p.rows - 1) / p.rows) * Hkv, share = units / slots;
     double whole = kBegin + most;
     if (share > 1) whole = std::max(whole, share * (kBegin + most - cut / 2) + (std::ceil(share) - share) * (kBegin + most - cut));
     else if (slots > cus && units <= cus) whole *= 0.6;
