@@ -598,7 +598,13 @@ __device__ __forceinline__ bool block_unit(const Args &a, uint32_t lds, int b, u
             }
             const uint32_t p = pack_half2<PVT>(x, y);
             ph[Q / 4][Q & 3] = (int)p;
-            if constexpr (PAIR) pl[Q / 4][Q & 3] = (int)pack_half2<PVT>(x - half_to_f32<PVT>(p), y - half_to_f32<PVT>(p >> 16));
+            if constexpr (PAIR) {
+                const float hx = half_to_f32<PVT>(p), hy = half_to_f32<PVT>(p >> 16);
+                x -= hx, y -= hy;
+                if (CAREFUL && fabsf(hx) == INFINITY) x = 0.0f;              // (nothing is left of an infinite one)
+                if (CAREFUL && fabsf(hy) == INFINITY) y = 0.0f;
+                pl[Q / 4][Q & 3] = (int)pack_half2<PVT>(x, y);
+            }
         };
         // A slot is a matrix instruction, the LDS read of the one AHEAD slots later, and what vector work it covers:
         // vector and matrix units work at the same time only where the instructions of both take turns (two
