@@ -28,6 +28,9 @@ int check(const char *name, Args &a, int codes, const void *q, int dtype, int64_
         return set_error(PSQ_E_SHAPE, "%s: %lld sequences of %lld pages are too many", name, (long long)B, (long long)table_cols);
     // (a rows' number, and that of a workgroup, in 31 bits)
     if (T > 0x3fffffffLL / Hq) return set_error(PSQ_E_SHAPE, "%s: %lld tokens of %d heads are too many", name, (long long)T, Hq);
+    // (a length past the table counts as the table's and the rows', and a tile or two: in 31 bits)
+    if (table_cols * page_size + T > 0x7fffff00LL)
+        return set_error(PSQ_E_SHAPE, "%s: %lld tokens on a table of %lld are too many", name, (long long)T, (long long)(table_cols * page_size));
     if ((uintptr_t)workspace & 255) return set_error(PSQ_E_SHAPE, "%s: the workspace must be 256-byte aligned", name);
     a.q = (const uint16_t *)q, a.q_token = q_token, a.q_head = q_head;
     a.kc = (const uint8_t *)k_cache, a.vc = (const uint8_t *)v_cache, a.ks = k_scale, a.vs = v_scale;
