@@ -1,6 +1,7 @@
 // block_attention.hip -- the entry points of the attention of prompts and of trees of drafts over the paged
 // cache (the kernel is in block_attention.hpp): checks of arguments, and the launch.
 #include "block_attention.hpp"
+#include "block_plan.hpp"
 
 namespace psq {
 namespace block {
@@ -98,7 +99,8 @@ int run(int codes, int dtype, Args &a, const Plan &p, void *workspace, int64_t w
     if (int e = require_device()) return e;
     const unsigned g = (unsigned)p.units;
     a.rows = p.rows;
-    if (p.runs && workspace && workspace_bytes >= p.bytes) a.runs = (int)p.runs, a.least = kLeast, a.part = (float *)workspace;
+    if (p.runs && workspace && workspace_bytes >= p.bytes && sums_fit(p.units, (int64_t)a.cols * a.page, a.N ? a.N : a.T, a.window, a.sinks, kKeys))
+        a.runs = (int)p.runs, a.least = kLeast, a.part = (float *)workspace;
     if (codes == PSQ_CODES_I8) return dtype == PSQ_BF16 ? launch_bf16_i8(a, g, st) : launch_f16_i8(a, g, st);
     if (codes == PSQ_CODES_E4M3) return dtype == PSQ_BF16 ? launch_bf16_fp8(a, g, st) : launch_f16_fp8(a, g, st);
     return dtype == PSQ_BF16 ? launch_bf16(a, g, st) : launch_f16(a, g, st);
