@@ -14,8 +14,13 @@
 //
 // Statistics are fp32.  The maximum that scores are taken off is raised only when a row's has grown by 2^8 since
 // (a raise multiplies the row's whole output); probabilities are at most 2^8 then, held 2^7 times as large in f16.
-// A probability enters the second product as one 16-bit number (off by half a step, as the output is), with f16
-// rows on codes, whose values are bf16, as the sum of two.
+// A probability enters the second product as one 16-bit number, off by half a step as the output is (bf16 2^-8, f16 2^-11; on
+// codes times its value's scale, in bf16): an output is off by 1.1 to 1.4 times its rounding alone (relative root
+// mean square against 64 bits: bf16 0.0017 -> 0.0018 to 0.0023, f16 0.00021 -> 0.00027).  A second number for the rest
+// makes 48 products of 32 and some 100 more vector instructions a tile (us, one | two: 8191 tokens bf16 760 | 996, the f16
+// window 548 | 697, 512 on 64977 bf16 on int8 916 | 1164, trees of 24 on int8 289 | 322, of 64 on e4m3 361 | 435).  f16 rows on
+// codes, whose values are bf16, have it: one bf16 number would be off by 8 times their output's half step.  So has the
+// one-token kernel, which waits for memory, for all types.
 //
 // Many tiles of rows: a workgroup each, those with most keys first.  Few: the key tiles of all units (sequence, kv
 // head, tile of rows), in their order, are cut into equal runs, one per workgroup, as many as the chip holds: the
@@ -24,11 +29,17 @@
 //
 // Tiles come by loads that go to LDS past the registers, some tiles ahead, in rings; the loop waits for them by count.
 // The scores of the next tile are worked out while the weights of this one are: matrix and vector instructions
-// alternate, each in the other's shadow, with one barrier a tile.  Bound by instruction issue, not by memory: the two
-// kinds fill 90% of a wave's cycles (per 32 rows x 64 keys x 128 dims 32 products of about 35 cycles and some 250
-// vector instructions).  Measured: 8191 tokens, 40 heads on 8 of 128, bf16, causal: 690 to 735 us on several cards,
-// 930 to 1000 TFLOP/s (a library product of 16384^3: 1567); 512 tokens on 64977, int8: 1133 us, 605; 7 prompts with a
-// window of 1024, f16, dims of 64: 514 us, 515; trees of 24 on 61 sequences of up to 4096, int8: 288 us; a tree of 16 on 4000: 28.
+// alternate in one stream, with one barrier a tile.  Bound by the two kinds in turn, not by memory: of a SIMD's cycles the matrix
+// unit is busy for 49% and the vector unit for 49% (8191 tokens, bf16; dims of 64, f16 26% and 63%; f16 on int8 40% and
+// 56%), so what one wave does in the other's shadow is little, although two share a SIMD.  Per 32 rows x 64 keys x
+// 128 dims, 16 bits, beside 32 products of 32 cycles: 155 vector instructions, 32 of them exponentials (188 with what comes
+// in front of the loop and behind it), and 107 scalar ones.  Measured: 8191 tokens, 40 heads on 8 of 128, bf16, causal: 690
+// to 750 us on several cards, 915 to 1000 TFLOP/s (a library product of 16384^3: 1567); 512 tokens on 64977, f16 on int8:
+// 1128 us, 608; 7 prompts with a window of 1024, f16, dims of 64: 519 us, 510; trees of 24 on 61 sequences of up to 4096,
+// int8: 288 us; a tree of 16 on 4000: 28.
+// The loop has no registers to spare (256 a lane, 512 for dims above 128).  A tile step reloads from scratch, and waits with that
+// for all loads before: nothing on 16 bits up to dims of 64, and for bf16 rows on codes above that up to 128; 1 to 3 words
+// for the other types up to 128; above, 1 to 8 on 16 bits and 14 to 20 on codes.
 // Tried without gain: half the barriers, deeper rings, loads by one wave, wave priorities, chains of products interleaved.
 //
 // Tiles that all rows of a wave see whole take no masks.  In the others a masked score is -inf whatever its key

@@ -79,7 +79,11 @@ class DecoderLayer(nn.Module):
 
     heads, kv_heads, head_dim: of the attention; mlp: hidden features of the gated MLP (up_proj holds the
     gate's rows, then the up rows); rotary: a Rotary, which layers may share; window, sinks: a token sees the last
-    `window` (0: all) and the first `sinks` of those in front of it, with a rotary."""
+    `window` (0: all) and the first `sinks` of those in front of it, with a rotary.
+
+    With a rotary, the attention of prompts and drafts holds a probability as one 16-bit number (ops.paged_prompt_attention),
+    a step's as two, and a layer without one has its prompt's in fp32: outputs of the same text by different forms differ
+    by such roundings."""
 
     def __init__(self, hidden, heads, kv_heads, head_dim, mlp, eps=1e-6, dtype=torch.bfloat16, device=None, rotary=None, window=0, sinks=0):
         super().__init__()
@@ -117,7 +121,8 @@ class DecoderLayer(nn.Module):
 
     def prompt(self, x, h, cache, layer, seq, slots):
         """The newest tokens of a sequence, x [tokens, hidden], whose slots cache.extend gave.  h: the
-        residual stream (None in front of the first layer).  (x, h) for the next layer."""
+        residual stream (None in front of the first layer).  (x, h) for the next layer.  With a rotary each layer has the
+        cache make its prompts([seq], ...), copies to the device among it: prompts() takes one made once, and may be captured."""
         return self(x, h, cache, layer, slots, seq=seq)
 
     def prompts(self, x, h, cache, layer, slots, prompts, positions=None):

@@ -682,8 +682,8 @@ def rope_kv_write(q, k, v, positions, inv_freq, slots, k_cache, v_cache, k_scale
     types are converted on each call), the angle per position of each pair, pairs a multiple of 8; pair i is
     the elements i and i + pairs of a row, 2 i and 2 i + 1 when interleaved; elements from 2 * pairs on stay as
     they are.  positions: [tokens] int32 or int64, or [n, tokens] with axes, [pairs] int32: which of the n
-    positions (time, height and width, say) turns each pair.  Angles are worked out in
-    fp64; keys are turned in fp32 and quantized from there.
+    positions (time, height and width, say) turns each pair.  Angles are worked out in fp64 and sines in fp32 (off by at
+    most 2^-22 + 3 |angle| 2^-53); keys are turned in fp32 and quantized from there.
     """
     index = q.get_device()
     if index >= 0 and _timer is None and (direct := _native.direct()):
@@ -854,6 +854,8 @@ def paged_prompt_attention(q, k_cache, v_cache, block_table, starts, lengths, k_
     int32, the new tokens included.  A token sees those in front of it and itself; with a window, of these the last
     `window` and the first `sinks` of the sequence.  The cache, scale, max_len and return_lse (lse [tokens, heads]) as
     in paged_attention.
+    Scores, softmax statistics and sums are fp32; a probability meets its value as one 16-bit number, of q's type or bf16 on
+    codes, off by half a step as the output is (f16 rows on codes: as two; paged_attention: as two always).
     A row that sees a token whose page is outside the pool, or past the table, gets NaN.
     """
     if (index := q.get_device()) >= 0 and _timer is None and (direct := _native.direct()):

@@ -337,9 +337,10 @@ PSQ_API int psq_kv_write(int codes, const void *k, const void *v, int dtype, int
 /* psq_kv_write with the positions turned on the way: queries and keys are rotated by pairs, then keys and values
  * appended.  For pair i of a row, i < rotary / 2, elements (i, i + rotary / 2), or (2 i, 2 i + 1) with interleaved:
  *   t = position * inv_freq[i];  (a, b) <- (a cos t - b sin t, b cos t + a sin t)
- * elements past `rotary` stay as they are.  t is worked out in fp64 and its whole turns are dropped before it is rounded
- * (positions up to 2^31 lose nothing that fp32 sines would show); sines and products are fp32.  Queries are rounded once to their type; keys in a cache of codes are not rounded before
- * they are quantized (in a 16-bit one they are rounded once).
+ * elements past `rotary` stay as they are.  t is worked out in fp64 and its whole turns are dropped before it is rounded;
+ * sines and products are fp32: a sine is off by at most 2^-22 + 3 |t| 2^-53 (at |t| = 2^31 four times what it is up to
+ * 2^24).  Queries are rounded once to their type; keys in a cache of codes are not rounded before they are quantized (in a
+ * 16-bit one they are rounded once).
  *   q [T, Hq, D], k, v [T, Hkv, D] bf16/f16 (element strides as in psq_kv_write), q_out [T, Hq, D] dense
  *   positions: T integers of positions_bits (32 or 64), `axes` rows of them axis_stride elements apart;
  *   pair_axis [rotary / 2] int32: the axis whose position turns each pair (values outside 0 .. axes - 1: the
@@ -408,7 +409,7 @@ PSQ_API int psq_paged_attention_sinks(int codes, const void *q, int dtype, int64
  *   lengths [B] int32: each sequence's tokens, the new ones included (shorter than its rows: the rows in front
  *   of position 0 get zeros, lse -inf)
  * A row that sees a token whose page is outside the pool, or past its table, gets NaN.  A value that is not finite
- * reaches only the rows that see it.
+ * reaches only the rows that see it.  table_cols * page_size + T may be 2^31 - 256 at most.
  * max_len: about the longest length, for the number of workgroups (any value gives right results).
  * workspace: NULL (no sequence is split over its length), or memory of the call's own (any contents; the call makes two
  * launches then, and nothing else may write to it in between) of psq_paged_block_workspace_bytes() bytes, 256-byte
